@@ -190,6 +190,81 @@ MT_API int mt_nchw_to_nhwc(const mt_tensor* x, const mt_tensor* out, void* strea
 MT_API int mt_conv2d_wgrad_noalloc(const mt_tensor* dy, const mt_tensor* x, const mt_tensor* dw, uint64_t stride,
                                    uint64_t padding, int mode, void* stream);
 
+/* ---- low-bit forms of Linear, and the norm that makes its input ----------------------
+ * No counterpart in the reference, which holds everything in float. Activations, gradients
+ * and results stay float; 8 bits are a storage form of an activation (saved by the forward
+ * pass, read by the weight gradient), 4 bits one of a weight (for inference). All calls are
+ * deterministic. Outputs must not share memory with inputs unless a function says so. */
+
+enum { MT_Q8_INT8 = 0, MT_Q8_E4M3 = 1 };
+
+/* A rows x cols tensor in 8 bits. Blocks of 32 columns of a row (the last one shorter) share
+ * a scale byte b; a code c (int8, or an e4m3 float) stands for c * 2^(b - 127), and b = 255
+ * for NaN. Codes and scales have unit column stride. */
+typedef struct mt_q8 {
+    void* codes;          /* code (r, c) at codes + r * code_pitch + c */
+    uint8_t* scales;      /* scale of block j of row r at scales + r * scale_pitch + j */
+    uint64_t rows, cols;
+    uint64_t code_pitch;  /* bytes, >= cols */
+    uint64_t scale_pitch; /* bytes, >= ceil(cols / 32) */
+    int format;           /* MT_Q8_INT8 or MT_Q8_E4M3 */
+} mt_q8;
+
+/* A Linear weight [in, out] in 4 bits. Row n of the codes is column n of the weight: a code
+ * c = 0..15 stands for (c - 8) * scale, with one bfloat16 scale per `group` inputs. A row of
+ * codes is padded with code 8 to spans of 128 codes (64 bytes); the little-endian 32-bit
+ * word 4 t + b of a span (t, b = 0..3) holds the span's codes 32 b + 8 t + (0..7): code 2 i
+ * of these in bits 4 i .. 4 i + 3, code 2 i + 1 in bits 4 i + 16 .. 4 i + 19. */
+typedef struct mt_q4 {
+    void* codes;          /* row n at codes + n * code_pitch, 16-byte aligned */
+    void* scales;         /* bfloat16; scale of group g of row n at element n * scale_pitch + g */
+    uint64_t in, out;
+    uint64_t group;       /* 32, 64 or 128 */
+    uint64_t code_pitch;  /* bytes, a multiple of 16, >= 64 * ceil(in / 128) */
+    uint64_t scale_pitch; /* elements, >= ceil(in / group) */
+} mt_q4;
+
+/* h = x + residual; rstd = 1 / sqrt(mean(h^2) + eps) per row; y = h * rstd * gamma; q8 = y in
+ * 8 bits. x, residual, h, y are [rows, features] views, gamma [features], rstd [rows].
+ * residual, h, y, rstd and q8 may each be NULL (h then is x, or is not written). h may be the
+ * very view that x or residual is (the addition in place), and so may y; of q8, `format`
+ * says what to write. eps >= 0. */
+MT_API int mt_rms_norm(const mt_tensor* x, const mt_tensor* residual, const mt_tensor* gamma, const mt_tensor* h,
+                       const mt_tensor* y, const mt_tensor* rstd, const mt_q8* q8, float eps, void* stream);
+
+/* Gradients of mt_rms_norm from its h and rstd: dx = rstd * (g - xhat * mean(g * xhat)) + dh
+ * with g = dy * gamma and xhat = h * rstd (this is the gradient of x and of residual both),
+ * dgamma = the sum over rows of dy * xhat. dh, the gradient that reaches h from elsewhere,
+ * and dgamma may be NULL. dx may be the very view that dy or dh is. Takes scratch for
+ * dgamma's partial sums (one row of features per group of rows). */
+MT_API int mt_rms_norm_backward(const mt_tensor* dy, const mt_tensor* h, const mt_tensor* gamma,
+                                const mt_tensor* rstd, const mt_tensor* dh, const mt_tensor* dx,
+                                const mt_tensor* dgamma, void* stream);
+
+/* x [rows, cols] to 8 bits: per block the smallest scale that clips no code, each code
+ * rounded to nearest even. A block with an infinity or a NaN stands for NaN. */
+MT_API int mt_quantize_q8(const mt_tensor* x, const mt_q8* q, void* stream);
+
+enum { MT_F32 = 0, MT_BF16 = 1 };
+/* q's values to out, rows x cols with `pitch` elements between rows and unit column stride,
+ * type MT_F32 (exact) or MT_BF16 (exact too, but for e4m3 blocks below 2^-124 * 448). */
+MT_API int mt_dequantize_q8(const mt_q8* q, void* out, int type, uint64_t pitch, void* stream);
+
+/* Linear's weight and bias gradient with its input X [M, in] held in 8 bits: dW [in, out] =
+ * X^T dY and db [out] or [1, out] = the column sums of dY (NULL: not wanted), to the accuracy
+ * of a float product (there is no TF32 form). */
+MT_API int mt_linear_wgrad_q8(const mt_q8* x, const mt_tensor* dY, const mt_tensor* dW, const mt_tensor* db,
+                              void* stream);
+
+/* W [in, out] to 4 bits: scale = bf16(amax / 7) per group, code = round(w / scale) + 8. */
+MT_API int mt_quantize_q4(const mt_tensor* W, const mt_q4* q, void* stream);
+MT_API int mt_dequantize_q4(const mt_q4* q, const mt_tensor* W, void* stream);
+
+/* Y [M, out] = X [M, in] * W + bias (+ReLU) as mt_linear_fwd_gpu, W in 4 bits; to the accuracy
+ * of a float product. */
+MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor* bias, const mt_tensor* Y, int relu,
+                            void* stream);
+
 /* ---- general entry point ----------------------------------------------------------- */
 
 /* C = epi(A * B) for 2-D or 3-D (batched) views with an explicit mode. `bias` is a device

@@ -65,7 +65,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
     if not force and up_to_date():
         return LIB
     cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
-           "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
+           "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-t", "0",
            "-I", INCLUDE, "-I", CSRC, "-o", LIB + ".tmp", *sources()]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")

@@ -13,6 +13,7 @@
 
 #include "mtgemm.h"
 #include "mt_common.cuh"
+#include "mt_host.h"
 #include "simt_gemm.cuh"
 #include "umma_gemm.cuh"
 #include "umma_gemm2.cuh"
@@ -2238,9 +2239,50 @@ MT_API int mt_device_status(int reset) {
         int z = 0;
         cudaMemcpyToSymbol(mt::g_dev_status, &z, sizeof(int));
     }
-    return v;
+    const int lowbit = mt::host::lowbit_device_status(reset);
+    return v ? v : lowbit;
 }
 
 MT_API const char* mt_version(void) { return "minitensor_b200 mtgemm 0.1 (sm_100a)"; }
 
 }  // extern "C"
+
+// ---- services for the other translation units (mt_host.h) ---------------------------
+namespace mt {
+namespace host {
+
+int fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    t_err = buf;
+    return code;
+}
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+int launched(const char* what) {
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess && e != cudaErrorStreamCaptureUnsupported) return ::cuda_fail(e, what);
+    g_launches.fetch_add(1);
+    return MT_OK;
+}
+void set_path(const char* path) { t_path = path; }
+int sm_count() { return dev_info().sms; }
+int device_cc() { return dev_info().cc; }
+int scratch_alloc(void** p, size_t bytes, cudaStream_t st, const char* who) { return ::scratch_alloc(p, bytes, st, who); }
+void scratch_free(void* p, size_t bytes, cudaStream_t st) { ::scratch_free(p, bytes, st); }
+bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* d, const uint64_t* s, const uint32_t* b) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn || rank < 2 || rank > 3) return false;
+    cuuint64_t dims[3], strides[2];
+    cuuint32_t box[3], es[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) { dims[i] = d[i]; box[i] = b[i]; }
+    for (int i = 0; i + 1 < rank; ++i) strides[i] = s[i];
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace host
+}  // namespace mt

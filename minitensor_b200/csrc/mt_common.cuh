@@ -25,9 +25,8 @@ enum DevStatus : int {
     kDevBadLaunch = 7,        // launch shape disagrees with the kernel's parameters (no work done)
 };
 
-// Defined here: every kernel of the library is compiled in the single translation unit
-// mt_api.cu, so there is exactly one definition.
-__device__ int g_dev_status = 0;
+// One word per translation unit; mt_device_status reads and clears them all.
+static __device__ int g_dev_status = 0;
 
 // Wall-clock limit for one barrier wait. A legitimate wait in these kernels lasts
 // microseconds to a few milliseconds; after this the kernel reports and unwinds.

@@ -1,0 +1,534 @@
+// mt_lowbit.cu -- C entries of the low-bit operators (declared in include/mtgemm.h): argument
+// checks, choice of kernel and launches.
+#include <algorithm>
+
+#include "mtgemm.h"
+#include "mt_host.h"
+#include "lowbit_common.cuh"
+#include "q4.cuh"
+#include "q8.cuh"
+#include "q8_wgrad.cuh"
+#include "rms_norm.cuh"
+
+namespace {
+
+using mt::host::fail;
+using mt::host::launched;
+using mt::lowbit::Mat;
+using mt::lowbit::Q8;
+
+constexpr int64_t kMaxExtent = INT32_MAX;   // rows or features of one operand
+
+// A checked 2-D view; is1d: a vector, as one row.
+struct View2 {
+    Mat m{nullptr, 0, 0};
+    int64_t rows = 0, cols = 0;
+    bool given = false;
+};
+
+int to_mat(const mt_tensor* t, const char* who, const char* name, View2& v) {
+    if (!t) return fail(MT_EINVAL, "%s: %s is null", who, name);
+    if (t->ndim != 2) return fail(MT_EINVAL, "%s: %s must be 2-D, got %u-D", who, name, t->ndim);
+    if (t->shape[0] > (uint64_t)kMaxExtent || t->shape[1] > (uint64_t)kMaxExtent)
+        return fail(MT_EUNSUPPORTED, "%s: %s has an extent beyond 2^31", who, name);
+    v.rows = (int64_t)t->shape[0];
+    v.cols = (int64_t)t->shape[1];
+    if (v.rows * v.cols > 0 && !t->data) return fail(MT_EINVAL, "%s: %s has a null data pointer", who, name);
+    v.m = Mat{t->data ? t->data + t->offset : nullptr, (int64_t)t->strides[0], (int64_t)t->strides[1]};
+    v.given = true;
+    return MT_OK;
+}
+
+// A vector of n elements: [n], [1, n] or [n, 1].
+int to_vec(const mt_tensor* t, int64_t n, const char* who, const char* name, View2& v) {
+    if (!t) return fail(MT_EINVAL, "%s: %s is null", who, name);
+    uint64_t total = 1;
+    int64_t stride = 1;
+    int longer = 0;
+    for (uint32_t i = 0; i < t->ndim && i < MT_MAX_DIMS; ++i) {
+        total *= t->shape[i];
+        if (t->shape[i] != 1) { stride = (int64_t)t->strides[i]; ++longer; }
+    }
+    if (t->ndim < 1 || t->ndim > 2 || longer > 1 || (int64_t)total != n)
+        return fail(MT_EINVAL, "%s: %s must hold %lld elements in one dimension", who, name, (long long)n);
+    if (n > 0 && !t->data) return fail(MT_EINVAL, "%s: %s has a null data pointer", who, name);
+    v.m = Mat{t->data ? t->data + t->offset : nullptr, 0, stride};
+    v.rows = 1;
+    v.cols = n;
+    v.given = true;
+    return MT_OK;
+}
+
+// Byte ranges for the overlap check.
+struct Span {
+    uintptr_t lo, hi;   // [lo, hi)
+    int64_t pitch;      // bytes between rows of unit-stride columns, 0 if not of that form
+    int64_t width;      // bytes of such a row
+};
+Span span_of(const View2& v) {
+    Span s{0, 0, 0, 0};
+    if (!v.given || v.rows * v.cols == 0) return s;
+    s.lo = reinterpret_cast<uintptr_t>(v.m.p);
+    s.hi = s.lo + 4 * (uintptr_t)((v.rows - 1) * v.m.rs + (v.cols - 1) * v.m.cs + 1);
+    if (v.m.cs == 1 || v.cols == 1) { s.pitch = 4 * v.m.rs; s.width = 4 * v.cols; }
+    return s;
+}
+Span span_of_rows(const void* p, int64_t rows, int64_t pitch, int64_t width) {
+    Span s{0, 0, 0, 0};
+    if (!p || rows == 0 || width == 0) return s;
+    s.lo = reinterpret_cast<uintptr_t>(p);
+    s.hi = s.lo + (uintptr_t)((rows - 1) * pitch + width);
+    s.pitch = pitch;
+    s.width = width;
+    return s;
+}
+// Conservative: ranges that meet overlap, except disjoint column windows of one row pitch.
+bool overlap(const Span& a, const Span& b) {
+    if (a.lo >= a.hi || b.lo >= b.hi || a.hi <= b.lo || b.hi <= a.lo) return false;
+    if (a.pitch > 0 && a.pitch == b.pitch) {
+        const int64_t diff = (int64_t)(b.lo - a.lo);
+        const int64_t d = ((diff % a.pitch) + a.pitch) % a.pitch;
+        if (d >= a.width && d + b.width <= a.pitch) return false;
+    }
+    return true;
+}
+bool same_view(const View2& a, const View2& b) {
+    return a.given && b.given && a.m.p == b.m.p && a.rows == b.rows && a.cols == b.cols &&
+           (a.rows <= 1 || a.m.rs == b.m.rs) && (a.cols <= 1 || a.m.cs == b.m.cs);
+}
+// An output whose elements are all different memory.
+int check_distinct(const View2& v, const char* who, const char* name) {
+    if (!v.given || v.rows * v.cols <= 1) return MT_OK;
+    const int64_t rs = v.rows > 1 ? v.m.rs : INT64_MAX / 2, cs = v.cols > 1 ? v.m.cs : INT64_MAX / 2;
+    const bool by_row = v.rows <= 1 || (cs > 0 && (v.cols <= 1 || rs > (v.cols - 1) * cs));
+    const bool by_col = v.cols <= 1 || (rs > 0 && (v.rows <= 1 || cs > (v.rows - 1) * rs));
+    if (rs <= 0 || cs <= 0 || !(by_row || by_col))
+        return fail(MT_EINVAL, "%s: %s is an output with overlapping or broadcast elements", who, name);
+    return MT_OK;
+}
+int check_apart(const Span& out, const char* out_name, const Span& in, const char* in_name, const char* who) {
+    if (overlap(out, in)) return fail(MT_EINVAL, "%s: %s and %s share memory", who, out_name, in_name);
+    return MT_OK;
+}
+
+int64_t blocks_of(int64_t cols) { return (cols + mt::lowbit::kBlock - 1) / mt::lowbit::kBlock; }
+
+int to_q8(const mt_q8* q, const char* who, Q8& o, int64_t& rows, int64_t& cols) {
+    if (!q) return fail(MT_EINVAL, "%s: the 8-bit tensor is null", who);
+    if (q->format != MT_Q8_INT8 && q->format != MT_Q8_E4M3) return fail(MT_EINVAL, "%s: bad 8-bit format %d", who, q->format);
+    if (q->rows > (uint64_t)kMaxExtent || q->cols > (uint64_t)kMaxExtent)
+        return fail(MT_EUNSUPPORTED, "%s: the 8-bit tensor has an extent beyond 2^31", who);
+    rows = (int64_t)q->rows;
+    cols = (int64_t)q->cols;
+    if (rows * cols > 0 && (!q->codes || !q->scales)) return fail(MT_EINVAL, "%s: the 8-bit tensor has a null pointer", who);
+    if (rows > 1 && (q->code_pitch < q->cols || q->scale_pitch < (uint64_t)blocks_of(cols)))
+        return fail(MT_EINVAL, "%s: the 8-bit tensor's pitch is smaller than a row", who);
+    if (q->code_pitch > (1ull << 40) || q->scale_pitch > (1ull << 40))
+        return fail(MT_EINVAL, "%s: the 8-bit tensor's pitch is out of range", who);
+    o = Q8{static_cast<uint8_t*>(q->codes), q->scales, (int64_t)q->code_pitch, (int64_t)q->scale_pitch, q->format};
+    return MT_OK;
+}
+Span code_span(const Q8& q, int64_t rows, int64_t cols) { return span_of_rows(q.codes, rows, q.cp, cols); }
+Span scale_span(const Q8& q, int64_t rows, int64_t cols) { return span_of_rows(q.scales, rows, q.sp, blocks_of(cols)); }
+
+int to_q4(const mt_q4* q, const char* who, mt::q4::Weight& o) {
+    if (!q) return fail(MT_EINVAL, "%s: the 4-bit weight is null", who);
+    if (q->group != 32 && q->group != 64 && q->group != 128)
+        return fail(MT_EINVAL, "%s: group must be 32, 64 or 128, got %llu", who, (unsigned long long)q->group);
+    if (q->in > (uint64_t)kMaxExtent - 127 || q->out > (uint64_t)kMaxExtent)
+        return fail(MT_EUNSUPPORTED, "%s: the 4-bit weight has an extent beyond 2^31", who);
+    const uint64_t spans = (q->in + 127) / 128, groups = (q->in + q->group - 1) / q->group;
+    if (q->in * q->out > 0) {
+        if (!q->codes || !q->scales) return fail(MT_EINVAL, "%s: the 4-bit weight has a null pointer", who);
+        if ((reinterpret_cast<uintptr_t>(q->codes) & 15) || q->code_pitch % 16)
+            return fail(MT_EINVAL, "%s: rows of 4-bit codes must start on 16-byte boundaries", who);
+        if (reinterpret_cast<uintptr_t>(q->scales) & 1) return fail(MT_EINVAL, "%s: misaligned 4-bit scales", who);
+        if (q->code_pitch < 64 * spans || q->scale_pitch < groups)
+            return fail(MT_EINVAL, "%s: the 4-bit weight's pitch is smaller than a row", who);
+        if (q->code_pitch > (1ull << 40) || q->scale_pitch > (1ull << 40))
+            return fail(MT_EINVAL, "%s: the 4-bit weight's pitch is out of range", who);
+    }
+    o = mt::q4::Weight{static_cast<uint32_t*>(q->codes), static_cast<__nv_bfloat16*>(q->scales),
+                       (int64_t)q->code_pitch / 4, (int64_t)q->scale_pitch, (int64_t)q->in, (int64_t)q->out,
+                       (int)q->group};
+    return MT_OK;
+}
+Span q4_code_span(const mt::q4::Weight& q) { return span_of_rows(q.codes, q.K ? q.N : 0, 4 * q.cp, (q.K + 127) / 128 * 64); }
+Span q4_scale_span(const mt::q4::Weight& q) {
+    return span_of_rows(q.scales, q.K ? q.N : 0, 2 * q.sp, 2 * ((q.K + q.group - 1) / q.group));
+}
+
+// Rows of unit stride that start on 16-byte boundaries.
+bool vec4(const View2& v) {
+    if (!v.given) return true;
+    return v.m.cs == 1 && (reinterpret_cast<uintptr_t>(v.m.p) & 15) == 0 && (v.rows <= 1 || v.m.rs % 4 == 0);
+}
+
+unsigned grid_of(int64_t n, int64_t most) { return (unsigned)std::max<int64_t>(1, std::min(n, most)); }
+
+#define MT_TRY(expr)                  \
+    do {                              \
+        const int rc_ = (expr);       \
+        if (rc_ != MT_OK) return rc_; \
+    } while (0)
+
+// ------------------------------------- RMS norm ---------------------------------------
+
+// Largest row held in registers: 32 warps x V = 8 pieces of 32 lanes x VEC features.
+constexpr int64_t kRowPieces = 32 * 8 * 32;
+
+template <int VEC, int V, int WPR, int RPC>
+int launch_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
+    const int64_t ctas = (p.rows + RPC - 1) / RPC;
+    mt::rms::fwd_kernel<VEC, V, WPR, RPC><<<grid_of(ctas, INT32_MAX), 32 * WPR * RPC, 0, st>>>(p);
+    return launched("rms_norm launch");
+}
+
+// Warps per row and pieces per lane by the row's length. Rows that are too few to fill the
+// GPU take more warps each.
+template <int VEC>
+int run_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
+    const int64_t pieces = (p.K + 32 * VEC - 1) / (32 * VEC);
+    const bool few = p.rows <= 2 * mt::host::sm_count();
+    if (pieces <= 4) return launch_fwd<VEC, 4, 1, 4>(p, st);
+    if (few && pieces <= 32) return launch_fwd<VEC, 1, 32, 1>(p, st);
+    if (pieces <= 32) return launch_fwd<VEC, 4, 8, 1>(p, st);
+    if (pieces <= 128) return launch_fwd<VEC, 4, 32, 1>(p, st);
+    return launch_fwd<VEC, 8, 32, 1>(p, st);
+}
+
+// Row groups whose dgamma partials are kept; the launch has one per CTA (or warp, RPC > 1).
+template <int VEC, int V, int WPR, int RPC>
+int64_t bwd_groups(int64_t rows) {
+    const int per_sm = std::max(1, 1024 / (32 * WPR * RPC));
+    const int64_t ctas = std::min<int64_t>((rows + RPC - 1) / RPC, (int64_t)mt::host::sm_count() * per_sm);
+    return ctas * RPC;
+}
+template <int VEC, int V, int WPR, int RPC>
+int launch_bwd(const mt::rms::Bwd& p, int64_t groups, cudaStream_t st) {
+    mt::rms::bwd_kernel<VEC, V, WPR, RPC><<<(unsigned)(groups / RPC), 32 * WPR * RPC, 0, st>>>(p);
+    return launched("rms_norm_backward launch");
+}
+
+// Calls f with the variant for the row length as template arguments.
+template <int VEC, typename F>
+int with_bwd_variant(int64_t K, F&& f) {
+    const int64_t pieces = (K + 32 * VEC - 1) / (32 * VEC);
+    if (pieces <= 4) return f.template run<VEC, 4, 1, 4>();
+    if (pieces <= 32) return f.template run<VEC, 4, 8, 1>();
+    if (pieces <= 128) return f.template run<VEC, 4, 32, 1>();
+    return f.template run<VEC, 8, 32, 1>();
+}
+struct GroupsOf {
+    int64_t rows, *out;
+    template <int VEC, int V, int WPR, int RPC> int run() { *out = bwd_groups<VEC, V, WPR, RPC>(rows); return MT_OK; }
+};
+struct LaunchBwd {
+    const mt::rms::Bwd& p;
+    int64_t groups;
+    cudaStream_t st;
+    template <int VEC, int V, int WPR, int RPC> int run() { return launch_bwd<VEC, V, WPR, RPC>(p, groups, st); }
+};
+
+}  // namespace
+
+extern "C" {
+
+MT_API int mt_rms_norm(const mt_tensor* x, const mt_tensor* residual, const mt_tensor* gamma, const mt_tensor* h,
+                       const mt_tensor* y, const mt_tensor* rstd, const mt_q8* q8, float eps, void* stream) {
+    const char* who = "rms_norm";
+    View2 vx, vr, vg, vh, vy, vs;
+    Q8 q{nullptr, nullptr, 0, 0, 0};
+    MT_TRY(to_mat(x, who, "x", vx));
+    const int64_t M = vx.rows, K = vx.cols;
+    if (K == 0) return fail(MT_EINVAL, "%s: rows of no features have no mean", who);
+    MT_TRY(to_vec(gamma, K, who, "gamma", vg));
+    if (residual) MT_TRY(to_mat(residual, who, "residual", vr));
+    if (h) MT_TRY(to_mat(h, who, "h", vh));
+    if (y) MT_TRY(to_mat(y, who, "y", vy));
+    if (rstd) MT_TRY(to_vec(rstd, M, who, "rstd", vs));
+    for (const View2* v : {&vr, &vh, &vy})
+        if (v->given && (v->rows != M || v->cols != K))
+            return fail(MT_EINVAL, "%s: residual, h and y must have x's shape [%lld, %lld]", who, (long long)M, (long long)K);
+    if (!(eps >= 0.f)) return fail(MT_EINVAL, "%s: eps must not be negative", who);
+    Span sq{0, 0, 0, 0}, ss{0, 0, 0, 0};
+    if (q8) {
+        int64_t qr, qc;
+        MT_TRY(to_q8(q8, who, q, qr, qc));
+        if (qr != M || qc != K) return fail(MT_EINVAL, "%s: the 8-bit output must have x's shape", who);
+        sq = code_span(q, M, K);
+        ss = scale_span(q, M, K);
+    }
+    if (!h && !y && !rstd && !q8) return fail(MT_EINVAL, "%s: no output is wanted", who);
+    MT_TRY(check_distinct(vh, who, "h"));
+    MT_TRY(check_distinct(vy, who, "y"));
+    MT_TRY(check_distinct(vs, who, "rstd"));
+    const Span in[] = {span_of(vx), span_of(vr), span_of(vg)};
+    const Span out[] = {span_of(vh), span_of(vy), span_of(vs), sq, ss};
+    const View2 *vin[] = {&vx, &vr, &vg}, *vout[] = {&vh, &vy, nullptr, nullptr, nullptr};
+    for (int o = 0; o < 5; ++o) {
+        for (int i = 0; i < 3; ++i)
+            if (!(i < 2 && vout[o] && same_view(*vout[o], *vin[i])) && overlap(out[o], in[i]))
+                return fail(MT_EINVAL, "%s: an output shares memory with an input", who);
+        for (int p = 0; p < o; ++p)
+            if (overlap(out[o], out[p])) return fail(MT_EINVAL, "%s: two outputs share memory", who);
+    }
+    if (M == 0) return MT_OK;
+    mt::rms::Fwd p{vx.m, vr.m, vg.m, vh.m, vy.m, vs.m, q, M, K, eps};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool vec = K % 4 == 0 && vec4(vx) && vec4(vr) && vec4(vg) && vec4(vh) && vec4(vy) &&
+                     (!q8 || ((reinterpret_cast<uintptr_t>(q.codes) & 3) == 0 && (M == 1 || q.cp % 4 == 0)));
+    int rc;
+    if (K > kRowPieces * (vec ? 4 : 1)) {
+        mt::rms::fwd_long_kernel<<<grid_of(M, INT32_MAX), 32 * mt::rms::kLongWarps, 0, st>>>(p);
+        rc = launched("rms_norm launch");
+        if (rc == MT_OK) mt::host::set_path("rms_norm long rows");
+        return rc;
+    }
+    rc = vec ? run_fwd<4>(p, st) : run_fwd<1>(p, st);
+    if (rc == MT_OK) mt::host::set_path(vec ? "rms_norm vec=4" : "rms_norm vec=1");
+    return rc;
+}
+
+MT_API int mt_rms_norm_backward(const mt_tensor* dy, const mt_tensor* h, const mt_tensor* gamma,
+                                const mt_tensor* rstd, const mt_tensor* dh, const mt_tensor* dx,
+                                const mt_tensor* dgamma, void* stream) {
+    const char* who = "rms_norm_backward";
+    View2 vdy, vh, vg, vs, vdh, vdx, vdg;
+    MT_TRY(to_mat(dy, who, "dy", vdy));
+    const int64_t M = vdy.rows, K = vdy.cols;
+    if (K == 0) return fail(MT_EINVAL, "%s: rows of no features have no mean", who);
+    MT_TRY(to_mat(h, who, "h", vh));
+    MT_TRY(to_vec(gamma, K, who, "gamma", vg));
+    MT_TRY(to_vec(rstd, M, who, "rstd", vs));
+    if (dh) MT_TRY(to_mat(dh, who, "dh", vdh));
+    MT_TRY(to_mat(dx, who, "dx", vdx));
+    if (dgamma) MT_TRY(to_vec(dgamma, K, who, "dgamma", vdg));
+    for (const View2* v : {&vh, &vdh, &vdx})
+        if (v->given && (v->rows != M || v->cols != K))
+            return fail(MT_EINVAL, "%s: h, dh and dx must have dy's shape [%lld, %lld]", who, (long long)M, (long long)K);
+    MT_TRY(check_distinct(vdx, who, "dx"));
+    MT_TRY(check_distinct(vdg, who, "dgamma"));
+    const View2* in[] = {&vdy, &vdh, &vh, &vg, &vs};
+    for (int i = 0; i < 5; ++i) {
+        if (!(i < 2 && same_view(vdx, *in[i])) && overlap(span_of(vdx), span_of(*in[i])))
+            return fail(MT_EINVAL, "%s: dx shares memory with an input", who);
+        if (overlap(span_of(vdg), span_of(*in[i]))) return fail(MT_EINVAL, "%s: dgamma shares memory with an input", who);
+    }
+    MT_TRY(check_apart(span_of(vdx), "dx", span_of(vdg), "dgamma", who));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    mt::rms::Bwd p{vdy.m, vh.m, vg.m, vs.m, vdh.m, vdx.m, nullptr, M, K};
+    const bool vec = K % 4 == 0 && vec4(vdy) && vec4(vh) && vec4(vg) && vec4(vdh) && vec4(vdx);
+    const bool is_long = K > kRowPieces * (vec ? 4 : 1);
+    int64_t groups = 0;
+    if (is_long) {
+        groups = std::min<int64_t>(M, std::max<int64_t>(1, 8LL * mt::host::sm_count() * 256 / K));
+    } else {
+        MT_TRY(vec ? with_bwd_variant<4>(K, GroupsOf{M, &groups}) : with_bwd_variant<1>(K, GroupsOf{M, &groups}));
+    }
+    void* ws = nullptr;
+    const size_t bytes = dgamma ? (size_t)groups * K * sizeof(float) : 0;
+    MT_TRY(mt::host::scratch_alloc(&ws, bytes, st, who));
+    p.part = static_cast<float*>(ws);
+    int rc = MT_OK;
+    if (M > 0) {
+        if (is_long) {
+            if (p.part) {
+                mt::rms::dgamma_long_kernel<<<dim3((unsigned)((K + 255) / 256), (unsigned)groups), 256, 0, st>>>(p);
+                rc = launched("rms_norm_backward dgamma launch");
+            }
+            if (rc == MT_OK) {
+                mt::rms::bwd_long_kernel<<<grid_of(M, INT32_MAX), 32 * mt::rms::kLongWarps, 0, st>>>(p);
+                rc = launched("rms_norm_backward launch");
+            }
+        } else {
+            rc = vec ? with_bwd_variant<4>(K, LaunchBwd{p, groups, st}) : with_bwd_variant<1>(K, LaunchBwd{p, groups, st});
+        }
+    }
+    if (rc == MT_OK && dgamma) {
+        mt::rms::sum_parts_kernel<<<(unsigned)((K + 31) / 32), dim3(32, 8), 0, st>>>(p.part, groups, K, vdg.m);
+        rc = launched("rms_norm_backward dgamma sum launch");
+    }
+    mt::host::scratch_free(ws, bytes, st);
+    if (rc == MT_OK)
+        mt::host::set_path(is_long ? "rms_norm_backward long rows" : vec ? "rms_norm_backward vec=4" : "rms_norm_backward vec=1");
+    return rc;
+}
+
+MT_API int mt_quantize_q8(const mt_tensor* x, const mt_q8* q, void* stream) {
+    const char* who = "quantize_q8";
+    View2 vx;
+    Q8 o;
+    int64_t M, K;
+    MT_TRY(to_mat(x, who, "x", vx));
+    MT_TRY(to_q8(q, who, o, M, K));
+    if (vx.rows != M || vx.cols != K) return fail(MT_EINVAL, "%s: the 8-bit tensor must have x's shape", who);
+    MT_TRY(check_apart(code_span(o, M, K), "the codes", span_of(vx), "x", who));
+    MT_TRY(check_apart(scale_span(o, M, K), "the scales", span_of(vx), "x", who));
+    MT_TRY(check_apart(code_span(o, M, K), "the codes", scale_span(o, M, K), "the scales", who));
+    if (M * K == 0) return MT_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool vec = K % 4 == 0 && vec4(vx) && (reinterpret_cast<uintptr_t>(o.codes) & 3) == 0 && (M == 1 || o.cp % 4 == 0);
+    const int64_t width = 32 * (vec ? 4 : 1) * mt::q8::kWarps;
+    const dim3 grid((unsigned)((K + width - 1) / width), grid_of((M + mt::q8::kRows - 1) / mt::q8::kRows, 65535));
+    if (vec) mt::q8::quantize_kernel<4><<<grid, 32 * mt::q8::kWarps, 0, st>>>(vx.m, o, M, K);
+    else mt::q8::quantize_kernel<1><<<grid, 32 * mt::q8::kWarps, 0, st>>>(vx.m, o, M, K);
+    MT_TRY(launched("quantize_q8 launch"));
+    mt::host::set_path(vec ? "quantize_q8 vec=4" : "quantize_q8 vec=1");
+    return MT_OK;
+}
+
+MT_API int mt_dequantize_q8(const mt_q8* q, void* out, int type, uint64_t pitch, void* stream) {
+    const char* who = "dequantize_q8";
+    Q8 o;
+    int64_t M, K;
+    MT_TRY(to_q8(q, who, o, M, K));
+    if (type != MT_F32 && type != MT_BF16) return fail(MT_EINVAL, "%s: bad output type %d", who, type);
+    if (M * K == 0) return MT_OK;
+    if (!out) return fail(MT_EINVAL, "%s: null output", who);
+    const int es = type == MT_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(out) % es) return fail(MT_EINVAL, "%s: misaligned output", who);
+    if ((M > 1 && pitch < (uint64_t)K) || pitch > (1ull << 40)) return fail(MT_EINVAL, "%s: the output's pitch is smaller than a row or out of range", who);
+    const Span so = span_of_rows(out, M, (int64_t)pitch * es, K * es);
+    MT_TRY(check_apart(so, "the output", code_span(o, M, K), "the codes", who));
+    MT_TRY(check_apart(so, "the output", scale_span(o, M, K), "the scales", who));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto al16 = [](const void* p, int64_t pitch_bytes, int64_t rows) {
+        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || pitch_bytes % 16 == 0);
+    };
+    const bool vec = K % 16 == 0 && al16(o.codes, o.cp, M) && al16(out, (int64_t)pitch * es, M);
+    const int64_t width = 256 * (vec ? 16 : 1);
+    const dim3 grid((unsigned)((K + width - 1) / width), grid_of(M, 65535));
+    if (type == MT_F32) {
+        float* f = static_cast<float*>(out);
+        if (vec) mt::q8::dequantize_kernel<float, 16><<<grid, 256, 0, st>>>(o, f, (int64_t)pitch, M, K);
+        else mt::q8::dequantize_kernel<float, 1><<<grid, 256, 0, st>>>(o, f, (int64_t)pitch, M, K);
+    } else {
+        __nv_bfloat16* f = static_cast<__nv_bfloat16*>(out);
+        if (vec) mt::q8::dequantize_kernel<__nv_bfloat16, 16><<<grid, 256, 0, st>>>(o, f, (int64_t)pitch, M, K);
+        else mt::q8::dequantize_kernel<__nv_bfloat16, 1><<<grid, 256, 0, st>>>(o, f, (int64_t)pitch, M, K);
+    }
+    MT_TRY(launched("dequantize_q8 launch"));
+    mt::host::set_path(vec ? "dequantize_q8 vec=16" : "dequantize_q8 vec=1");
+    return MT_OK;
+}
+
+MT_API int mt_linear_wgrad_q8(const mt_q8* x, const mt_tensor* dY, const mt_tensor* dW, const mt_tensor* db,
+                              void* stream) {
+    const char* who = "linear_wgrad_q8";
+    Q8 q;
+    int64_t M, K;
+    View2 vdy, vdw, vdb;
+    MT_TRY(to_q8(x, who, q, M, K));
+    MT_TRY(to_mat(dY, who, "dY", vdy));
+    MT_TRY(to_mat(dW, who, "dW", vdw));
+    const int64_t N = vdy.cols;
+    if (vdy.rows != M)
+        return fail(MT_EINVAL, "%s: dY has %lld rows, the 8-bit input %lld", who, (long long)vdy.rows, (long long)M);
+    if (vdw.rows != K || vdw.cols != N)
+        return fail(MT_EINVAL, "%s: dW must be [%lld, %lld]", who, (long long)K, (long long)N);
+    if (db) MT_TRY(to_vec(db, N, who, "db", vdb));
+    MT_TRY(check_distinct(vdw, who, "dW"));
+    MT_TRY(check_distinct(vdb, who, "db"));
+    for (const View2* o : {&vdw, &vdb}) {
+        MT_TRY(check_apart(span_of(*o), "an output", span_of(vdy), "dY", who));
+        MT_TRY(check_apart(span_of(*o), "an output", code_span(q, M, K), "the codes", who));
+        MT_TRY(check_apart(span_of(*o), "an output", scale_span(q, M, K), "the scales", who));
+    }
+    MT_TRY(check_apart(span_of(vdw), "dW", span_of(vdb), "db", who));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (N == 0) return MT_OK;
+    if (K > 0) {
+        const int64_t ty = (K + mt::wgrad8::T - 1) / mt::wgrad8::T;
+        if (ty > 65535) return fail(MT_EUNSUPPORTED, "%s: too many input features", who);
+        mt::wgrad8::simple_kernel<<<dim3((unsigned)((N + mt::wgrad8::T - 1) / mt::wgrad8::T), (unsigned)ty), 256, 0, st>>>(
+            q, vdy.m, vdw.m, M, K, N);
+        MT_TRY(launched("linear_wgrad_q8 launch"));
+    }
+    if (db) MT_TRY(mt_sum_rows_gpu(dY, db, stream));
+    mt::host::set_path("linear_wgrad_q8 simple");
+    return MT_OK;
+}
+
+MT_API int mt_quantize_q4(const mt_tensor* W, const mt_q4* q, void* stream) {
+    const char* who = "quantize_q4";
+    View2 vw;
+    mt::q4::Weight o;
+    MT_TRY(to_mat(W, who, "W", vw));
+    MT_TRY(to_q4(q, who, o));
+    if (vw.rows != o.K || vw.cols != o.N) return fail(MT_EINVAL, "%s: W must be [%lld, %lld]", who, (long long)o.K, (long long)o.N);
+    MT_TRY(check_apart(q4_code_span(o), "the codes", span_of(vw), "W", who));
+    MT_TRY(check_apart(q4_scale_span(o), "the scales", span_of(vw), "W", who));
+    MT_TRY(check_apart(q4_code_span(o), "the codes", q4_scale_span(o), "the scales", who));
+    if (o.K * o.N == 0) return MT_OK;
+    const int64_t spans = (o.K + mt::q4::kSpan - 1) / mt::q4::kSpan;
+    mt::q4::quantize_kernel<<<dim3((unsigned)((o.N + 127) / 128), grid_of(spans, 65535)), 128, 0,
+                              static_cast<cudaStream_t>(stream)>>>(vw.m, o, spans);
+    MT_TRY(launched("quantize_q4 launch"));
+    mt::host::set_path("quantize_q4");
+    return MT_OK;
+}
+
+MT_API int mt_dequantize_q4(const mt_q4* q, const mt_tensor* W, void* stream) {
+    const char* who = "dequantize_q4";
+    View2 vw;
+    mt::q4::Weight o;
+    MT_TRY(to_q4(q, who, o));
+    MT_TRY(to_mat(W, who, "W", vw));
+    if (vw.rows != o.K || vw.cols != o.N) return fail(MT_EINVAL, "%s: W must be [%lld, %lld]", who, (long long)o.K, (long long)o.N);
+    MT_TRY(check_distinct(vw, who, "W"));
+    MT_TRY(check_apart(span_of(vw), "W", q4_code_span(o), "the codes", who));
+    MT_TRY(check_apart(span_of(vw), "W", q4_scale_span(o), "the scales", who));
+    if (o.K * o.N == 0) return MT_OK;
+    mt::q4::dequantize_kernel<<<dim3((unsigned)((o.N + 127) / 128), grid_of((o.K + 7) / 8, 65535)), 128, 0,
+                                static_cast<cudaStream_t>(stream)>>>(o, vw.m);
+    MT_TRY(launched("dequantize_q4 launch"));
+    mt::host::set_path("dequantize_q4");
+    return MT_OK;
+}
+
+MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor* bias, const mt_tensor* Y, int relu,
+                            void* stream) {
+    const char* who = "linear_fwd_q4";
+    View2 vx, vb, vy;
+    mt::q4::Weight w;
+    MT_TRY(to_mat(X, who, "X", vx));
+    MT_TRY(to_q4(W, who, w));
+    MT_TRY(to_mat(Y, who, "Y", vy));
+    if (vx.cols != w.K)
+        return fail(MT_EINVAL, "%s: x features (%lld) != weight in (%lld)", who, (long long)vx.cols, (long long)w.K);
+    if (vy.rows != vx.rows || vy.cols != w.N) return fail(MT_EINVAL, "%s: Y shape mismatch", who);
+    if (bias) {
+        MT_TRY(to_vec(bias, w.N, who, "bias", vb));
+        if (w.N > 1 && vb.m.cs != 1) return fail(MT_EINVAL, "%s: bias must be contiguous", who);
+    }
+    MT_TRY(check_distinct(vy, who, "Y"));
+    const Span in[] = {span_of(vx), span_of(vb), q4_code_span(w), q4_scale_span(w)};
+    const char* names[] = {"X", "bias", "the codes", "the scales"};
+    for (int i = 0; i < 4; ++i) MT_TRY(check_apart(span_of(vy), "Y", in[i], names[i], who));
+    const int64_t M = vx.rows;
+    if (M * w.N == 0) return MT_OK;
+    mt::q4::linear_simple_kernel<<<dim3((unsigned)((w.N + 7) / 8), grid_of((M + 3) / 4, 65535)), 256, 0,
+                                   static_cast<cudaStream_t>(stream)>>>(vx.m, w, vb.m.p, vy.m, M, relu);
+    MT_TRY(launched("linear_fwd_q4 launch"));
+    mt::host::set_path("linear_fwd_q4 simple");
+    return MT_OK;
+}
+
+}  // extern "C"
+
+namespace mt {
+namespace host {
+
+int lowbit_device_status(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_dev_status, sizeof(int)) != cudaSuccess) return -MT_ECUDA;
+    if (reset) {
+        const int z = 0;
+        cudaMemcpyToSymbol(g_dev_status, &z, sizeof(int));
+    }
+    return v;
+}
+
+}  // namespace host
+}  // namespace mt

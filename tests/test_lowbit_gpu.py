@@ -1,0 +1,451 @@
+"""The low-bit operators on the GPU against their plain 64-bit forms (tests/lowbit_ref.py)."""
+import pytest
+import torch
+
+import lowbit_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mt(eng):
+    import minitensor_b200
+    return minitensor_b200
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rand(g, *shape, scale=1.0):
+    return torch.randn(*shape, generator=g) * scale
+
+
+def host(t):
+    return t.detach().cpu()
+
+
+def strided(t, how):
+    """The same values on the GPU in another layout."""
+    rows, cols = t.shape
+    if how == "dense":
+        return t.cuda()
+    if how == "transposed":
+        return t.t().contiguous().cuda().t()
+    if how == "window":        # a column window of a wider buffer, off the 16-byte grid
+        base = torch.full((rows, cols + 7), float("nan"), device="cuda")
+        base[:, 3:3 + cols] = t.cuda()
+        return base[:, 3:3 + cols]
+    if how == "every second":
+        base = torch.full((2 * rows, 2 * cols), float("nan"), device="cuda")
+        base[::2, ::2] = t.cuda()
+        return base[::2, ::2]
+    if how == "pitched":       # 16-byte rows with a pitch
+        base = torch.full((rows, cols + 8), float("nan"), device="cuda")
+        base[:, :cols] = t.cuda()
+        return base[:, :cols]
+    raise AssertionError(how)
+
+
+LAYOUTS = ["dense", "transposed", "window", "every second", "pitched"]
+
+# ---- RMS norm ---------------------------------------------------------------------------
+# y = h * rstd * gamma. With s terms per lane and ten shuffle or shared-memory levels, the sum
+# of squares is off by at most (s + 10) u, half of which reaches rstd; squares, the division by
+# K, the addition of eps, the square root, the division and two products add at most 6 u, and
+# h's own rounding, where a residual is added, u of itself and u of the row's root mean
+# square. s <= 32 in registers, K / 1024 in rows longer than that.
+
+def norm_bound(K):
+    return 0.5 * (max(32, K / 1024) + 10) + 10
+
+
+SHAPES = [(1, 1), (1, 4096), (3, 5), (5, 32), (2, 33), (7, 100), (9, 128), (300, 127), (4, 512), (130, 516), (3, 1000),
+          (3, 1024), (2, 1025), (5, 4100), (320, 1028), (2, 4097), (2, 8191), (3, 16384), (2, 20000), (1, 32768), (2, 8193),
+          (2, 40004), (1, 70001)]
+
+
+@pytest.mark.parametrize("rows,K", SHAPES)
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_rms_norm(mt, rows, K, with_residual):
+    g = gen(rows * 100003 + K)
+    x, gamma = rand(g, rows, K), 1 + rand(g, K, scale=0.1)
+    r = rand(g, rows, K, scale=3.0) if with_residual else None
+    out = mt.rms_norm(x.cuda(), gamma.cuda(), residual=r.cuda() if with_residual else None, eps=1e-6)
+    h, rstd, y = R.rms_norm(x, r, gamma, 1e-6)
+    if with_residual:
+        assert torch.equal(host(out.h), x + r)
+    assert out.q8 is None
+    b = norm_bound(K)
+    assert R.worst(host(out.rstd) - rstd, rstd) <= b
+    # the rounding of h is relative to h itself
+    assert R.worst(host(out.y) - y, y) <= b + 1
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("rows,K", [(6, 96), (5, 1028), (3, 130)])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_rms_norm_layouts(mt, layout, rows, K, fmt):
+    g = gen(K)
+    x, r, gamma = rand(g, rows, K), rand(g, rows, K), 1 + rand(g, K, scale=0.1)
+    dense = mt.rms_norm(x.cuda(), gamma.cuda(), residual=r.cuda(), q8=fmt)
+    out = mt.rms_norm(strided(x, layout), gamma.cuda(), residual=strided(r, layout), q8=fmt)
+    h, rstd, y = R.rms_norm(x, r, gamma, 1e-6)
+    assert R.worst(host(out.y) - y, y) <= norm_bound(K) + 1
+    assert torch.equal(out.h, dense.h)
+    # the 8-bit output is exactly the 8-bit form of the float output
+    q = mt.quantize_q8(out.y, fmt)
+    assert torch.equal(q.codes.view(torch.uint8), out.q8.codes.view(torch.uint8))
+    assert torch.equal(q.scales, out.q8.scales)
+
+
+@pytest.mark.parametrize("K", [64, 100, 4096, 40004])
+def test_rms_norm_in_place_and_8_bit_output_alone(mt, K):
+    g = gen(K)
+    x, r, gamma = rand(g, 5, K), rand(g, 5, K), 1 + rand(g, K, scale=0.1)
+    ref = mt.rms_norm(x.cuda(), gamma.cuda(), residual=r.cuda(), q8="int8")
+    xd = x.cuda()
+    out = mt.rms_norm(xd, gamma.cuda(), residual=r.cuda(), q8="int8", want_y=False, inplace=True)
+    assert out.y is None and out.h is xd
+    assert torch.equal(xd, ref.h) and torch.equal(out.q8.codes, ref.q8.codes) and torch.equal(out.rstd, ref.rstd)
+
+
+def test_rms_norm_special_rows(mt):
+    K = 200
+    x = torch.ones(5, K)
+    x[0] = 0                      # all zeros: eps alone
+    x[1, 7] = float("nan")
+    x[2, 9] = float("inf")
+    x[3] = 1e-30                  # squares underflow: eps alone
+    gamma = torch.ones(K)
+    out = mt.rms_norm(x.cuda(), gamma.cuda(), eps=1e-6, q8="int8")
+    y = host(out.y)
+    assert torch.equal(y[0], torch.zeros(K))
+    assert torch.isnan(y[1]).all()
+    assert torch.isnan(y[2, 9]) and torch.equal(y[2, :9], torch.zeros(9))
+    assert R.worst(y[3] - 1e-27, torch.full((K,), 1e-27)) <= 40
+    assert R.worst(y[4] - 1 / (1 + 1e-6) ** 0.5, torch.ones(K)) <= norm_bound(K)
+    v = host(mt.dequantize_q8(out.q8))
+    assert torch.isnan(v[1]).all() and torch.isnan(v[2, :32]).all() and not torch.isnan(v[2, 32:]).any()
+    assert torch.equal(v[0], torch.zeros(K))
+
+
+def test_rms_norm_empty_and_strided_gamma(mt):
+    out = mt.rms_norm(torch.empty(0, 8, device="cuda"), torch.ones(8, device="cuda"), q8="int8")
+    assert out.y.shape == (0, 8) and out.q8.codes.shape == (0, 8)
+    g = gen(3)
+    x, gamma = rand(g, 4, 36), rand(g, 36)
+    wide = torch.zeros(36, 2, device="cuda")
+    wide[:, 1] = gamma.cuda()
+    a = mt.rms_norm(x.cuda(), wide[:, 1]).y
+    assert torch.allclose(a, mt.rms_norm(x.cuda(), gamma.cuda()).y, rtol=1e-5, atol=0)
+
+
+# dx is off, relative to its terms' magnitudes, by the sum over the row (as above) and at
+# most 8 roundings; dgamma by the sum over the rows in any order and 3 roundings.
+@pytest.mark.parametrize("rows,K", SHAPES + [(2000, 64), (1200, 260)])
+@pytest.mark.parametrize("with_dh", [False, True])
+def test_rms_norm_backward(mt, rows, K, with_dh):
+    g = gen(rows * 7 + K)
+    h, gamma, dy = rand(g, rows, K, scale=2.0), 1 + rand(g, K, scale=0.1), rand(g, rows, K)
+    dh = rand(g, rows, K) if with_dh else None
+    rstd = (1 / torch.sqrt((h.double() ** 2).mean(1) + 1e-6)).float()
+    dx, dgamma = mt.rms_norm_backward(dy.cuda(), h.cuda(), gamma.cuda(), rstd.cuda(), dh=dh.cuda() if with_dh else None)
+    want, mag, want_g, mag_g = R.rms_norm_backward(dy, h, gamma, rstd, dh)
+    assert R.worst(host(dx) - want, mag) <= max(32, K / 1024) + 10 + 8
+    assert R.worst(host(dgamma) - want_g, mag_g) <= rows + 3
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_rms_norm_backward_layouts(mt, layout):
+    g = gen(5)
+    h, gamma, dy, dh = rand(g, 9, 132), rand(g, 132), rand(g, 9, 132), rand(g, 9, 132)
+    rstd = (1 / torch.sqrt((h.double() ** 2).mean(1) + 1e-6)).float()
+    dx, dgamma = mt.rms_norm_backward(strided(dy, layout), strided(h, layout), gamma.cuda(), rstd.cuda(),
+                                      dh=strided(dh, layout))
+    want, mag, want_g, mag_g = R.rms_norm_backward(dy, h, gamma, rstd, dh)
+    assert R.worst(host(dx) - want, mag) <= 50 and R.worst(host(dgamma) - want_g, mag_g) <= 12
+
+
+def test_rms_norm_gradient_matches_differences(mt):
+    # f(x, gamma) = sum(y * c) in 64 bits of the formula; central differences of step 1e-4
+    # are off by O(step^2) ~ 1e-8 of f's third derivatives and 1e-12 of f by rounding.
+    g = gen(11)
+    x, gamma, c = rand(g, 3, 20).double(), (1 + rand(g, 20, scale=0.1)).double(), rand(g, 3, 20).double()
+
+    def f(x, gamma):
+        return (R.rms_norm(x, None, gamma, 1e-6)[2] * c).sum()
+
+    rstd = R.rms_norm(x, None, gamma, 1e-6)[1].float()
+    dx, dgamma = mt.rms_norm_backward(c.float().cuda(), x.float().cuda(), gamma.float().cuda(), rstd.cuda())
+    e = 1e-4
+    for i, j in ((0, 0), (1, 7), (2, 19)):
+        d = torch.zeros_like(x)
+        d[i, j] = e
+        assert abs(float((f(x + d, gamma) - f(x - d, gamma)) / (2 * e)) - float(dx[i, j])) < 1e-5
+    d = torch.zeros_like(gamma)
+    d[4] = e
+    assert abs(float((f(x, gamma + d) - f(x, gamma - d)) / (2 * e)) - float(dgamma[4])) < 1e-5
+
+
+def test_rms_norm_backward_empty(mt):
+    dx, dg = mt.rms_norm_backward(torch.empty(0, 8, device="cuda"), torch.empty(0, 8, device="cuda"),
+                                  torch.ones(8, device="cuda"), torch.empty(0, device="cuda"))
+    assert dx.shape == (0, 8) and torch.equal(host(dg), torch.zeros(8))
+
+
+# ---- 8 bits -----------------------------------------------------------------------------
+
+def q8_input(g, rows, cols):
+    """Magnitudes from 2^-140 to 2^120, block by block, zeros and exact powers of two among
+    them, and values next to a scale's border."""
+    x = rand(g, rows, cols)
+    e = torch.randint(-140, 120, (rows, -(-cols // 32)), generator=g).repeat_interleave(32, 1)[:, :cols]
+    x = torch.ldexp(x, e)
+    x[:, ::37] = 0
+    if rows > 2 and cols >= 32:
+        x[0, :32] = 0
+        x[1, :32] = torch.linspace(-127, 127, 32)
+        x[2, :32] = torch.nextafter(torch.tensor(127.0), torch.tensor(200.0))
+    return x
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 31), (5, 32), (4, 33), (6, 128), (3, 1000), (9, 1024), (2, 4099), (7, 160)])
+@pytest.mark.parametrize("layout", ["dense", "transposed", "window", "pitched"])
+def test_quantize_q8_is_exact(mt, fmt, rows, cols, layout):
+    x = q8_input(gen(rows + cols), rows, cols)
+    q = mt.quantize_q8(strided(x, layout), fmt)
+    b = R.q8_scale_bytes(x, fmt)
+    assert torch.equal(host(q.scales).long(), b)
+    assert torch.equal(host(q.codes).view(torch.uint8) & 0x7F if fmt == "e4m3" else host(q.codes),
+                       R.q8_codes(x, b, fmt).view(torch.uint8) & 0x7F if fmt == "e4m3" else R.q8_codes(x, b, fmt))
+    v = R.q8_values(host(q.codes).float(), host(q.scales))
+    assert torch.equal(host(mt.dequantize_q8(q)).double(), v)
+    assert torch.equal(host(mt.dequantize_q8(q, dtype=torch.bfloat16)), v.float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_quantize_q8_non_finite_blocks(mt, fmt):
+    x = torch.ones(3, 100)
+    x[0, 40] = float("inf")
+    x[1, 99] = float("nan")
+    q = mt.quantize_q8(x.cuda(), fmt)
+    v = host(mt.dequantize_q8(q))
+    bad = torch.zeros(3, 100, dtype=torch.bool)
+    bad[0, 32:64] = True
+    bad[1, 96:] = True
+    assert torch.equal(torch.isnan(v), bad) and torch.equal(v[~bad], x[~bad])
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_dequantize_q8_of_a_pitched_view(mt, fmt):
+    x = q8_input(gen(1), 6, 96)
+    q = mt.quantize_q8(x.cuda(), fmt)
+    wide = torch.zeros(6, 130, dtype=torch.int8, device="cuda")
+    wide[:, 1:97] = q.codes.view(torch.int8)
+    view = mt.Q8Tensor(wide[:, 1:97].view(q.codes.dtype), q.scales)
+    assert torch.equal(mt.dequantize_q8(view), mt.dequantize_q8(q))
+
+
+WGRAD_SHAPES = [(1, 1, 1), (2, 3, 5), (16, 64, 64), (17, 65, 63), (100, 130, 257), (128, 128, 128), (129, 256, 300),
+                (300, 33, 700), (1000, 520, 136), (64, 600, 1100)]
+
+
+def wgrad_input(g, M, K, N, fmt, mt):
+    q = mt.quantize_q8(rand(g, M, K).cuda(), fmt)
+    return q, rand(g, M, N) * torch.exp(rand(g, M, 1))
+
+
+def check_wgrad(q, dy, dW, db):
+    xv = R.q8_values(host(q.codes).float(), host(q.scales))
+    M = dy.shape[0]
+    want, mag = xv.t() @ dy.double(), xv.abs().t() @ dy.double().abs()
+    assert R.worst(host(dW) - want, mag) <= M + 8
+    assert R.worst(host(db) - dy.double().sum(0, keepdim=True), dy.double().abs().sum(0, keepdim=True)) <= M
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("M,K,N", WGRAD_SHAPES)
+def test_linear_weight_grad_q8(mt, fmt, M, K, N):
+    q, dy = wgrad_input(gen(M * K + N), M, K, N, fmt, mt)
+    dW, db = mt.linear_weight_grad_q8(q, dy.cuda())
+    check_wgrad(q, dy, dW, db)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_linear_weight_grad_q8_layouts(mt, layout):
+    q, dy = wgrad_input(gen(2), 70, 96, 132, "int8", mt)
+    check_wgrad(q, dy, *mt.linear_weight_grad_q8(q, strided(dy, layout)))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_linear_weight_grad_q8_keeps_every_bit(mt, fmt):
+    """One row: dW[k][n] = xhat[k] * dy[n] needs one rounding, so it is the float product."""
+    g = gen(4)
+    x = rand(g, 1, 96)
+    dy = rand(g, 1, 200) * torch.exp(5 * rand(g, 1, 200))
+    q = mt.quantize_q8(x.cuda(), fmt)
+    dW, db = mt.linear_weight_grad_q8(q, dy.cuda())
+    want = host(mt.dequantize_q8(q)).double().t() @ dy.double()
+    assert R.worst(host(dW) - want, want) <= 3     # three exact parts, added in float
+    assert torch.equal(host(db), dy)
+
+
+def test_linear_weight_grad_q8_empty(mt):
+    q = mt.quantize_q8(torch.empty(0, 64, device="cuda"))
+    dW, db = mt.linear_weight_grad_q8(q, torch.empty(0, 40, device="cuda"))
+    assert torch.equal(host(dW), torch.zeros(64, 40)) and torch.equal(host(db), torch.zeros(1, 40))
+
+
+def test_linear_weight_grad_q8_non_finite(mt):
+    """A NaN block of the checkpoint reaches its 32 rows of dW, an infinite gradient its column,
+    and nothing else."""
+    x, dy = torch.ones(40, 96), torch.ones(40, 70)
+    x[3, 40] = float("nan")
+    dy[5, 9] = float("inf")
+    dy[6, 11] = float("nan")
+    dW, db = mt.linear_weight_grad_q8(mt.quantize_q8(x.cuda()), dy.cuda())
+    dW, db = host(dW), host(db)
+    assert torch.isnan(dW[32:64]).all()
+    rest = torch.cat([dW[:32], dW[64:]])
+    assert torch.isinf(rest[:, 9]).all() and torch.isnan(rest[:, 11]).all()
+    keep = [n for n in range(70) if n not in (9, 11)]
+    assert torch.equal(rest[:, keep], torch.full((64, 68), 40.0))
+    assert torch.isinf(db[0, 9]) and torch.isnan(db[0, 11]) and torch.equal(db[0, keep], torch.full((68,), 40.0))
+
+
+def test_training_step_through_a_checkpoint(mt):
+    """norm -> Linear -> its backward -> the norm's, as a training step calls them."""
+    g = gen(8)
+    M, K, N = 96, 256, 160
+    x, r, gamma = rand(g, M, K).cuda(), rand(g, M, K).cuda(), (1 + rand(g, K, scale=0.1)).cuda()
+    W, b, dY, dh = rand(g, K, N, scale=0.1).cuda(), rand(g, 1, N).cuda(), rand(g, M, N).cuda(), rand(g, M, K).cuda()
+    n = mt.rms_norm(x, gamma, residual=r, q8="int8")
+    Y, saved = mt.linear_forward_q8(n.y, W, b)
+    assert torch.equal(saved.codes, n.q8.codes) and torch.equal(saved.scales, n.q8.scales)
+    assert torch.equal(Y, mt.linear_forward(n.y, W, b))
+    dX, dW, db = mt.linear_backward_q8(saved, W, dY)
+    check_wgrad(saved, host(dY), dW, db)
+    eX, _, eb = mt.linear_backward(n.y, W, dY)
+    assert torch.equal(dX, eX)
+    dx, dgamma = mt.rms_norm_backward(dX, n.h, gamma, n.rstd, dh=dh)
+    want, mag, want_g, mag_g = R.rms_norm_backward(host(dX), host(n.h), host(gamma), host(n.rstd), host(dh))
+    assert R.worst(host(dx) - want, mag) <= 50 and R.worst(host(dgamma) - want_g, mag_g) <= M + 3
+
+
+# ---- 4 bits -----------------------------------------------------------------------------
+
+Q4_SHAPES = [(1, 1), (5, 3), (64, 16), (127, 40), (128, 64), (129, 17), (300, 130), (1000, 33), (1024, 256)]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("K,N", Q4_SHAPES)
+def test_quantize_q4_is_exact(mt, group, K, N):
+    W = rand(gen(K + N), K, N)
+    W[:, N // 2] = 0
+    q = mt.quantize_q4(W.cuda(), group)
+    codes, s = R.q4_quantize(W, group)
+    assert torch.equal(host(q.scales), s)
+    assert torch.equal(host(q.codes), R.q4_pack(codes, K))
+    assert torch.equal(host(mt.dequantize_q4(q)).double(), R.q4_weight(codes, s, group))
+    qt = mt.quantize_q4(W.t().contiguous().cuda().t(), group)
+    assert torch.equal(qt.codes, q.codes) and torch.equal(qt.scales, q.scales)
+
+
+def q4_case(g, M, K, N, group):
+    codes = torch.randint(0, 16, (N, K), generator=g)
+    s = (0.01 * torch.exp(rand(g, N, -(-K // group)))).to(torch.bfloat16)
+    x = rand(g, M, K) * torch.exp(rand(g, 1, K))
+    return x, codes, s
+
+
+def check_q4(y, x, W, bias, relu):
+    """A float sum of K terms in any order, the scale's and the bias's roundings."""
+    want, mag = x.double() @ W, x.double().abs() @ W.abs()
+    if bias is not None:
+        want, mag = want + bias.double(), mag + bias.double().abs()
+    K = x.shape[1]
+    err = host(y).double() - (want.clamp_min(0) if relu else want)
+    assert R.worst(err, mag) <= K + 8
+
+
+Q4_ROWS = [1, 2, 3, 5, 8, 9, 16, 21, 40, 130, 300]
+
+
+@pytest.mark.parametrize("M", Q4_ROWS)
+@pytest.mark.parametrize("K,N,group", [(1, 1, 32), (31, 5, 32), (128, 16, 64), (300, 130, 32), (1000, 77, 128),
+                                       (2048, 264, 64), (1111, 401, 128)])
+def test_linear_forward_q4(mt, M, K, N, group):
+    g = gen(M * 1000003 + K * 1009 + N)
+    x, codes, s = q4_case(g, M, K, N, group)
+    bias = rand(g, N) if N % 2 else None
+    relu = M % 2 == 0
+    w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, group)
+    y = mt.linear_forward_q4(x.cuda(), w, bias=bias.cuda() if bias is not None else None, relu=relu)
+    check_q4(y, x, R.q4_weight(codes, s, group), bias, relu)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("M", [1, 4, 50])
+def test_linear_forward_q4_layouts(mt, layout, M):
+    g = gen(M)
+    x, codes, s = q4_case(g, M, 260, 50, 64)
+    w = mt.Q4Weight(R.q4_pack(codes, 260).cuda(), s.cuda(), 260, 64)
+    check_q4(mt.linear_forward_q4(strided(x, layout), w), x, R.q4_weight(codes, s, 64), None, False)
+
+
+@pytest.mark.parametrize("M", Q4_ROWS)
+def test_linear_forward_q4_keeps_every_bit(mt, M):
+    """Weights with one code other than 8 in a column: y is x's value times code times scale, so
+    at most the three exact parts and the scale round; every position of K is met."""
+    K, N, group = 288, 288, 32
+    g = gen(M)
+    x = rand(g, M, K) * torch.exp(5 * rand(g, M, K))
+    codes = torch.full((N, K), 8, dtype=torch.int64)
+    n = torch.arange(N)
+    codes[n, n] = torch.where(n % 15 < 8, n % 15, n % 15 + 1)
+    s = torch.exp(rand(g, N, K // group)).to(torch.bfloat16)
+    w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, group)
+    want = x.double() @ R.q4_weight(codes, s, group)
+    assert R.worst(host(mt.linear_forward_q4(x.cuda(), w)) - want, want) <= 4
+
+
+def test_linear_forward_q4_non_finite(mt):
+    """A NaN or an infinity in one row of x stays in that row; a NaN scale in its column."""
+    K, N = 256, 48
+    codes = torch.full((N, K), 9, dtype=torch.int64)
+    s = torch.ones(N, 4, dtype=torch.bfloat16)
+    s[7, 2] = float("nan")
+    for M in (3, 40):
+        x = torch.ones(M, K)
+        x[0, 5], x[1, 200] = float("nan"), float("inf")
+        w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, 64)
+        y = host(mt.linear_forward_q4(x.cuda(), w))
+        assert torch.isnan(y[0]).all() and torch.isnan(y[:, 7]).all()
+        keep = [n for n in range(N) if n != 7]
+        assert torch.equal(y[1, keep], torch.full((N - 1,), float("inf")))
+        assert torch.equal(y[2:, keep], torch.full((M - 2, N - 1), 256.0))
+
+
+def test_linear_forward_q4_empty(mt):
+    w = mt.quantize_q4(torch.randn(64, 32).cuda())
+    assert mt.linear_forward_q4(torch.empty(0, 64, device="cuda"), w).shape == (0, 32)
+    none = mt.quantize_q4(torch.empty(0, 32, device="cuda"))
+    bias = torch.randn(32, device="cuda")
+    y = mt.linear_forward_q4(torch.empty(3, 0, device="cuda"), none, bias=bias)
+    assert torch.equal(y, bias.expand(3, 32))
+
+
+def test_decoding_step(mt):
+    """norm -> 4-bit Linear -> residual -> norm, as one decoded token goes through."""
+    g = gen(21)
+    K, N = 256, 256
+    x, r, gamma, W = rand(g, 1, K), rand(g, 1, K), 1 + rand(g, K, scale=0.1), rand(g, K, N, scale=0.06)
+    w = mt.quantize_q4(W.cuda(), 64)
+    n = mt.rms_norm(x.cuda(), gamma.cuda(), residual=r.cuda())
+    y = mt.linear_forward_q4(n.y, w)
+    check_q4(y, host(n.y), host(mt.dequantize_q4(w)).double(), None, False)
+    n2 = mt.rms_norm(y, gamma.cuda(), residual=n.h, inplace=True)
+    h, rstd, want = R.rms_norm(host(n2.h), None, gamma, 1e-6)
+    assert R.worst(host(n2.y) - want, want) <= norm_bound(K) + 1
