@@ -1,13 +1,15 @@
 // mt_lowbit.cu -- C entries of the low-bit operators (declared in include/mtgemm.h): argument
 // checks, choice of kernel and launches.
 #include <algorithm>
+#include <atomic>
+#include <cstdio>
 
 #include "mtgemm.h"
 #include "mt_host.h"
 #include "lowbit_common.cuh"
+#include "planes_gemm.cuh"
 #include "q4.cuh"
 #include "q8.cuh"
-#include "q8_wgrad.cuh"
 #include "rms_norm.cuh"
 
 namespace {
@@ -230,6 +232,144 @@ struct LaunchBwd {
     template <int VEC, int V, int WPR, int RPC> int run() { return launch_bwd<VEC, V, WPR, RPC>(p, groups, st); }
 };
 
+// ------------------------- exact-by-float tensor-core product -------------------------
+
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// Scratch of one call, given back on every way out (stream order makes that safe).
+struct Scratch {
+    void* p = nullptr;
+    size_t bytes = 0;
+    cudaStream_t st;
+    explicit Scratch(cudaStream_t s) : st(s) {}
+    Scratch(const Scratch&) = delete;
+    ~Scratch() { mt::host::scratch_free(p, bytes, st); }
+    int take(size_t n, const char* who) {
+        bytes = n;
+        return mt::host::scratch_alloc(&p, n, st, who);
+    }
+};
+
+// Splits of the sum over k: the least of rounds x length, a 64-deep block of a pair tile
+// taking about 1,600 cycles and the partials' way through memory about 3,000 bytes a cycle.
+int pick_splits(int64_t tiles, int64_t kblocks, int64_t chunk_blocks, int64_t clusters, int64_t out_bytes) {
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, kblocks / chunk_blocks));
+    int best = 1;
+    double least = 1e300;
+    for (int64_t s = 1; s <= most; ++s) {
+        const int64_t len = (kblocks / chunk_blocks + s - 1) / s * chunk_blocks;
+        const double cost = (double)((tiles * s + clusters - 1) / clusters) * len * 1600. +
+                            (s > 1 ? (2. * s + 1.) * out_bytes / 3000. + 4000. : 0.);
+        if (cost < least * 0.98) { least = cost; best = (int)s; }
+    }
+    return best;
+}
+
+// D = A * B^T over `kpitch` padded values of k: a [R][kpitch], b [3][C][kpitch], both bfloat16.
+// p carries the output, the scales (SCALED), the bias and spc.
+template <bool SCALED>
+int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16* b, int64_t kpitch, cudaStream_t st,
+               const char* who) {
+    using namespace mt::planes;
+    const int sms = mt::host::sm_count();
+    const int64_t clusters = std::max(1, sms / 2);
+    p.kblocks = (int)((kpitch + BK - 1) / BK);
+    p.tiles_r = (p.R + BM - 1) / BM;
+    p.tiles_c = (p.C + BN - 1) / BN;
+    const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c;
+    if (tiles > INT32_MAX / 64) return fail(MT_EUNSUPPORTED, "%s: too many output tiles", who);
+    p.splits = pick_splits(tiles, p.kblocks, p.spc == 8 ? 2 : 1, clusters, (int64_t)p.R * p.C * 4);
+    p.units = (int)tiles * p.splits;
+    Scratch part(st);
+    if (p.splits > 1) MT_TRY(part.take((size_t)p.splits * p.R * p.C * sizeof(float), who));
+    p.part = static_cast<float*>(part.p);
+    CUtensorMap ta, tb;
+    const uint64_t da[3] = {(uint64_t)kpitch, (uint64_t)p.R, 1}, db[3] = {(uint64_t)kpitch, (uint64_t)p.C, 3};
+    const uint64_t sa[2] = {(uint64_t)kpitch * 2, (uint64_t)kpitch * 2 * p.R}, sb[2] = {(uint64_t)kpitch * 2, (uint64_t)kpitch * 2 * p.C};
+    const uint32_t ba[3] = {BK, 128, 1}, bb[3] = {BK, 128, 3};
+    if (!mt::host::encode_bf16(&ta, a, 3, da, sa, ba) || !mt::host::encode_bf16(&tb, b, 3, db, sb, bb))
+        return fail(MT_ECUDA, "%s: tensor map encoding failed", who);
+    static std::atomic<uint64_t> smem_set{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(smem_set.load() & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<SCALED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+        if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
+        smem_set.fetch_or(bit);
+    }
+    const unsigned grid = 2 * (unsigned)std::min<int64_t>(p.units, clusters);
+    gemm_kernel<SCALED><<<grid, THREADS, SMEM_BYTES, st>>>(ta, tb, p);
+    MT_TRY(launched(who));
+    if (p.splits > 1) {
+        join_kernel<<<grid_of(((int64_t)p.R * p.C + 255) / 256, 16LL * sms), 256, 0, st>>>(p);
+        MT_TRY(launched(who));
+    }
+    char path[96];
+    snprintf(path, sizeof path, "%s planes splits=%d", who, p.splits);
+    mt::host::set_path(path);
+    return MT_OK;
+}
+
+int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64_t M, int64_t K, int64_t N,
+                 cudaStream_t st, const char* who) {
+    const int64_t pitch = std::max<int64_t>(8, round_up(M, 8));
+    const size_t a_bytes = round_up(K * pitch * 2, 256), b_bytes = round_up(3 * N * pitch * 2, 256);
+    const int64_t tiles_m = (pitch + 63) / 64;
+    const size_t s_bytes = db.p ? (size_t)tiles_m * N * sizeof(float) : 0;
+    Scratch ws(st);
+    MT_TRY(ws.take(a_bytes + b_bytes + s_bytes, who));
+    __nv_bfloat16* a = static_cast<__nv_bfloat16*>(ws.p);
+    __nv_bfloat16* b = a + a_bytes / 2;
+    float* sums = db.p ? reinterpret_cast<float*>(b + b_bytes / 2) : nullptr;
+    if (K > 0) {
+        mt::planes::expand_q8_kernel<<<dim3((unsigned)((K + 63) / 64), grid_of(tiles_m, 65535)), 256, 0, st>>>(q, a, M, K, pitch);
+        MT_TRY(launched(who));
+    }
+    mt::planes::split_rows_kernel<<<dim3((unsigned)((N + 63) / 64), grid_of(tiles_m, 65535)), 256, 0, st>>>(dy, b, M, N, pitch, sums);
+    MT_TRY(launched(who));
+    if (db.p) {
+        mt::rms::sum_parts_kernel<<<(unsigned)((N + 31) / 32), dim3(32, 8), 0, st>>>(sums, tiles_m, N, db);
+        MT_TRY(launched(who));
+    }
+    if (K == 0) return MT_OK;
+    mt::planes::Params p{};
+    p.R = (int)K;
+    p.C = (int)N;
+    p.spc = 8;
+    p.out = dw.p;
+    p.os_r = dw.rs;
+    p.os_c = dw.cs;
+    return run_planes<false>(p, a, b, pitch, st, who);
+}
+
+int linear_q4_planes(const Mat& x, const mt::q4::Weight& w, const float* bias, const Mat& y, int64_t M, int relu,
+                     cudaStream_t st, const char* who) {
+    const int64_t pitch = round_up(w.K, mt::q4::kSpan);
+    const size_t a_bytes = w.N * pitch * 2, b_bytes = 3 * M * pitch * 2;
+    Scratch ws(st);
+    MT_TRY(ws.take(a_bytes + b_bytes, who));
+    __nv_bfloat16* a = static_cast<__nv_bfloat16*>(ws.p);
+    __nv_bfloat16* b = a + a_bytes / 2;
+    mt::planes::expand_q4_kernel<<<dim3((unsigned)((pitch / 8 + 255) / 256), grid_of(w.N, 65535)), 256, 0, st>>>(w, a, pitch);
+    MT_TRY(launched(who));
+    mt::planes::split_cols_kernel<<<dim3((unsigned)((pitch / 4 + 255) / 256), grid_of(M, 65535)), 256, 0, st>>>(x, b, M, w.K, pitch);
+    MT_TRY(launched(who));
+    mt::planes::Params p{};
+    p.R = (int)w.N;
+    p.C = (int)M;
+    p.spc = w.group / 16;
+    p.out = y.p;
+    p.os_r = y.cs;
+    p.os_c = y.rs;
+    p.scales = w.scales;
+    p.sp = w.sp;
+    p.groups = (int)((w.K + w.group - 1) / w.group);
+    p.bias = bias;
+    p.relu = relu;
+    return run_planes<true>(p, a, b, pitch, st, who);
+}
+
 }  // namespace
 
 extern "C" {
@@ -438,16 +578,7 @@ MT_API int mt_linear_wgrad_q8(const mt_q8* x, const mt_tensor* dY, const mt_tens
     MT_TRY(check_apart(span_of(vdw), "dW", span_of(vdb), "db", who));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (N == 0) return MT_OK;
-    if (K > 0) {
-        const int64_t ty = (K + mt::wgrad8::T - 1) / mt::wgrad8::T;
-        if (ty > 65535) return fail(MT_EUNSUPPORTED, "%s: too many input features", who);
-        mt::wgrad8::simple_kernel<<<dim3((unsigned)((N + mt::wgrad8::T - 1) / mt::wgrad8::T), (unsigned)ty), 256, 0, st>>>(
-            q, vdy.m, vdw.m, M, K, N);
-        MT_TRY(launched("linear_wgrad_q8 launch"));
-    }
-    if (db) MT_TRY(mt_sum_rows_gpu(dY, db, stream));
-    mt::host::set_path("linear_wgrad_q8 simple");
-    return MT_OK;
+    return wgrad_planes(q, vdy.m, vdw.m, vdb.m, M, K, N, st, who);
 }
 
 MT_API int mt_quantize_q4(const mt_tensor* W, const mt_q4* q, void* stream) {
@@ -508,6 +639,8 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     for (int i = 0; i < 4; ++i) MT_TRY(check_apart(span_of(vy), "Y", in[i], names[i], who));
     const int64_t M = vx.rows;
     if (M * w.N == 0) return MT_OK;
+    if (M > 8 && w.K > 0)
+        return linear_q4_planes(vx.m, w, vb.m.p, vy.m, M, relu, static_cast<cudaStream_t>(stream), who);
     mt::q4::linear_simple_kernel<<<dim3((unsigned)((w.N + 7) / 8), grid_of((M + 3) / 4, 65535)), 256, 0,
                                    static_cast<cudaStream_t>(stream)>>>(vx.m, w, vb.m.p, vy.m, M, relu);
     MT_TRY(launched("linear_fwd_q4 launch"));

@@ -1,0 +1,439 @@
+// planes_gemm.cuh -- a float-accurate tensor-core product for a left operand that bfloat16
+// holds exactly (8-bit checkpoints, 4-bit weight codes).
+//
+//   D[r][c] = sum_k A[r][k] * B[c][k],  A bfloat16, B float
+//
+// Mathematics. A float is the exact sum of three bfloat16 numbers: truncating it to its top
+// 8 significand bits leaves a remainder of 16 bits, truncating that leaves 8 (split3). So
+// A * B is the sum of three products of 8-bit by 8-bit significands, each exact in the
+// float accumulator: three kind::f16 MMAs per k-step instead of the three of 3xTF32 at half
+// their rate, twice as fast, and no bits of the operands are lost.
+//
+// Accumulation. The tensor core adds into its accumulator by truncation, so a long sum
+// drifts towards zero by about one part in 2^24 per step; over thousands of rows that
+// exceeds a float sum's error. The accumulator is therefore drained every `spc` k-steps
+// (32 to 128 values of k) into registers that add with rounding, while the next chunk goes
+// into the other half of TMEM. The 4-bit product multiplies by the group's scale there, once
+// per group instead of once per weight.
+//
+// Work. A pair of CTAs shares a 256 x 256 tile (tcgen05 cta_group::2, as umma_gemm2.cuh): each
+// holds its 128 rows of A and its 128 columns of the three planes of B, 64 KB per 64-deep
+// stage, 3 stages. Warp 0 loads by TMA, warp 1 of the even CTA issues the MMAs, warps 2-9
+// drain: lane quarter = warp & 3, 128 columns each, 128 accumulators per thread. Few tiles:
+// the sum over k is split between clusters, partial tiles go to scratch and a second kernel
+// adds them in order. Bound: tensor pipe, 3 * 2 R C K operations.
+#pragma once
+
+#include "lowbit_common.cuh"
+#include "q4.cuh"
+
+namespace mt {
+namespace planes {
+
+using lowbit::Mat;
+
+constexpr int BM = 256, BN = 256;       // pair tile
+constexpr int BK = 64;                  // k per stage: 128-byte rows
+constexpr int STAGES = 3;
+constexpr uint32_t A_BYTES = 128 * BK * 2;
+constexpr uint32_t B_BYTES = 128 * BK * 2;            // one plane
+constexpr uint32_t STAGE_BYTES = A_BYTES + 3 * B_BYTES;
+constexpr uint32_t RING_BYTES = STAGE_BYTES * STAGES;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 32 * (2 + EPI_WARPS);
+constexpr uint32_t EPI_BYTES = EPI_WARPS * 32 * 33 * 4;
+constexpr uint32_t BAR_BYTES = 8 * (2 * STAGES + 4) + 16;
+constexpr uint32_t SMEM_BYTES = 1024 + RING_BYTES + EPI_BYTES + BAR_BYTES;
+static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
+
+struct Params {
+    int R, C;                    // rows of A, rows of B
+    int kblocks;                 // 64-deep blocks of k
+    int spc;                     // k16-steps per chunk: 2, 4 or 8
+    int tiles_r, tiles_c, splits;
+    int units;                   // tiles * splits
+    float* out;                  // D[r][c] at out + r * os_r + c * os_c
+    int64_t os_r, os_c;
+    float* part;                 // splits > 1: partial s of D at part + s * R * C, row-major
+    const __nv_bfloat16* scales; // SCALED: scale of row r, chunk j at r * sp + j
+    int64_t sp;
+    int groups;                  // scales per row; chunks behind them have no codes
+    const float* bias;           // per row r, may be null (SCALED)
+    int relu;
+};
+
+// Unit u -> tile and the k-blocks [kb0, kb1) of its split; a split begins on a chunk.
+// Row blocks go in groups of 8, so that clusters at work share rows of A and B in L2.
+__device__ __forceinline__ void unit_of(const Params& p, int u, int& rb, int& cb, int& sp, int& kb0, int& kb1) {
+    sp = u % p.splits;
+    const int t = u / p.splits;
+    const int per = 8 * p.tiles_c;
+    const int g = t / per, in = t - g * per;
+    const int rows = min(8, p.tiles_r - g * 8);
+    cb = in / rows;
+    rb = g * 8 + in - cb * rows;
+    const int cpb = p.spc == 8 ? 2 : 1;                        // k-blocks per chunk boundary
+    const int nb = (p.kblocks + cpb - 1) / cpb;
+    kb0 = (int)((long long)nb * sp / p.splits) * cpb;
+    kb1 = min(p.kblocks, (int)((long long)nb * (sp + 1) / p.splits) * cpb);
+}
+
+// kind::f16 instruction descriptor: bfloat16 operands, K-major, float accumulate.
+__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accum) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+        : "memory");
+}
+
+template <bool SCALED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* ring = smem;
+    float* epi = reinterpret_cast<float*>(smem + RING_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + RING_BYTES + EPI_BYTES);
+    uint64_t* full = bars;
+    uint64_t* empty = bars + STAGES;
+    uint64_t* acc_full = bars + 2 * STAGES;
+    uint64_t* acc_empty = bars + 2 * STAGES + 2;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * STAGES + 4);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * STAGES + 4) + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(smem_u32(&acc_full[a]), 1);
+            mbar_init(smem_u32(&acc_empty[a]), 2 * EPI_WARPS);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32((const void*)tmem_slot), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    int rb, cb, sp, kb0, kb1;
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            for (int u = first; u < p.units; u += step) {
+                unit_of(p, u, rb, cb, sp, kb0, kb1);
+                const int r0 = rb * BM + (int)rank * 128, c0 = cb * BN + (int)rank * 128;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait_cl(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) goto done;
+                    const uint32_t sa = smem_u32(ring + s * STAGE_BYTES);
+                    if (leader) mbar_arrive_expect_tx(smem_u32(&full[s]), 2 * STAGE_BYTES);
+                    const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+                    tma_load_3d_pair(sa, &tmA, bar, kb * BK, r0, 0);
+                    tma_load_3d_pair(sa + A_BYTES, &tmB, bar, kb * BK, c0, 0);
+                    if (++s == STAGES) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            constexpr uint32_t idesc = idesc_bf16(BM, BN);
+            const int nsub = p.spc == 2 ? 2 : 1, steps = 4 / nsub;
+            int s = 0, n = 0;          // stage, chunks begun
+            uint32_t ph = 0;
+            for (int u = first; u < p.units; u += step) {
+                unit_of(p, u, rb, cb, sp, kb0, kb1);
+                int in_chunk = 0;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait_cl(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) goto done;
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(ring + s * STAGE_BYTES);
+                    for (int sub = 0; sub < nsub; ++sub) {
+                        const int a = n & 1;
+                        if (in_chunk == 0) {
+                            if (!mbar_wait_cl(smem_u32(&acc_empty[a]), ((n >> 1) & 1) ^ 1, abort_flag, kDevTimeoutAccEmpty))
+                                goto done;
+                            tc_fence_after();
+                        }
+                        // Smallest plane first: its sums meet a small accumulator.
+                        for (int pl = 2; pl >= 0; --pl) {
+                            const uint32_t sb = sa + A_BYTES + pl * B_BYTES;
+                            for (int k = sub * steps; k < (sub + 1) * steps; ++k) {
+                                umma_bf16_pair(tmem_base + a * BN, umma_desc(sa + k * 32, 16, 1024, kLayoutSw128),
+                                               umma_desc(sb + k * 32, 16, 1024, kLayoutSw128), idesc,
+                                               in_chunk > 0 || pl < 2 || k > sub * steps ? 1u : 0u);
+                            }
+                        }
+                        in_chunk += steps;
+                        if (in_chunk == p.spc || (kb == kb1 - 1 && sub == nsub - 1)) {
+                            umma_commit_pair(smem_u32(&acc_full[a]));
+                            umma_commit_pair(mapa_shared(smem_u32(&acc_full[a]), 1));
+                            ++n;
+                            in_chunk = 0;
+                        }
+                    }
+                    umma_commit_pair(smem_u32(&empty[s]));
+                    umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 1));
+                    if (++s == STAGES) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+    } else {
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        float* buf = epi + (warp - 2) * 32 * 33;
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * 128;
+        const uint32_t empty_bar[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
+        int n = 0;
+        for (int u = first; u < p.units; u += step) {
+            unit_of(p, u, rb, cb, sp, kb0, kb1);
+            const int row0 = rb * BM + (int)rank * 128 + q * 32;
+            const int col0 = cb * BN + half * 128;
+            const int chunks = ((kb1 - kb0) * 4 + p.spc - 1) / p.spc;
+            const __nv_bfloat16* sc = nullptr;
+            const int g0 = kb0 * 4 / p.spc;
+            if (SCALED) sc = p.scales + (int64_t)min(row0 + lane, p.R - 1) * p.sp;
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+#pragma unroll 1
+            for (int ch = 0; ch < chunks; ++ch, ++n) {
+                const int a = n & 1;
+                float scale = 1.f;
+                if (SCALED) scale = g0 + ch < p.groups ? __bfloat162float(sc[g0 + ch]) : 0.f;
+                if (!mbar_wait_cl(smem_u32(&acc_full[a]), (n >> 1) & 1, abort_flag, kDevTimeoutAccFull)) goto done;
+                __syncwarp();
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t r[16];
+                    tmem_ld_32x32b_x16(taddr + a * BN + c * 16, r);
+                    tmem_ld_wait();
+                    if (c == 7) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(empty_bar[a]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        acc[c * 16 + j] = SCALED ? fmaf(__uint_as_float(r[j]), scale, acc[c * 16 + j])
+                                                 : acc[c * 16 + j] + __uint_as_float(r[j]);
+                }
+            }
+            float* out = p.splits > 1 ? p.part + (int64_t)sp * p.R * p.C : p.out;
+            const int64_t os_r = p.splits > 1 ? p.C : p.os_r, os_c = p.splits > 1 ? 1 : p.os_c;
+            if (SCALED && p.splits == 1) {
+                const int row = row0 + lane;
+                const float b = p.bias && row < p.R ? p.bias[row] : 0.f;
+#pragma unroll
+                for (int j = 0; j < 128; ++j) {
+                    acc[j] += b;
+                    if (p.relu) acc[j] = acc[j] > 0.f ? acc[j] : 0.f;
+                }
+            }
+            if (os_r == 1) {
+                // Lanes are neighbours in memory: one 128-byte line per column.
+                if (row0 + lane < p.R) {
+                    float* o = out + row0 + lane;
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (col0 + j < p.C) o[(int64_t)(col0 + j) * os_c] = acc[j];
+                }
+            } else {
+                // 32 x 32 blocks turned in shared memory: lanes along c.
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) buf[lane * 33 + j] = acc[c * 32 + j];
+                    __syncwarp();
+                    const int col = col0 + c * 32 + lane;
+                    if (col < p.C) {
+                        const int rows = min(32, p.R - row0);
+                        float* o = out + (int64_t)row0 * os_r + (int64_t)col * os_c;
+                        for (int i = 0; i < rows; ++i) o[(int64_t)i * os_r] = buf[i * 33 + lane];
+                    }
+                }
+            }
+        }
+    }
+
+done:
+    if (warp == 0 && lane == 0 && *abort_flag) {
+        // Give copies already issued time to land before the CTA leaves.
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// D = sum of the splits' partials in order (+ bias per row, ReLU).
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+    const int64_t n = (int64_t)p.R * p.C;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        // Neighbouring threads along the output's unit stride.
+        const int64_t r = p.os_r == 1 ? i % p.R : i / p.C, c = p.os_r == 1 ? i / p.R : i % p.C;
+        float v = p.part[r * p.C + c];
+        for (int s = 1; s < p.splits; ++s) v += p.part[s * n + r * p.C + c];
+        if (p.bias) v += p.bias[r];
+        if (p.relu) v = v > 0.f ? v : 0.f;
+        p.out[r * p.os_r + c * p.os_c] = v;
+    }
+}
+
+// x = h + m + l exactly, each part a bfloat16 (truncations: 8 + 8 + 8 significand bits). An
+// infinity or NaN is its own first part.
+__device__ __forceinline__ void split3(float x, uint16_t (&o)[3]) {
+    const uint32_t b = __float_as_uint(x);
+    if ((b & 0x7F800000u) == 0x7F800000u) {
+        o[0] = (uint16_t)(b >> 16) | ((b & 0x7FFFFFu) ? 0x40u : 0u);   // a NaN stays one
+        o[1] = o[2] = 0;
+        return;
+    }
+    const uint32_t h = b & 0xFFFF0000u;
+    const float r = x - __uint_as_float(h);
+    const uint32_t m = __float_as_uint(r) & 0xFFFF0000u;
+    const float l = r - __uint_as_float(m);
+    o[0] = (uint16_t)(h >> 16);
+    o[1] = (uint16_t)(m >> 16);
+    o[2] = (uint16_t)(__float_as_uint(l) >> 16);
+}
+
+// Planes of B for a sum over rows of x [M, N]: out[plane][n][m], m padded with zeros to `pitch`.
+// 64 x 64 tiles turned in shared memory. col_sums, if not null: sums of each tile's columns
+// at [tile][N], for the bias gradient.
+__global__ void __launch_bounds__(256) split_rows_kernel(Mat x, __nv_bfloat16* out, int64_t M, int64_t N, int64_t pitch,
+                                                         float* col_sums) {
+    __shared__ float s[64][65];
+    __shared__ float cs[4][64];
+    const int64_t n0 = (int64_t)blockIdx.x * 64;
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int64_t mt = blockIdx.y; mt * 64 < pitch; mt += gridDim.y) {
+        const int64_t m0 = mt * 64;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t m = m0 + ty + 4 * i;
+            const float v = m < M && n0 + tx < N ? x.p[m * x.rs + (n0 + tx) * x.cs] : 0.f;
+            s[ty + 4 * i][tx] = v;
+            sum += v;
+        }
+        cs[ty][tx] = sum;
+        __syncthreads();
+        if (col_sums && ty == 0 && n0 + tx < N) {
+            col_sums[mt * N + n0 + tx] = cs[0][tx] + cs[1][tx] + cs[2][tx] + cs[3][tx];
+        }
+        const int64_t m = m0 + 2 * lane;
+        if (m < pitch) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t n = n0 + warp * 8 + i;
+                if (n >= N) break;
+                uint16_t a[3], b[3];
+                split3(s[2 * lane][warp * 8 + i], a);
+                split3(s[2 * lane + 1][warp * 8 + i], b);
+#pragma unroll
+                for (int pl = 0; pl < 3; ++pl)
+                    *reinterpret_cast<uint32_t*>(out + (pl * N + n) * pitch + m) = a[pl] | ((uint32_t)b[pl] << 16);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Planes of B for a sum over columns of x [M, K]: out[plane][m][k], k padded with zeros to `pitch`
+// (a multiple of 4).
+__global__ void __launch_bounds__(256) split_cols_kernel(Mat x, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch) {
+    const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (k >= pitch) return;
+    for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+        uint16_t o[4][3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split3(k + i < K ? x.p[m * x.rs + (k + i) * x.cs] : 0.f, o[i]);
+#pragma unroll
+        for (int pl = 0; pl < 3; ++pl)
+            *reinterpret_cast<uint2*>(out + (pl * M + m) * pitch + k) =
+                make_uint2(o[0][pl] | ((uint32_t)o[1][pl] << 16), o[2][pl] | ((uint32_t)o[3][pl] << 16));
+    }
+}
+
+// A for the 4-bit product: out[n][k] = code - 8, k up to `pitch` (whole spans). A thread takes a
+// word: 128 + c is a bfloat16 with c in its low bits, and 136 comes off exactly.
+__global__ void __launch_bounds__(256) expand_q4_kernel(q4::Weight q, __nv_bfloat16* out, int64_t pitch) {
+    const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (k >= pitch) return;
+    const int64_t in = k % q4::kSpan;
+    const int64_t w = k / q4::kSpan * q4::kSpanWords + in % 32 / 8 * 4 + in / 32;
+    const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
+    for (int64_t n = blockIdx.y; n < q.N; n += gridDim.y) {
+        const uint32_t word = q.codes[n * q.cp + w];
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+            const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
+            o[i] = *reinterpret_cast<const uint32_t*>(&d);
+        }
+        *reinterpret_cast<uint4*>(out + n * pitch + k) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+// A for the weight gradient: out[k][m] = code value of (m, k), m padded with zeros to `pitch`.
+__global__ void __launch_bounds__(256) expand_q8_kernel(lowbit::Q8 q, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch) {
+    __shared__ uint16_t s[64][66];
+    const int64_t k0 = (int64_t)blockIdx.x * 64;
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int64_t mt = blockIdx.y; mt * 64 < pitch; mt += gridDim.y) {
+        const int64_t m0 = mt * 64;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t m = m0 + ty + 4 * i, k = k0 + tx;
+            float v = 0.f;
+            if (m < M && k < K)
+                v = lowbit::code_value(q.codes[m * q.cp + k], q.fmt) * lowbit::scale_value(q.scales[m * q.sp + k / lowbit::kBlock]);
+            s[tx][ty + 4 * i] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+        }
+        __syncthreads();
+        const int64_t m = m0 + 2 * lane;
+        if (m < pitch) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t k = k0 + warp * 8 + i;
+                if (k >= K) break;
+                *reinterpret_cast<uint32_t*>(out + k * pitch + m) = *reinterpret_cast<const uint32_t*>(&s[warp * 8 + i][2 * lane]);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace planes
+}  // namespace mt
