@@ -9,6 +9,7 @@
 #include "lowbit_common.cuh"
 #include "planes_gemm.cuh"
 #include "q4.cuh"
+#include "q4_gemv.cuh"
 #include "q8.cuh"
 #include "rms_norm.cuh"
 
@@ -370,6 +371,95 @@ int linear_q4_planes(const Mat& x, const mt::q4::Weight& w, const float* bias, c
     return run_planes<true>(p, a, b, pitch, st, who);
 }
 
+// ------------------------------- 4 bits, few rows -------------------------------------
+
+constexpr size_t kMaxSmem = 232448;
+
+template <int NT, int G>
+int launch_gemv(const mt::q4::Gemv& p, dim3 grid, cudaStream_t st, const char* who) {
+    static std::atomic<uint64_t> smem_set{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(smem_set.load() & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(mt::q4::gemv_kernel<NT, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
+        if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
+        smem_set.fetch_or(bit);
+    }
+    mt::q4::gemv_kernel<NT, G><<<grid, mt::q4::kGemvThreads, mt::q4::gemv_smem(NT, G, p.spans), st>>>(p);
+    return launched(who);
+}
+template <int NT>
+int launch_gemv(const mt::q4::Gemv& p, dim3 grid, cudaStream_t st, const char* who) {
+    switch (p.w.group) {
+        case 32: return launch_gemv<NT, 32>(p, grid, st, who);
+        case 64: return launch_gemv<NT, 64>(p, grid, st, who);
+        default: return launch_gemv<NT, 128>(p, grid, st, who);
+    }
+}
+
+int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, const Mat& y, int64_t M, int relu,
+                   cudaStream_t st, const char* who) {
+    using namespace mt::q4;
+    const int64_t spans = (w.K + kSpan - 1) / kSpan;
+    // Rows per CTA: as many as 16, but rather fewer (their CTAs read the weights again, from
+    // L2) than K in several launches, down to 4.
+    int64_t chunks = (M + 2 * kGemvMaxTiles - 1) / (2 * kGemvMaxTiles);
+    int64_t rows = (M + chunks - 1) / chunks;
+    while (rows > 4 && gemv_smem((int)(rows + 1) / 2, w.group, (int)spans) > kMaxSmem) {
+        ++chunks;
+        rows = (M + chunks - 1) / chunks;
+    }
+    if (chunks > 65535) return fail(MT_EUNSUPPORTED, "%s: too many rows", who);
+    const int nt = (int)(rows + 1) / 2;
+    int64_t most = std::max<int64_t>(1, spans);
+    while (most > 1 && gemv_smem(nt, w.group, (int)most) > kMaxSmem) most = (most + 1) / 2;
+    const int sms = mt::host::sm_count();
+    const int64_t ctas = std::max<int64_t>(1, sms / chunks);
+    Gemv p{};
+    p.x = x.m;
+    p.w = w;
+    p.bias = bias;
+    p.y = y;
+    p.M = M;
+    p.rows = (int)rows;
+    p.relu = relu;
+    p.tiles = (int)((w.N + 15) / 16);
+    p.xvec = vec4(x);
+    const int64_t launches = spans ? (spans + most - 1) / most : 1;   // no inputs: the bias alone
+    for (int64_t i = 0; i < launches; ++i) {
+        const int64_t s0 = i * most;
+        p.span0 = (int)s0;
+        p.spans = (int)std::min(most, spans - s0);
+        p.accumulate = i > 0;
+        p.finish = i == launches - 1;
+        // Warps per tile: rounds x (spans per warp and the sums' way through shared memory, which
+        // takes about as long as two spans).
+        int64_t least = INT64_MAX;
+        for (int kp = 1; kp <= kGemvWarps; kp *= 2) {
+            const int64_t per_round = ctas * (kGemvWarps / kp);
+            const int64_t cost = (p.tiles + per_round - 1) / per_round * ((p.spans + kp - 1) / kp + 2);
+            if (cost < least) { least = cost; p.kp = kp; }
+        }
+        const int per_cta = kGemvWarps / p.kp;
+        const dim3 grid(grid_of((p.tiles + per_cta - 1) / per_cta, ctas), (unsigned)chunks);
+        switch (nt) {
+            case 1: MT_TRY(launch_gemv<1>(p, grid, st, who)); break;
+            case 2: MT_TRY(launch_gemv<2>(p, grid, st, who)); break;
+            case 3: MT_TRY(launch_gemv<3>(p, grid, st, who)); break;
+            case 4: MT_TRY(launch_gemv<4>(p, grid, st, who)); break;
+            case 5: MT_TRY(launch_gemv<5>(p, grid, st, who)); break;
+            case 6: MT_TRY(launch_gemv<6>(p, grid, st, who)); break;
+            case 7: MT_TRY(launch_gemv<7>(p, grid, st, who)); break;
+            default: MT_TRY(launch_gemv<8>(p, grid, st, who)); break;
+        }
+    }
+    char path[96];
+    snprintf(path, sizeof path, "%s gemv kp=%d rows=%d x %d", who, p.kp, (int)rows, (int)chunks);
+    mt::host::set_path(path);
+    return MT_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -639,13 +729,9 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     for (int i = 0; i < 4; ++i) MT_TRY(check_apart(span_of(vy), "Y", in[i], names[i], who));
     const int64_t M = vx.rows;
     if (M * w.N == 0) return MT_OK;
-    if (M > 8 && w.K > 0)
-        return linear_q4_planes(vx.m, w, vb.m.p, vy.m, M, relu, static_cast<cudaStream_t>(stream), who);
-    mt::q4::linear_simple_kernel<<<dim3((unsigned)((w.N + 7) / 8), grid_of((M + 3) / 4, 65535)), 256, 0,
-                                   static_cast<cudaStream_t>(stream)>>>(vx.m, w, vb.m.p, vy.m, M, relu);
-    MT_TRY(launched("linear_fwd_q4 launch"));
-    mt::host::set_path("linear_fwd_q4 simple");
-    return MT_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (M > 64 && w.K > 0) return linear_q4_planes(vx.m, w, vb.m.p, vy.m, M, relu, st, who);
+    return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
 }
 
 }  // extern "C"

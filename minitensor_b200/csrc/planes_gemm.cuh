@@ -39,6 +39,7 @@ constexpr uint32_t A_BYTES = 128 * BK * 2;
 constexpr uint32_t B_BYTES = 128 * BK * 2;            // one plane
 constexpr uint32_t STAGE_BYTES = A_BYTES + 3 * B_BYTES;
 constexpr uint32_t RING_BYTES = STAGE_BYTES * STAGES;
+constexpr float kCodeUnit = 2048.f;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
 constexpr uint32_t EPI_BYTES = EPI_WARPS * 32 * 33 * 4;
@@ -242,13 +243,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
             float* out = p.splits > 1 ? p.part + (int64_t)sp * p.R * p.C : p.out;
             const int64_t os_r = p.splits > 1 ? p.C : p.os_r, os_c = p.splits > 1 ? 1 : p.os_c;
-            if (SCALED && p.splits == 1) {
+            if (SCALED) {
                 const int row = row0 + lane;
-                const float b = p.bias && row < p.R ? p.bias[row] : 0.f;
+                const bool whole = p.splits == 1;
+                const float b = whole && p.bias && row < p.R ? p.bias[row] : 0.f;
 #pragma unroll
                 for (int j = 0; j < 128; ++j) {
-                    acc[j] += b;
-                    if (p.relu) acc[j] = acc[j] > 0.f ? acc[j] : 0.f;
+                    acc[j] = fmaf(acc[j], kCodeUnit, b);
+                    if (whole && p.relu) acc[j] = acc[j] > 0.f ? acc[j] : 0.f;
                 }
             }
             if (os_r == 1) {
@@ -384,21 +386,24 @@ __global__ void __launch_bounds__(256) split_cols_kernel(Mat x, __nv_bfloat16* o
     }
 }
 
-// A for the 4-bit product: out[n][k] = code - 8, k up to `pitch` (whole spans). A thread takes a
-// word: 128 + c is a bfloat16 with c in its low bits, and 136 comes off exactly.
+// A for the 4-bit product: out[n][k] = (code - 8) / kCodeUnit, k up to `pitch` (whole spans). A
+// thread takes a word: 128 + c is a bfloat16 with c in its low bits, and 136 comes off exactly.
+// The unit keeps the sum over a group, at most 128 * 8 times the largest x, within x's range
+// until the group's scale meets it; the tile is multiplied by it when it is done.
 __global__ void __launch_bounds__(256) expand_q4_kernel(q4::Weight q, __nv_bfloat16* out, int64_t pitch) {
     const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (k >= pitch) return;
     const int64_t in = k % q4::kSpan;
     const int64_t w = k / q4::kSpan * q4::kSpanWords + in % 32 / 8 * 4 + in / 32;
     const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
+    const __nv_bfloat162 unit = __floats2bfloat162_rn(1.f / kCodeUnit, 1.f / kCodeUnit);
     for (int64_t n = blockIdx.y; n < q.N; n += gridDim.y) {
         const uint32_t word = q.codes[n * q.cp + w];
         uint32_t o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t v = ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-            const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
+            const __nv_bfloat162 d = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off), unit);
             o[i] = *reinterpret_cast<const uint32_t*>(&d);
         }
         *reinterpret_cast<uint4*>(out + n * pitch + k) = make_uint4(o[0], o[1], o[2], o[3]);

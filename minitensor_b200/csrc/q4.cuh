@@ -81,36 +81,5 @@ __global__ void __launch_bounds__(128) dequantize_kernel(Weight q, Mat w) {
     }
 }
 
-// Simple form of y = x W + b: a warp per output column and 4 rows of x, float FMA.
-__global__ void __launch_bounds__(256) linear_simple_kernel(Mat x, Weight q, const float* bias, Mat y, int64_t rows,
-                                                            int relu) {
-    const int lane = threadIdx.x & 31;
-    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (n >= q.N) return;
-    const int64_t words = (q.K + kSpan - 1) / kSpan * kSpanWords;
-    for (int64_t m0 = (int64_t)blockIdx.y * 4; m0 < rows; m0 += (int64_t)gridDim.y * 4) {
-        float acc[4] = {};
-        for (int64_t w = lane; w < words; w += 32) {
-            const uint32_t word = q.codes[n * q.cp + w];
-            const int64_t k0 = word_k(w);
-            if (k0 >= q.K) continue;
-            const float s = __bfloat162float(q.scales[n * q.sp + k0 / q.group]);
-            for (int j = 0; j < 8 && k0 + j < q.K; ++j) {
-                const float v = (float)((int)((word >> code_shift(j)) & 15u) - 8) * s;
-                for (int i = 0; i < 4; ++i)
-                    if (m0 + i < rows) acc[i] = fmaf(x.p[(m0 + i) * x.rs + (k0 + j) * x.cs], v, acc[i]);
-            }
-        }
-        for (int i = 0; i < 4; ++i) {
-            float v = lowbit::warp_sum(acc[i]);
-            if (lane == 0 && m0 + i < rows) {
-                if (bias) v += bias[n];
-                if (relu) v = v > 0.f ? v : 0.f;
-                y.p[(m0 + i) * y.rs + n * y.cs] = v;
-            }
-        }
-    }
-}
-
 }  // namespace q4
 }  // namespace mt

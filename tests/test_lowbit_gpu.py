@@ -360,14 +360,23 @@ def q4_case(g, M, K, N, group):
     return x, codes, s
 
 
-def check_q4(y, x, W, bias, relu):
-    """A float sum of K terms in any order, the scale's and the bias's roundings."""
-    want, mag = x.double() @ W, x.double().abs() @ W.abs()
+def check_q4(y, x, codes, s, group, bias, relu):
+    """Many rows: y is the sum over groups of s * sum (c - 8) x; a tensor-core step aligns 17
+    terms to the largest and may drop 2 u of it from each (34 u), 24 steps meet in one
+    accumulator at 2 u each, the groups are added as a float sum of at most K terms, and the
+    scale's product and the bias add 2 u. Few rows: the products and sums are exact integers
+    after x is rounded to 2^-30 of the largest of its span of 128 (2^-6 u); two conversions, two
+    products and the bias add 5 u, the spans a float sum. Either way fewer than K + 90."""
+    K = x.shape[1]
+    W = R.q4_weight(codes, s, group)
+    full = s.double().repeat_interleave(group, 1)[:, :K].t()
+    spans = torch.nn.functional.pad(x.double().abs(), (0, -K % 128)).view(x.shape[0], -1, 128)
+    top = spans.amax(2, keepdim=True).expand_as(spans).reshape(x.shape[0], -1)[:, :K]
+    want, mag = x.double() @ W, x.double().abs() @ (W.abs() + 8 * full) + 2.0 ** -6 * (top @ W.abs())
     if bias is not None:
         want, mag = want + bias.double(), mag + bias.double().abs()
-    K = x.shape[1]
     err = host(y).double() - (want.clamp_min(0) if relu else want)
-    assert R.worst(err, mag) <= K + 8
+    assert R.worst(err, mag) <= K + 90
 
 
 Q4_ROWS = [1, 2, 3, 5, 8, 9, 16, 21, 40, 130, 300]
@@ -383,7 +392,7 @@ def test_linear_forward_q4(mt, M, K, N, group):
     relu = M % 2 == 0
     w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, group)
     y = mt.linear_forward_q4(x.cuda(), w, bias=bias.cuda() if bias is not None else None, relu=relu)
-    check_q4(y, x, R.q4_weight(codes, s, group), bias, relu)
+    check_q4(y, x, codes, s, group, bias, relu)
 
 
 @pytest.mark.parametrize("layout", LAYOUTS)
@@ -392,23 +401,59 @@ def test_linear_forward_q4_layouts(mt, layout, M):
     g = gen(M)
     x, codes, s = q4_case(g, M, 260, 50, 64)
     w = mt.Q4Weight(R.q4_pack(codes, 260).cuda(), s.cuda(), 260, 64)
-    check_q4(mt.linear_forward_q4(strided(x, layout), w), x, R.q4_weight(codes, s, 64), None, False)
+    check_q4(mt.linear_forward_q4(strided(x, layout), w), x, codes, s, 64, None, False)
 
 
 @pytest.mark.parametrize("M", Q4_ROWS)
-def test_linear_forward_q4_keeps_every_bit(mt, M):
-    """Weights with one code other than 8 in a column: y is x's value times code times scale, so
-    at most the three exact parts and the scale round; every position of K is met."""
-    K, N, group = 288, 288, 32
+@pytest.mark.parametrize("offset", [0, 37, 150])
+def test_linear_forward_q4_finds_every_position(mt, M, offset):
+    """Rows of x with a single value: y is s * (c - 8) * x. x's parts and digits are exact; at most
+    three products and sums round, the tensor core's by truncation (2 u). A lost part of x
+    (2^-8 or 2^-16 of it) is far off."""
+    K, N, group = 288, 80, 32
     g = gen(M)
-    x = rand(g, M, K) * torch.exp(5 * rand(g, M, K))
-    codes = torch.full((N, K), 8, dtype=torch.int64)
-    n = torch.arange(N)
-    codes[n, n] = torch.where(n % 15 < 8, n % 15, n % 15 + 1)
+    at = (torch.arange(M) * 11 + offset) % K
+    x = torch.zeros(M, K)
+    x[torch.arange(M), at] = rand(g, M) * torch.exp(5 * rand(g, M))
+    codes = torch.randint(0, 16, (N, K), generator=g)
     s = torch.exp(rand(g, N, K // group)).to(torch.bfloat16)
     w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, group)
     want = x.double() @ R.q4_weight(codes, s, group)
-    assert R.worst(host(mt.linear_forward_q4(x.cuda(), w)) - want, want) <= 4
+    assert R.worst(host(mt.linear_forward_q4(x.cuda(), w)) - want, want) <= 7
+
+
+def test_linear_forward_q4_range_of_x(mt):
+    """Blocks of x from 2^-120 to 2^125 in one call."""
+    K, N = 512, 48
+    g = gen(5)
+    for M in (1, 6, 20):
+        for top in (125, 100):
+            x, codes, s = q4_case(g, M, K, N, 64)
+            e = torch.randint(-120, top, (M, K // 32), generator=g).repeat_interleave(32, 1)
+            x = torch.ldexp(torch.rand(M, K, generator=g) + 0.5, e)
+            x[0, :32] = 1.5 * 2.0 ** top
+            s = (s.float() * 1e-6).to(torch.bfloat16)
+            w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, 64)
+            check_q4(mt.linear_forward_q4(x.cuda(), w), x, codes, s, 64, None, False)
+
+
+@pytest.mark.parametrize("M,K", [(16, 12800), (5, 24000), (1, 60000)])
+def test_linear_forward_q4_long_rows(mt, M, K):
+    """Rows of x that do not fit shared memory at once."""
+    g = gen(K)
+    x, codes, s = q4_case(g, M, K, 33, 128)
+    w = mt.Q4Weight(pack_fast(codes, K).cuda(), s.cuda(), K, 128)
+    bias = rand(g, 33)
+    check_q4(mt.linear_forward_q4(x.cuda(), w, bias=bias.cuda(), relu=True), x, codes, s, 128, bias, True)
+
+
+def pack_fast(codes, K):
+    """R.q4_pack for long rows: spans of 128 codes are packed alike."""
+    N = codes.shape[0]
+    spans = -(-K // 128)
+    full = torch.full((N, spans * 128), 8, dtype=torch.int64)
+    full[:, :K] = codes
+    return R.q4_pack(full.view(N * spans, 128), 128).view(N, spans * 64)
 
 
 def test_linear_forward_q4_non_finite(mt):
@@ -445,7 +490,7 @@ def test_decoding_step(mt):
     w = mt.quantize_q4(W.cuda(), 64)
     n = mt.rms_norm(x.cuda(), gamma.cuda(), residual=r.cuda())
     y = mt.linear_forward_q4(n.y, w)
-    check_q4(y, host(n.y), host(mt.dequantize_q4(w)).double(), None, False)
+    check_q4(y, host(n.y), *R.q4_quantize(W, 64), 64, None, False)
     n2 = mt.rms_norm(y, gamma.cuda(), residual=n.h, inplace=True)
     h, rstd, want = R.rms_norm(host(n2.h), None, gamma, 1e-6)
     assert R.worst(host(n2.y) - want, want) <= norm_bound(K) + 1
