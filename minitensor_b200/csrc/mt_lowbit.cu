@@ -424,7 +424,10 @@ int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, c
     p.M = M;
     p.rows = (int)rows;
     p.relu = relu;
-    p.tiles = (int)((w.N + 15) / 16);
+    const int64_t tiles = (w.N + 15) / 16;
+    const dim3 grid(grid_of(tiles, ctas), (unsigned)chunks);
+    p.tiles_each = (int)(tiles / grid.x);
+    p.tiles_more = (int)(tiles % grid.x);
     p.xvec = vec4(x);
     const int64_t launches = spans ? (spans + most - 1) / most : 1;   // no inputs: the bias alone
     for (int64_t i = 0; i < launches; ++i) {
@@ -433,16 +436,6 @@ int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, c
         p.spans = (int)std::min(most, spans - s0);
         p.accumulate = i > 0;
         p.finish = i == launches - 1;
-        // Warps per tile: rounds x (spans per warp and the sums' way through shared memory, which
-        // takes about as long as two spans).
-        int64_t least = INT64_MAX;
-        for (int kp = 1; kp <= kGemvWarps; kp *= 2) {
-            const int64_t per_round = ctas * (kGemvWarps / kp);
-            const int64_t cost = (p.tiles + per_round - 1) / per_round * ((p.spans + kp - 1) / kp + 2);
-            if (cost < least) { least = cost; p.kp = kp; }
-        }
-        const int per_cta = kGemvWarps / p.kp;
-        const dim3 grid(grid_of((p.tiles + per_cta - 1) / per_cta, ctas), (unsigned)chunks);
         switch (nt) {
             case 1: MT_TRY(launch_gemv<1>(p, grid, st, who)); break;
             case 2: MT_TRY(launch_gemv<2>(p, grid, st, who)); break;
@@ -455,7 +448,7 @@ int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, c
         }
     }
     char path[96];
-    snprintf(path, sizeof path, "%s gemv kp=%d rows=%d x %d", who, p.kp, (int)rows, (int)chunks);
+    snprintf(path, sizeof path, "%s gemv rows=%d x %d", who, (int)rows, (int)chunks);
     mt::host::set_path(path);
     return MT_OK;
 }

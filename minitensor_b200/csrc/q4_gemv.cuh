@@ -18,10 +18,12 @@
 // A span that holds an infinity or a NaN has no fixed point; a CTA that meets one computes its
 // tiles by float FMA.
 //
-// Work. A CTA of 16 warps keeps its rows of x in shared memory and walks over tiles of 16 weight
-// rows; kp warps share a tile, each taking a part of its spans. Four spans of codes and
-// scales are in flight per warp, across tiles. The warps' sums meet in shared memory and are
-// added in order. blockIdx.y takes up to 16 rows of x each.
+// Work. A CTA of 16 warps keeps its rows of x in shared memory and has a run of tiles of 16
+// weight rows, whose spans, taken tile after tile, are cut into 16 equal parts: one barrier,
+// then a tile's partial sums are added in order. A warp's codes come GROUP spans (4 or
+// 2 KB) at a time by cp.async, two groups in flight: each lane copies the pieces that it will read, so
+// nothing but its own wait stands between. The scales of a group are spread over the four
+// lanes of a row. blockIdx.y takes up to 16 rows of x each.
 #pragma once
 
 #include "q4.cuh"
@@ -31,7 +33,6 @@ namespace q4 {
 
 constexpr int kGemvWarps = 16;
 constexpr int kGemvThreads = 32 * kGemvWarps;
-constexpr int kGemvDepth = 4;          // spans in flight per warp
 constexpr int kGemvMaxTiles = 8;       // 8-column tiles: 16 rows of x
 
 struct Gemv {
@@ -44,17 +45,27 @@ struct Gemv {
     int relu;
     int span0, spans;                  // this launch's part of K, in spans
     int accumulate, finish;            // y holds the sum over earlier spans; bias and ReLU are due
-    int kp;                            // warps per tile: 1, 2, 4, 8 or 16
-    int tiles;                         // of 16 weight rows
+    int tiles_each, tiles_more;        // tiles of 16 weight rows per blockIdx.x, and CTAs that have one more
     int xvec;                          // rows of x on 16-byte boundaries, unit stride
 };
 
+// Spans per copy group; more columns leave less room and need less of it.
+__host__ __device__ constexpr int gemv_group(int nt) { return nt == 1 ? 4 : 2; }
+// Bytes of a warp's two groups.
+__host__ __device__ constexpr int gemv_ring(int nt) { return 2 * gemv_group(nt) * 1024; }
+// Spans in shared memory: whole groups, zeros behind the last span.
+__host__ __device__ constexpr int gemv_pad(int nt, int spans) {
+    return (spans + gemv_group(nt) - 1) / gemv_group(nt) * gemv_group(nt);
+}
+// Tiles of a CTA between two barriers; with its warps they make the partial sums.
+__host__ __device__ constexpr int gemv_run(int nt) { return 192 / nt - (kGemvWarps - 1); }
+
 // Shared memory: digits [8 NT columns][spans * 128 + 16] (the 16 put neighbouring columns on other
-// banks), accumulator starts [2 NT rows][2][spans * segments] of two ints, powers of two
-// [2 NT rows][2][spans], sums [warps][16][2 NT].
+// banks), accumulator starts and powers of two [2 NT rows][2][spans * segments + 1] of 16 bytes,
+// partial sums [run + 15][16][2 NT], codes [warps][2][group][rows g, g + 8][lanes] of 16 bytes.
 __host__ __device__ constexpr size_t gemv_smem(int nt, int group, int spans) {
-    return (size_t)8 * nt * (spans * kSpan + 16) + (size_t)4 * nt * spans * (kSpan / group) * 8 +
-           (size_t)4 * nt * spans * 4 + (size_t)kGemvWarps * 16 * 2 * nt * 4;
+    return (size_t)8 * nt * (gemv_pad(nt, spans) * kSpan + 16) + (size_t)4 * nt * (gemv_pad(nt, spans) * (kSpan / group) + 1) * 16 +
+           (size_t)(gemv_run(nt) + kGemvWarps - 1) * 16 * 2 * nt * 4 + (size_t)kGemvWarps * gemv_ring(nt);
 }
 
 __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -69,26 +80,43 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, 
 // A warp takes a span, a lane 4 of its features. A word's bytes are masked out as codes
 // 0 4 1 5 and 2 6 3 7 of its 8, the digits go in that order.
 template <int NT, int G>
-__device__ __forceinline__ bool gemv_stage_x(const Gemv& p, uint8_t* xs, int2* zi, float* fs) {
-    constexpr int SEG = kSpan / G;
+__device__ __forceinline__ bool gemv_stage_x(const Gemv& p, uint8_t* xs, int4* zs) {
+    constexpr int SEG = kSpan / G, WARPS = kGemvWarps;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int col_bytes = p.spans * kSpan + 16;
+    const int spans = gemv_pad(NT, p.spans), col_bytes = spans * kSpan + 16;
     const int64_t m0 = (int64_t)blockIdx.y * p.rows;
     int bad = 0;
-    for (int i = warp; i < 2 * NT * p.spans; i += kGemvWarps) {
-        const int r = i / p.spans, s = i - r * p.spans;
+    constexpr int BATCH = 4;   // spans whose loads are in flight together
+    for (int i0 = warp; i0 < 2 * NT * spans; i0 += BATCH * WARPS) {
+    float vs[BATCH][4];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        const int i = i0 + u * WARPS, r = i / spans, s = i - r * spans;
         const int64_t m = m0 + r, k = (int64_t)(p.span0 + s) * kSpan + lane * 4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (r < p.rows && m < p.M) {
+        vs[u][0] = vs[u][1] = vs[u][2] = vs[u][3] = 0.f;
+        if (r < p.rows && m < p.M && s < p.spans) {
             if (p.xvec && k + 4 <= p.w.K) {
                 const float4 q = *reinterpret_cast<const float4*>(p.x.p + m * p.x.rs + k);
-                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+                vs[u][0] = q.x; vs[u][1] = q.y; vs[u][2] = q.z; vs[u][3] = q.w;
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (k + j < p.w.K) v[j] = p.x.p[m * p.x.rs + (k + j) * p.x.cs];
+                    if (k + j < p.w.K) vs[u][j] = p.x.p[m * p.x.rs + (k + j) * p.x.cs];
             }
         }
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        const int i = i0 + u * WARPS, r = i / spans, s = i - r * spans;
+        if (r >= 2 * NT) break;
+        if (r >= p.rows) {   // no row of x: zeros
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint32_t*>(xs + (size_t)(4 * r + j) * col_bytes + s * kSpan + lane * 4) = 0;
+            if (lane < 2 * SEG) zs[(2 * r + lane / SEG) * (spans * SEG + 1) + s * SEG + lane % SEG] = make_int4(0, 0, 0, 0);
+            continue;
+        }
+        const float (&v)[4] = vs[u];
         uint32_t a = max(max(lowbit::abs_bits(v[0]), lowbit::abs_bits(v[1])),
                          max(lowbit::abs_bits(v[2]), lowbit::abs_bits(v[3])));
         a = __reduce_max_sync(0xffffffffu, a);
@@ -119,20 +147,17 @@ __device__ __forceinline__ bool gemv_stage_x(const Gemv& p, uint8_t* xs, int2* z
             for (int w = 1; w < G / 4; w <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], w);
         }
         if (lane % (G / 4) == 0) {
-            const int at = s * SEG + lane / (G / 4);
-            zi[(2 * r) * p.spans * SEG + at] = make_int2(-8 * sum[0], -8 * sum[1]);
-            zi[(2 * r + 1) * p.spans * SEG + at] = make_int2(-8 * sum[2], -8 * sum[3]);
-        }
-        if (lane == 0) {
+            const int at = 2 * r * (spans * SEG + 1) + s * SEG + lane / (G / 4);
             const float f = __uint_as_float((uint32_t)(e - 29) << 23);
-            fs[(2 * r) * p.spans + s] = f;
-            fs[(2 * r + 1) * p.spans + s] = f * 65536.f;
+            zs[at] = make_int4(-8 * sum[0], -8 * sum[1], __float_as_int(f), 0);
+            zs[at + spans * SEG + 1] = make_int4(-8 * sum[2], -8 * sum[3], __float_as_int(f * 65536.f), 0);
         }
+    }
     }
     return __syncthreads_or(bad) == 0;
 }
 
-// The sums of one tile by float FMA, for x that is not finite.
+// A warp's part of one tile, spans [s0, s1), by float FMA: for x that is not finite.
 template <int NT>
 __device__ __noinline__ void gemv_tile_float(const Gemv& p, int64_t tile, int s0, int s1, float* red) {
     const int lane = threadIdx.x & 31;
@@ -156,97 +181,187 @@ __device__ __noinline__ void gemv_tile_float(const Gemv& p, int64_t tile, int s0
     }
 }
 
-// All warps of the CTA, from different places of their loops.
-__device__ __forceinline__ void gemv_barrier() { asm volatile("barrier.sync 1, %0;" ::"n"(kGemvThreads) : "memory"); }
-
 template <int NT, int G>
 __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
-    constexpr int SEG = kSpan / G;
+    constexpr int SEG = kSpan / G, GROUP = gemv_group(NT), WARPS = kGemvWarps;
     extern __shared__ __align__(16) uint8_t gemv_smem_raw[];
-    const int col_bytes = p.spans * kSpan + 16;
+    const int spans = gemv_pad(NT, p.spans), col_bytes = spans * kSpan + 16;
     uint8_t* xs = gemv_smem_raw;
-    int2* zi = reinterpret_cast<int2*>(xs + (size_t)8 * NT * col_bytes);
-    float* fs = reinterpret_cast<float*>(zi + (size_t)4 * NT * p.spans * SEG);
-    float* red = fs + (size_t)4 * NT * p.spans;
-
+    int4* zs = reinterpret_cast<int4*>(xs + (size_t)8 * NT * col_bytes);
+    float* red = reinterpret_cast<float*>(zs + (size_t)4 * NT * (spans * SEG + 1));
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int part = warp % p.kp, sub = warp / p.kp, per_cta = kGemvWarps / p.kp;
-    const int s0 = p.spans * part / p.kp, ns = p.spans * (part + 1) / p.kp - s0;
-    const int stride = (int)gridDim.x * per_cta;
-    const int first = (int)blockIdx.x * per_cta;
-    const int rounds = p.tiles > first ? (p.tiles - first + stride - 1) / stride : 0;   // the same for all warps
+    uint4* ring = reinterpret_cast<uint4*>(red + (gemv_run(NT) + WARPS - 1) * 16 * 2 * NT) +
+                  warp * (gemv_ring(NT) / 16) + lane;
 
-    uint4 wa[kGemvDepth], wb[kGemvDepth];
-    uint16_t sa[kGemvDepth][SEG], sb[kGemvDepth][SEG];
-    // Load cursor: rows g and g + 8 of a round's tile, from this warp's first span on.
-    const uint4 *la = nullptr, *lb = nullptr;
-    const uint16_t *ga = nullptr, *gb = nullptr;
-    int l_round = -1, l_s = ns;
-    // Groups of the last span that K reaches; those behind it have no scale.
-    const int groups = (int)((p.w.K + G - 1) / G) - (p.span0 + s0) * SEG;
-    auto fetch = [&](int d) {
-        if (l_s == ns) {
-            l_s = 0;
-            if (++l_round < rounds) {
-                const int64_t n = ((int64_t)first + sub + (int64_t)l_round * stride) * 16 + g;
-                const int64_t na = min(n, p.w.N - 1), nb = min(n + 8, p.w.N - 1);
-                const int64_t at = (int64_t)(p.span0 + s0) * 4 + t;
-                la = reinterpret_cast<const uint4*>(p.w.codes + na * p.w.cp) + at;
-                lb = reinterpret_cast<const uint4*>(p.w.codes + nb * p.w.cp) + at;
-                const uint16_t* s = reinterpret_cast<const uint16_t*>(p.w.scales) + (int64_t)(p.span0 + s0) * SEG;
-                ga = s + na * p.w.sp;
-                gb = s + nb * p.w.sp;
-            }
-        }
-        if (l_round >= rounds) return;
-        wa[d] = __ldcs(la + l_s * 4);
-        wb[d] = __ldcs(lb + l_s * 4);
-#pragma unroll
-        for (int i = 0; i < SEG; ++i) {
-            const int at = l_s * SEG + i;
-            sa[d][i] = at < groups ? __ldg(ga + at) : (uint16_t)0;
-            sb[d][i] = at < groups ? __ldg(gb + at) : (uint16_t)0;
-        }
-        ++l_s;
-    };
-    if (ns > 0) {
-#pragma unroll
-        for (int d = 0; d < kGemvDepth; ++d) fetch(d);
-    }
-    const bool fast = gemv_stage_x<NT, G>(p, xs, zi, fs);   // ends with a __syncthreads
+    // This CTA's tiles, in runs whose partial sums fit.
+    const int gpt = spans / GROUP;   // groups per tile
+    const int cta0 = (int)blockIdx.x * p.tiles_each + min((int)blockIdx.x, p.tiles_more);
+    const int cta1 = cta0 + p.tiles_each + ((int)blockIdx.x < p.tiles_more ? 1 : 0);
+    const int scales = (int)((p.w.K + G - 1) / G) - p.span0 * SEG;   // of a row, from this launch's first span on
+    // Groups that begin before this span have all their spans and scales.
+    const int whole = min(p.spans, scales / SEG) / GROUP * GROUP;
+    const int64_t m0 = (int64_t)blockIdx.y * p.rows;
+    bool fast = true;
 
-    float tot[NT][2];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) tot[i][0] = tot[i][1] = 0.f;
-    int round = 0;
+    for (int tile0 = cta0; tile0 < cta1; tile0 += gemv_run(NT)) {
+        const int tiles = min(gemv_run(NT), cta1 - tile0);
+        const int total = tiles * gpt;
+        const int lo = (int)((int64_t)total * warp / WARPS), hi = (int)((int64_t)total * (warp + 1) / WARPS);
 
-    // One round is over for this warp: its sums to shared memory, then the CTA adds them up.
-    auto flush = [&]() {
-        float* mine = red + warp * 16 * 2 * NT;
-        if (fast) {
+        // Copy cursor: rows g and g + 8 of a tile, at a group's first span.
+        const uint4 *la = nullptr, *lb = nullptr;
+        const uint16_t *ga = nullptr, *gb = nullptr;
+        int l_i = lo, l_tile = gpt ? lo / gpt : 0, l_s = (lo - l_tile * gpt) * GROUP;
+        const uint32_t ring32 = smem_u32(ring);
+        uint32_t to = ring32;
+        uint16_t sa[SEG], sb[SEG];   // scales of span t of the group fetched last
+        auto place = [&]() {
+            const int64_t n = (int64_t)(tile0 + l_tile) * 16 + g;
+            const int64_t na = min(n, p.w.N - 1), nb = min(n + 8, p.w.N - 1);
+            const int64_t at = (int64_t)(p.span0 + l_s) * 4 + t;
+            la = reinterpret_cast<const uint4*>(p.w.codes + na * p.w.cp) + at;
+            lb = reinterpret_cast<const uint4*>(p.w.codes + nb * p.w.cp) + at;
+            const uint16_t* s = reinterpret_cast<const uint16_t*>(p.w.scales) + (int64_t)(p.span0 + l_s + t) * SEG;
+            ga = s + na * p.w.sp;
+            gb = s + nb * p.w.sp;
+        };
+        if (lo < hi) place();
+        auto fetch = [&]() {
+            if (l_i < hi) {
+                if (l_s < whole) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                // Lanes t and t ^ 1 hold the low and the high digits of a row.
-                const float a = tot[i][0] + __shfl_xor_sync(0xffffffffu, tot[i][0], 1);
-                const float b = tot[i][1] + __shfl_xor_sync(0xffffffffu, tot[i][1], 1);
-                if ((t & 1) == 0) {
-                    mine[g * 2 * NT + i * 2 + t / 2] = a;
-                    mine[(g + 8) * 2 * NT + i * 2 + t / 2] = b;
+                    for (int j = 0; j < GROUP; ++j) {
+                        cp_async16(to + j * 1024, la + j * 4);
+                        cp_async16(to + j * 1024 + 512, lb + j * 4);
+                    }
+                    if (GROUP == 4 || t < GROUP) {
+#pragma unroll
+                        for (int i = 0; i < SEG; ++i) {
+                            sa[i] = __ldg(ga + i);
+                            sb[i] = __ldg(gb + i);
+                        }
+                    }
+                    la += GROUP * 4;
+                    lb += GROUP * 4;
+                    ga += GROUP * SEG;
+                    gb += GROUP * SEG;
+                } else {   // the row ends in this group
+#pragma unroll
+                    for (int j = 0; j < GROUP; ++j) {
+                        if (l_s + j < p.spans) {
+                            cp_async16(to + j * 1024, la + j * 4);
+                            cp_async16(to + j * 1024 + 512, lb + j * 4);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < SEG; ++i) {
+                        const bool in = t < GROUP && l_s + t < p.spans && (l_s + t) * SEG + i < scales;
+                        sa[i] = in ? __ldg(ga + i) : (uint16_t)0;
+                        sb[i] = in ? __ldg(gb + i) : (uint16_t)0;
+                    }
                 }
-                tot[i][0] = tot[i][1] = 0.f;
+                ++l_i;
+                to = to == ring32 ? ring32 + GROUP * 1024 : ring32;
+                l_s += GROUP;
+                if (l_s >= spans && l_i < hi) { l_s = 0; ++l_tile; place(); }
+            }
+            cp_async_commit();
+        };
+        fetch();
+        if (tile0 == cta0) fast = gemv_stage_x<NT, G>(p, xs, zs);   // ends with a __syncthreads
+
+        int tile = gpt ? lo / gpt : 0, c_s = (lo - tile * gpt) * GROUP;
+        if (fast) {
+            float tot[NT][2];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) tot[i][0] = tot[i][1] = 0.f;
+            const uint8_t* xl = xs + (size_t)g * col_bytes + t * 32;
+            const int4* zl = zs + t * (spans * SEG + 1);   // row t / 2 of an 8-column tile, its low or high digits
+            const uint4* w = ring;
+#pragma unroll 1
+            for (int i = lo; i < hi; ++i) {
+                uint16_t ca[SEG], cb[SEG];
+#pragma unroll
+                for (int k = 0; k < SEG; ++k) { ca[k] = sa[k]; cb[k] = sb[k]; }
+                fetch();
+                cp_async_wait<1>();
+#pragma unroll
+                for (int j = 0; j < GROUP; ++j) {
+                    const uint4 wa = w[j * 64], wb = w[j * 64 + 32];
+                    const uint32_t A[4] = {wa.x, wa.y, wa.z, wa.w};
+                    const uint32_t B[4] = {wb.x, wb.y, wb.z, wb.w};
+                    float fa[SEG], fb[SEG];
+#pragma unroll
+                    for (int k = 0; k < SEG; ++k) {
+                        fa[k] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)ca[k], (lane & 28) + j) << 16);
+                        fb[k] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)cb[k], (lane & 28) + j) << 16);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint8_t* x = xl + nt * 8 * col_bytes + (c_s + j) * kSpan;
+                        const uint4 x0 = *reinterpret_cast<const uint4*>(x), x1 = *reinterpret_cast<const uint4*>(x + 16);
+                        const uint32_t X[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+                        for (int k = 0; k < SEG; ++k) {
+                            const int4 z = zl[nt * 4 * (spans * SEG + 1) + (c_s + j) * SEG + k];
+                            const float f = __int_as_float(z.z);
+                            int acc[4] = {z.x, z.y, z.x, z.y};
+#pragma unroll
+                            for (int b = k * 4 / SEG; b < (k + 1) * 4 / SEG; ++b)
+                                mma_u8s8(acc, A[b] & 0x0F0F0F0Fu, B[b] & 0x0F0F0F0Fu, (A[b] >> 4) & 0x0F0F0F0Fu,
+                                         (B[b] >> 4) & 0x0F0F0F0Fu, X[2 * b], X[2 * b + 1]);
+                            tot[nt][0] = fmaf(f, fa[k] * (float)(acc[0] + 256 * acc[1]), tot[nt][0]);
+                            tot[nt][1] = fmaf(f, fb[k] * (float)(acc[2] + 256 * acc[3]), tot[nt][1]);
+                        }
+                    }
+                }
+                w = w == ring ? ring + GROUP * 64 : ring;
+                c_s += GROUP;
+                if (c_s == spans || i == hi - 1) {
+                    // This warp's part of the tile; parts in order have slots in order.
+                    float* mine = red + (tile + warp) * 16 * 2 * NT;
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) {
+                        // Lanes t and t ^ 1 hold the low and the high digits of a row.
+                        const float a = tot[k][0] + __shfl_xor_sync(0xffffffffu, tot[k][0], 1);
+                        const float b = tot[k][1] + __shfl_xor_sync(0xffffffffu, tot[k][1], 1);
+                        if ((t & 1) == 0) {
+                            mine[g * 2 * NT + k * 2 + t / 2] = a;
+                            mine[(g + 8) * 2 * NT + k * 2 + t / 2] = b;
+                        }
+                        tot[k][0] = tot[k][1] = 0.f;
+                    }
+                    c_s = 0;
+                    ++tile;
+                }
             }
         } else {
-            gemv_tile_float<NT>(p, (int64_t)first + sub + (int64_t)round * stride, s0, s0 + ns, mine);
+            for (int i = lo; i < hi;) {
+                const int n = min(hi - i, gpt - (i - tile * gpt));
+                const int s = (i - tile * gpt) * GROUP;
+                gemv_tile_float<NT>(p, tile0 + tile, min(s, p.spans), min(s + n * GROUP, p.spans),
+                                    red + (tile + warp) * 16 * 2 * NT);
+                i += n;
+                ++tile;
+            }
         }
-        gemv_barrier();
-        const int64_t m0 = (int64_t)blockIdx.y * p.rows;
-        for (int o = threadIdx.x; o < per_cta * 16 * p.rows; o += kGemvThreads) {
-            const int row = o % 16, m = o / 16 % p.rows, ct = o / (16 * p.rows);
-            const float* r = red + (ct * p.kp * 16 + row) * 2 * NT + m;
-            float v = r[0];
-            for (int i = 1; i < p.kp; ++i) v += r[i * 16 * 2 * NT];
-            const int64_t n = ((int64_t)first + ct + (int64_t)round * stride) * 16 + row;
+        cp_async_wait_all();
+        __syncthreads();
+        for (int o = threadIdx.x; o < tiles * 16 * p.rows; o += kGemvThreads) {
+            const int row = o % 16, m = o / 16 % p.rows, tl = o / (16 * p.rows);
+            float v = 0.f;
+            if (gpt) {
+                // Warps whose parts meet the tile: the last w with total * w / warps <= its first
+                // and its last group.
+                const int w0 = ((tl * gpt + 1) * WARPS - 1) / total, w1 = ((tl + 1) * gpt * WARPS - 1) / total;
+                const float* r = red + ((tl + w0) * 16 + row) * 2 * NT + m;
+                v = r[0];
+                for (int w = w0 + 1; w <= w1; ++w)
+                    if ((int)((int64_t)total * w / WARPS) < (int)((int64_t)total * (w + 1) / WARPS))
+                        v += r[(w - w0) * 16 * 2 * NT];
+            }
+            const int64_t n = (int64_t)(tile0 + tl) * 16 + row;
             if (n < p.w.N && m0 + m < p.M) {
                 float* y = p.y.p + (m0 + m) * p.y.rs + n * p.y.cs;
                 if (p.accumulate) v += *y;
@@ -257,53 +372,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
                 *y = v;
             }
         }
-        gemv_barrier();
-        ++round;
-    };
-
-    if (ns == 0 || !fast) {
-        while (round < rounds) flush();
-        return;
-    }
-    const uint8_t* xl = xs + (size_t)g * col_bytes + s0 * kSpan + t * 32;
-    const int2* zl = zi + (t * p.spans + s0) * SEG;   // row t / 2 of the tile, digits' half t & 1
-    const float* fl = fs + t * p.spans + s0;
-    const int items = rounds * ns;
-    int c_s = 0;
-    for (int i0 = 0; i0 < items; i0 += kGemvDepth) {
-#pragma unroll
-        for (int d = 0; d < kGemvDepth; ++d) {
-            if (i0 + d < items) {
-                const uint32_t A[4] = {wa[d].x, wa[d].y, wa[d].z, wa[d].w};
-                const uint32_t B[4] = {wb[d].x, wb[d].y, wb[d].z, wb[d].w};
-                float fa[SEG], fb[SEG];
-#pragma unroll
-                for (int i = 0; i < SEG; ++i) {
-                    fa[i] = __uint_as_float((uint32_t)sa[d][i] << 16);
-                    fb[i] = __uint_as_float((uint32_t)sb[d][i] << 16);
-                }
-                fetch(d);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const uint8_t* x = xl + (size_t)nt * 8 * col_bytes + c_s * kSpan;
-                    const uint4 x0 = *reinterpret_cast<const uint4*>(x), x1 = *reinterpret_cast<const uint4*>(x + 16);
-                    const uint32_t X[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-                    const float f = fl[nt * 4 * p.spans + c_s];
-#pragma unroll
-                    for (int i = 0; i < SEG; ++i) {
-                        const int2 z = zl[nt * 4 * p.spans * SEG + c_s * SEG + i];
-                        int acc[4] = {z.x, z.y, z.x, z.y};
-#pragma unroll
-                        for (int b = i * 4 / SEG; b < (i + 1) * 4 / SEG; ++b)
-                            mma_u8s8(acc, A[b] & 0x0F0F0F0Fu, B[b] & 0x0F0F0F0Fu, (A[b] >> 4) & 0x0F0F0F0Fu,
-                                     (B[b] >> 4) & 0x0F0F0F0Fu, X[2 * b], X[2 * b + 1]);
-                        tot[nt][0] = fmaf(f, fa[i] * (float)(acc[0] + 256 * acc[1]), tot[nt][0]);
-                        tot[nt][1] = fmaf(f, fb[i] * (float)(acc[2] + 256 * acc[3]), tot[nt][1]);
-                    }
-                }
-                if (++c_s == ns) { c_s = 0; flush(); }
-            }
-        }
+        __syncthreads();
     }
 }
 
