@@ -386,7 +386,7 @@ int launch_gemv(const mt::q4::Gemv& p, dim3 grid, cudaStream_t st, const char* w
         if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
         smem_set.fetch_or(bit);
     }
-    mt::q4::gemv_kernel<NT, G><<<grid, mt::q4::kGemvThreads, mt::q4::gemv_smem(NT, G, p.spans), st>>>(p);
+    mt::q4::gemv_kernel<NT, G><<<grid, mt::q4::kGemvThreads, mt::q4::gemv_smem(NT, p.spans), st>>>(p);
     return launched(who);
 }
 template <int NT>
@@ -406,14 +406,14 @@ int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, c
     // L2) than K in several launches, down to 4.
     int64_t chunks = (M + 2 * kGemvMaxTiles - 1) / (2 * kGemvMaxTiles);
     int64_t rows = (M + chunks - 1) / chunks;
-    while (rows > 4 && gemv_smem((int)(rows + 1) / 2, w.group, (int)spans) > kMaxSmem) {
+    while (rows > 4 && gemv_smem((int)(rows + 1) / 2, (int)spans) > kMaxSmem) {
         ++chunks;
         rows = (M + chunks - 1) / chunks;
     }
     if (chunks > 65535) return fail(MT_EUNSUPPORTED, "%s: too many rows", who);
     const int nt = (int)(rows + 1) / 2;
     int64_t most = std::max<int64_t>(1, spans);
-    while (most > 1 && gemv_smem(nt, w.group, (int)most) > kMaxSmem) most = (most + 1) / 2;
+    while (most > 1 && gemv_smem(nt, (int)most) > kMaxSmem) most = (most + 1) / 2;
     const int sms = mt::host::sm_count();
     const int64_t ctas = std::max<int64_t>(1, sms / chunks);
     Gemv p{};

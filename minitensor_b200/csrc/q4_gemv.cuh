@@ -2,16 +2,16 @@
 //
 // One row of x is bound by reading W once; 6.5 TB/s are 13 T weights a second, 45 a cycle of an
 // SM, so a weight can cost only a fraction of an instruction. Unpacking to half precision and
-// mma.sync on it took 450 and later 110 instructions for the 128 x 16 weights of a warp's
-// step; integers take 60.
+// mma.sync on it took 110 instructions for the 128 x 16 weights of a warp's step.
 //
 // Mathematics. Per span of 128 features x becomes a fixed-point number of 30 bits and a sign,
 // X = rn(x * 2^(29 - e)) with 2^e <= max |x| < 2^(e + 1), off by 2^-30 of the span's largest at
-// most, and X four signed digits of 8 bits, X = sum d_j 256^j. The codes 0..15 of a word are
-// unsigned bytes after a mask (three instructions for 8 weights), so the tensor core's u8 x s8
-// product (mma.sync m16n8k32, 1,950 multiply-adds a cycle measured) gives sum c d_j exactly.
-// Its accumulator begins at -8 sum d_j, which takes the codes' offset off exactly, too:
-//   y = sum over groups of scale * 2^(e - 29) * sum_j 256^j * sum (c - 8) d_j,
+// most, and X four signed digits of 8 bits, X = sum d_j 256^j. They are the bytes of
+// (X + 0x808080) ^ 0x808080: the addition carries what makes the lower bytes, less 128, signed.
+// A code c in a byte's upper half with that half's top bit turned is the signed byte 16 (c - 8),
+// so eight codes are unpacked by three instructions, and the tensor core's s8 x s8 product
+// (mma.sync m16n8k32, 1,950 multiply-adds a cycle measured) gives sum 16 (c - 8) d_j exactly:
+//   y = sum over groups of scale * 2^(e - 33) * sum_j 256^j * sum 16 (c - 8) d_j,
 // float only from the group's scale on. The four digits of a row are four columns of the
 // product, a tile of 8 columns holds two rows of x.
 //
@@ -61,98 +61,85 @@ __host__ __device__ constexpr int gemv_pad(int nt, int spans) {
 __host__ __device__ constexpr int gemv_run(int nt) { return 192 / nt - (kGemvWarps - 1); }
 
 // Shared memory: digits [8 NT columns][spans * 128 + 16] (the 16 put neighbouring columns on other
-// banks), accumulator starts and powers of two [2 NT rows][2][spans * segments + 1] of 16 bytes,
-// partial sums [run + 15][16][2 NT], codes [warps][2][group][rows g, g + 8][lanes] of 16 bytes.
-__host__ __device__ constexpr size_t gemv_smem(int nt, int group, int spans) {
-    return (size_t)8 * nt * (gemv_pad(nt, spans) * kSpan + 16) + (size_t)4 * nt * (gemv_pad(nt, spans) * (kSpan / group) + 1) * 16 +
+// banks), powers of two [2 NT rows][spans + 1], partial sums [run + 15][16][2 NT], codes
+// [warps][2][group][rows g, g + 8][lanes] of 16 bytes.
+// Whole lines: cp.async into 16-byte pieces that straddle 32-byte sectors took 20 % longer.
+__host__ __device__ constexpr int round128(int n) { return (n + 127) & ~127; }
+__host__ __device__ constexpr size_t gemv_smem(int nt, int spans) {
+    return (size_t)8 * nt * (gemv_pad(nt, spans) * kSpan + 16) + round128(2 * nt * (gemv_pad(nt, spans) + 1) * 4) +
            (size_t)(gemv_run(nt) + kGemvWarps - 1) * 16 * 2 * nt * 4 + (size_t)kGemvWarps * gemv_ring(nt);
 }
 
-__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The even and the odd nibbles of a word as signed bytes 16 (c - 8): codes 0 4 1 5 and 2 6 3 7.
+__device__ __forceinline__ uint32_t even_codes(uint32_t w) { return ((w << 4) & 0xF0F0F0F0u) ^ 0x80808080u; }
+__device__ __forceinline__ uint32_t odd_codes(uint32_t w) { return (w & 0xF0F0F0F0u) ^ 0x80808080u; }
 
 // Puts this CTA's rows and spans of x into shared memory; returns whether all of it is finite.
-// A warp takes a span, a lane 4 of its features. A word's bytes are masked out as codes
-// 0 4 1 5 and 2 6 3 7 of its 8, the digits go in that order.
-template <int NT, int G>
-__device__ __forceinline__ bool gemv_stage_x(const Gemv& p, uint8_t* xs, int4* zs) {
-    constexpr int SEG = kSpan / G, WARPS = kGemvWarps;
+// A warp takes a span, a lane the four features that meet one unpacked word: of octet lane / 2
+// of the span 0 4 1 5 or 2 6 3 7. Loads of four spans are in flight together.
+template <int NT>
+__device__ __forceinline__ bool gemv_stage_x(const Gemv& p, uint8_t* xs, float* fs) {
+    constexpr int BATCH = 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int spans = gemv_pad(NT, p.spans), col_bytes = spans * kSpan + 16;
     const int64_t m0 = (int64_t)blockIdx.y * p.rows;
+    const int octet = lane >> 1, first = octet * 8 + (lane & 1) * 2;   // features first, first + 1, first + 4, first + 5
+    uint8_t* to = xs + octet % 4 * 32 + octet / 4 * 8 + (lane & 1) * 4;
     int bad = 0;
-    constexpr int BATCH = 4;   // spans whose loads are in flight together
-    for (int i0 = warp; i0 < 2 * NT * spans; i0 += BATCH * WARPS) {
-    float vs[BATCH][4];
+    for (int r = 0; r < 2 * NT; ++r) {
+        const bool row = r < p.rows && m0 + r < p.M;
+        const float* x = p.x.p + (m0 + r) * p.x.rs;
+        for (int sb = warp; sb < spans; sb += BATCH * kGemvWarps) {
+            float v[BATCH][4];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-        const int i = i0 + u * WARPS, r = i / spans, s = i - r * spans;
-        const int64_t m = m0 + r, k = (int64_t)(p.span0 + s) * kSpan + lane * 4;
-        vs[u][0] = vs[u][1] = vs[u][2] = vs[u][3] = 0.f;
-        if (r < p.rows && m < p.M && s < p.spans) {
-            if (p.xvec && k + 4 <= p.w.K) {
-                const float4 q = *reinterpret_cast<const float4*>(p.x.p + m * p.x.rs + k);
-                vs[u][0] = q.x; vs[u][1] = q.y; vs[u][2] = q.z; vs[u][3] = q.w;
-            } else {
+            for (int u = 0; u < BATCH; ++u) {
+                const int s = sb + u * kGemvWarps;
+                const int64_t k = (int64_t)(p.span0 + s) * kSpan + first;
+                v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.f;
+                if (row && s < p.spans) {
+                    if (p.xvec && k + 6 <= p.w.K) {
+                        const float2 a = *reinterpret_cast<const float2*>(x + k), b = *reinterpret_cast<const float2*>(x + k + 4);
+                        v[u][0] = a.x; v[u][1] = a.y; v[u][2] = b.x; v[u][3] = b.y;
+                    } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (k + j < p.w.K) vs[u][j] = p.x.p[m * p.x.rs + (k + j) * p.x.cs];
+                        for (int j = 0; j < 4; ++j) {
+                            const int64_t kj = k + j + (j & 2);
+                            if (kj < p.w.K) v[u][j] = x[kj * p.x.cs];
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int s = sb + u * kGemvWarps;
+                if (s >= spans) break;
+                uint32_t a = max(max(lowbit::abs_bits(v[u][0]), lowbit::abs_bits(v[u][1])),
+                                 max(lowbit::abs_bits(v[u][2]), lowbit::abs_bits(v[u][3])));
+                a = __reduce_max_sync(0xffffffffu, a);
+                bad |= a >= 0x7F800000u;
+                const int e = max((int)(a >> 23), 34);   // biased exponent
+                const float up = __uint_as_float((uint32_t)(283 - e) << 23);
+                uint32_t d[4];   // the four digits of a value
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] = (uint32_t)(__float2int_rn(v[u][j] * up) + 0x808080) ^ 0x808080u;
+                // Values in the order 0 4 1 5 (d[0], d[2], d[1], d[3]); one digit of each to a word.
+                const uint32_t l0 = __byte_perm(d[0], d[2], 0x5140), l1 = __byte_perm(d[1], d[3], 0x5140);
+                const uint32_t h0 = __byte_perm(d[0], d[2], 0x7362), h1 = __byte_perm(d[1], d[3], 0x7362);
+                uint8_t* o = to + (size_t)(4 * r) * col_bytes + s * kSpan;
+                *reinterpret_cast<uint32_t*>(o) = __byte_perm(l0, l1, 0x5410);
+                *reinterpret_cast<uint32_t*>(o + col_bytes) = __byte_perm(l0, l1, 0x7632);
+                *reinterpret_cast<uint32_t*>(o + 2 * (size_t)col_bytes) = __byte_perm(h0, h1, 0x5410);
+                *reinterpret_cast<uint32_t*>(o + 3 * (size_t)col_bytes) = __byte_perm(h0, h1, 0x7632);
+                if (lane == 0) fs[r * (spans + 1) + s] = __uint_as_float((uint32_t)(e - 33) << 23);
             }
         }
-    }
-#pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-        const int i = i0 + u * WARPS, r = i / spans, s = i - r * spans;
-        if (r >= 2 * NT) break;
-        if (r >= p.rows) {   // no row of x: zeros
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<uint32_t*>(xs + (size_t)(4 * r + j) * col_bytes + s * kSpan + lane * 4) = 0;
-            if (lane < 2 * SEG) zs[(2 * r + lane / SEG) * (spans * SEG + 1) + s * SEG + lane % SEG] = make_int4(0, 0, 0, 0);
-            continue;
-        }
-        const float (&v)[4] = vs[u];
-        uint32_t a = max(max(lowbit::abs_bits(v[0]), lowbit::abs_bits(v[1])),
-                         max(lowbit::abs_bits(v[2]), lowbit::abs_bits(v[3])));
-        a = __reduce_max_sync(0xffffffffu, a);
-        bad |= a >= 0x7F800000u;
-        const int e = max((int)(a >> 23), 30);   // biased exponent
-        const float up = __uint_as_float((uint32_t)(283 - e) << 23);
-        uint32_t d[4] = {0, 0, 0, 0};            // digit j of the lane's four values
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            int X = __float2int_rn(v[c] * up);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int dj = (int)(int8_t)X;
-                d[j] |= (uint32_t)(dj & 0xFF) << (8 * c);
-                X = (X - dj) >> 8;
-            }
-        }
-        uint8_t* o = xs + (size_t)(4 * r) * col_bytes + s * kSpan + (lane % 8) / 2 * 32 + lane / 8 * 8 + (lane & 1) * 4;
-        int sum[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            // Even lanes hold codes 0..3, odd lanes 4..7 of an octet.
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, d[j], 1);
-            const uint32_t word = lane & 1 ? __byte_perm(other, d[j], 0x7362) : __byte_perm(d[j], other, 0x5140);
-            *reinterpret_cast<uint32_t*>(o + (size_t)j * col_bytes) = word;
-            sum[j] = __dp4a((int)d[j], 0x01010101, 0);
-#pragma unroll
-            for (int w = 1; w < G / 4; w <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], w);
-        }
-        if (lane % (G / 4) == 0) {
-            const int at = 2 * r * (spans * SEG + 1) + s * SEG + lane / (G / 4);
-            const float f = __uint_as_float((uint32_t)(e - 29) << 23);
-            zs[at] = make_int4(-8 * sum[0], -8 * sum[1], __float_as_int(f), 0);
-            zs[at + spans * SEG + 1] = make_int4(-8 * sum[2], -8 * sum[3], __float_as_int(f * 65536.f), 0);
-        }
-    }
     }
     return __syncthreads_or(bad) == 0;
 }
@@ -184,11 +171,11 @@ __device__ __noinline__ void gemv_tile_float(const Gemv& p, int64_t tile, int s0
 template <int NT, int G>
 __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
     constexpr int SEG = kSpan / G, GROUP = gemv_group(NT), WARPS = kGemvWarps;
-    extern __shared__ __align__(16) uint8_t gemv_smem_raw[];
+    extern __shared__ __align__(128) uint8_t gemv_smem_raw[];
     const int spans = gemv_pad(NT, p.spans), col_bytes = spans * kSpan + 16;
     uint8_t* xs = gemv_smem_raw;
-    int4* zs = reinterpret_cast<int4*>(xs + (size_t)8 * NT * col_bytes);
-    float* red = reinterpret_cast<float*>(zs + (size_t)4 * NT * (spans * SEG + 1));
+    float* fs = reinterpret_cast<float*>(xs + (size_t)8 * NT * col_bytes);
+    float* red = fs + round128(2 * NT * (spans + 1) * 4) / 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     uint4* ring = reinterpret_cast<uint4*>(red + (gemv_run(NT) + WARPS - 1) * 16 * 2 * NT) +
@@ -269,7 +256,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
             cp_async_commit();
         };
         fetch();
-        if (tile0 == cta0) fast = gemv_stage_x<NT, G>(p, xs, zs);   // ends with a __syncthreads
+        if (tile0 == cta0) fast = gemv_stage_x<NT>(p, xs, fs);   // ends with a __syncthreads
 
         int tile = gpt ? lo / gpt : 0, c_s = (lo - tile * gpt) * GROUP;
         if (fast) {
@@ -277,7 +264,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
 #pragma unroll
             for (int i = 0; i < NT; ++i) tot[i][0] = tot[i][1] = 0.f;
             const uint8_t* xl = xs + (size_t)g * col_bytes + t * 32;
-            const int4* zl = zs + t * (spans * SEG + 1);   // row t / 2 of an 8-column tile, its low or high digits
+            const float* fl = fs + t / 2 * (spans + 1);   // row t / 2 of an 8-column tile
             const uint4* w = ring;
 #pragma unroll 1
             for (int i = lo; i < hi; ++i) {
@@ -302,15 +289,13 @@ __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
                         const uint8_t* x = xl + nt * 8 * col_bytes + (c_s + j) * kSpan;
                         const uint4 x0 = *reinterpret_cast<const uint4*>(x), x1 = *reinterpret_cast<const uint4*>(x + 16);
                         const uint32_t X[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                        const float f = fl[nt * 2 * (spans + 1) + c_s + j];
 #pragma unroll
                         for (int k = 0; k < SEG; ++k) {
-                            const int4 z = zl[nt * 4 * (spans * SEG + 1) + (c_s + j) * SEG + k];
-                            const float f = __int_as_float(z.z);
-                            int acc[4] = {z.x, z.y, z.x, z.y};
+                            int acc[4] = {0, 0, 0, 0};
 #pragma unroll
                             for (int b = k * 4 / SEG; b < (k + 1) * 4 / SEG; ++b)
-                                mma_u8s8(acc, A[b] & 0x0F0F0F0Fu, B[b] & 0x0F0F0F0Fu, (A[b] >> 4) & 0x0F0F0F0Fu,
-                                         (B[b] >> 4) & 0x0F0F0F0Fu, X[2 * b], X[2 * b + 1]);
+                                mma_s8(acc, even_codes(A[b]), even_codes(B[b]), odd_codes(A[b]), odd_codes(B[b]), X[2 * b], X[2 * b + 1]);
                             tot[nt][0] = fmaf(f, fa[k] * (float)(acc[0] + 256 * acc[1]), tot[nt][0]);
                             tot[nt][1] = fmaf(f, fb[k] * (float)(acc[2] + 256 * acc[3]), tot[nt][1]);
                         }
@@ -324,8 +309,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
 #pragma unroll
                     for (int k = 0; k < NT; ++k) {
                         // Lanes t and t ^ 1 hold the low and the high digits of a row.
-                        const float a = tot[k][0] + __shfl_xor_sync(0xffffffffu, tot[k][0], 1);
-                        const float b = tot[k][1] + __shfl_xor_sync(0xffffffffu, tot[k][1], 1);
+                        const float a = fmaf(65536.f, __shfl_down_sync(0xffffffffu, tot[k][0], 1), tot[k][0]);
+                        const float b = fmaf(65536.f, __shfl_down_sync(0xffffffffu, tot[k][1], 1), tot[k][1]);
                         if ((t & 1) == 0) {
                             mine[g * 2 * NT + k * 2 + t / 2] = a;
                             mine[(g + 8) * 2 * NT + k * 2 + t / 2] = b;
