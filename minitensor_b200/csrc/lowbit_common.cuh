@@ -90,19 +90,20 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[WPR], int& buf) {
     return warp_sum(s);
 }
 
+// VEC features of a row of unit stride.
 template <int VEC>
 __device__ __forceinline__ void load_row(float (&v)[VEC], const Mat& m, int64_t row, int64_t f) {
     if (VEC == 4) {
         const float4 x = *reinterpret_cast<const float4*>(m.p + row * m.rs + f);
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
     } else {
-        v[0] = m.p[row * m.rs + f * m.cs];
+        v[0] = m.p[row * m.rs + f];
     }
 }
 template <int VEC>
 __device__ __forceinline__ void store_row(const float (&v)[VEC], const Mat& m, int64_t row, int64_t f) {
     if (VEC == 4) *reinterpret_cast<float4*>(m.p + row * m.rs + f) = make_float4(v[0], v[1], v[2], v[3]);
-    else m.p[row * m.rs + f * m.cs] = v[0];
+    else m.p[row * m.rs + f] = v[0];
 }
 
 // Quantises VEC values per lane, feature f of row `row` first; 32 / VEC lanes share a block.

@@ -161,6 +161,8 @@ Span q4_scale_span(const mt::q4::Weight& q) {
     return span_of_rows(q.scales, q.K ? q.N : 0, 2 * q.sp, 2 * ((q.K + q.group - 1) / q.group));
 }
 
+bool unit_cols(const View2& v) { return !v.given || v.cols <= 1 || v.m.cs == 1; }
+
 // Rows of unit stride that start on 16-byte boundaries.
 bool vec4(const View2& v) {
     if (!v.given) return true;
@@ -177,8 +179,9 @@ unsigned grid_of(int64_t n, int64_t most) { return (unsigned)std::max<int64_t>(1
 
 // ------------------------------------- RMS norm ---------------------------------------
 
-// Largest row held in registers: 32 warps x V = 8 pieces of 32 lanes x VEC features.
-constexpr int64_t kRowPieces = 32 * 8 * 32;
+// Pieces of 32 lanes x VEC features in the largest row held in registers.
+constexpr int64_t kFwdPieces = 32 * 8;
+constexpr int64_t bwd_pieces(bool vec) { return vec ? 32 * 4 : 32 * 8; }
 
 template <int VEC, int V, int WPR, int RPC>
 int launch_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
@@ -187,8 +190,9 @@ int launch_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
     return launched("rms_norm launch");
 }
 
-// Warps per row and pieces per lane by the row's length. Rows that are too few to fill the
-// GPU take more warps each.
+// Warps per row and pieces per lane by the row's length: 8 warps, as many as keep a CTA's
+// share of the registers small, until a lane would hold more than 32 floats. Rows that are
+// too few to fill the GPU take 32 warps each.
 template <int VEC>
 int run_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
     const int64_t pieces = (p.K + 32 * VEC - 1) / (32 * VEC);
@@ -196,6 +200,10 @@ int run_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
     if (pieces <= 4) return launch_fwd<VEC, 4, 1, 4>(p, st);
     if (few && pieces <= 32) return launch_fwd<VEC, 1, 32, 1>(p, st);
     if (pieces <= 32) return launch_fwd<VEC, 4, 8, 1>(p, st);
+    if (!few && pieces <= 64) return launch_fwd<VEC, 8, 8, 1>(p, st);
+    if constexpr (VEC == 1) {
+        if (!few) return pieces <= 128 ? launch_fwd<1, 16, 8, 1>(p, st) : launch_fwd<1, 32, 8, 1>(p, st);
+    }
     if (pieces <= 128) return launch_fwd<VEC, 4, 32, 1>(p, st);
     return launch_fwd<VEC, 8, 32, 1>(p, st);
 }
@@ -203,7 +211,17 @@ int run_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
 // Row groups whose dgamma partials are kept; the launch has one per CTA (or warp, RPC > 1).
 template <int VEC, int V, int WPR, int RPC>
 int64_t bwd_groups(int64_t rows) {
-    const int per_sm = std::max(1, 1024 / (32 * WPR * RPC));
+    // As many CTAs as are resident at once.
+    static std::atomic<int> resident{0};
+    int per_sm = resident.load();
+    if (per_sm == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, mt::rms::bwd_kernel<VEC, V, WPR, RPC>, 32 * WPR * RPC, 0) !=
+                cudaSuccess || per_sm < 1) {
+            cudaGetLastError();
+            per_sm = 1;
+        }
+        resident.store(per_sm);
+    }
     const int64_t ctas = std::min<int64_t>((rows + RPC - 1) / RPC, (int64_t)mt::host::sm_count() * per_sm);
     return ctas * RPC;
 }
@@ -218,9 +236,10 @@ template <int VEC, typename F>
 int with_bwd_variant(int64_t K, F&& f) {
     const int64_t pieces = (K + 32 * VEC - 1) / (32 * VEC);
     if (pieces <= 4) return f.template run<VEC, 4, 1, 4>();
-    if (pieces <= 32) return f.template run<VEC, 4, 8, 1>();
-    if (pieces <= 128) return f.template run<VEC, 4, 32, 1>();
-    return f.template run<VEC, 8, 32, 1>();
+    if (pieces <= 32) return f.template run<VEC, 2, 16, 1>();
+    if (pieces <= 64) return f.template run<VEC, 4, 16, 1>();
+    if constexpr (VEC == 4) return f.template run<4, 4, 32, 1>();
+    else return pieces <= 128 ? f.template run<1, 8, 16, 1>() : f.template run<1, 8, 32, 1>();
 }
 struct GroupsOf {
     int64_t rows, *out;
@@ -324,13 +343,16 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     __nv_bfloat16* b = a + a_bytes / 2;
     float* sums = db.p ? reinterpret_cast<float*>(b + b_bytes / 2) : nullptr;
     if (K > 0) {
-        mt::planes::expand_q8_kernel<<<dim3((unsigned)((K + 63) / 64), grid_of(tiles_m, 65535)), 256, 0, st>>>(q, a, M, K, pitch);
+        const bool vec = (reinterpret_cast<uintptr_t>(q.codes) & 15) == 0 && (M == 1 || q.cp % 16 == 0);
+        const dim3 grid((unsigned)((K + 63) / 64), grid_of(tiles_m, 65535));
+        if (vec) mt::planes::expand_q8_kernel<true><<<grid, 256, 0, st>>>(q, a, M, K, pitch);
+        else mt::planes::expand_q8_kernel<false><<<grid, 256, 0, st>>>(q, a, M, K, pitch);
         MT_TRY(launched(who));
     }
     mt::planes::split_rows_kernel<<<dim3((unsigned)((N + 63) / 64), grid_of(tiles_m, 65535)), 256, 0, st>>>(dy, b, M, N, pitch, sums);
     MT_TRY(launched(who));
     if (db.p) {
-        mt::rms::sum_parts_kernel<<<(unsigned)((N + 31) / 32), dim3(32, 8), 0, st>>>(sums, tiles_m, N, db);
+        mt::rms::sum_parts_kernel<<<(unsigned)((N + 31) / 32), dim3(32, 32), 0, st>>>(sums, tiles_m, N, db);
         MT_TRY(launched(who));
     }
     if (K == 0) return MT_OK;
@@ -502,7 +524,8 @@ MT_API int mt_rms_norm(const mt_tensor* x, const mt_tensor* residual, const mt_t
     const bool vec = K % 4 == 0 && vec4(vx) && vec4(vr) && vec4(vg) && vec4(vh) && vec4(vy) &&
                      (!q8 || ((reinterpret_cast<uintptr_t>(q.codes) & 3) == 0 && (M == 1 || q.cp % 4 == 0)));
     int rc;
-    if (K > kRowPieces * (vec ? 4 : 1)) {
+    const bool unit = unit_cols(vx) && unit_cols(vr) && unit_cols(vg) && unit_cols(vh) && unit_cols(vy);
+    if (!unit || (K + 32 * (vec ? 4 : 1) - 1) / (32 * (vec ? 4 : 1)) > kFwdPieces) {
         mt::rms::fwd_long_kernel<<<grid_of(M, INT32_MAX), 32 * mt::rms::kLongWarps, 0, st>>>(p);
         rc = launched("rms_norm launch");
         if (rc == MT_OK) mt::host::set_path("rms_norm long rows");
@@ -542,7 +565,8 @@ MT_API int mt_rms_norm_backward(const mt_tensor* dy, const mt_tensor* h, const m
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     mt::rms::Bwd p{vdy.m, vh.m, vg.m, vs.m, vdh.m, vdx.m, nullptr, M, K};
     const bool vec = K % 4 == 0 && vec4(vdy) && vec4(vh) && vec4(vg) && vec4(vdh) && vec4(vdx);
-    const bool is_long = K > kRowPieces * (vec ? 4 : 1);
+    const bool unit = unit_cols(vdy) && unit_cols(vh) && unit_cols(vg) && unit_cols(vdh) && unit_cols(vdx);
+    const bool is_long = !unit || (K + 32 * (vec ? 4 : 1) - 1) / (32 * (vec ? 4 : 1)) > bwd_pieces(vec);
     int64_t groups = 0;
     if (is_long) {
         groups = std::min<int64_t>(M, std::max<int64_t>(1, 8LL * mt::host::sm_count() * 256 / K));
@@ -569,7 +593,7 @@ MT_API int mt_rms_norm_backward(const mt_tensor* dy, const mt_tensor* h, const m
         }
     }
     if (rc == MT_OK && dgamma) {
-        mt::rms::sum_parts_kernel<<<(unsigned)((K + 31) / 32), dim3(32, 8), 0, st>>>(p.part, groups, K, vdg.m);
+        mt::rms::sum_parts_kernel<<<(unsigned)((K + 31) / 32), dim3(32, 32), 0, st>>>(p.part, groups, K, vdg.m);
         rc = launched("rms_norm_backward dgamma sum launch");
     }
     mt::host::scratch_free(ws, bytes, st);
@@ -620,7 +644,7 @@ MT_API int mt_dequantize_q8(const mt_q8* q, void* out, int type, uint64_t pitch,
         return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || pitch_bytes % 16 == 0);
     };
     const bool vec = K % 16 == 0 && al16(o.codes, o.cp, M) && al16(out, (int64_t)pitch * es, M);
-    const int64_t width = 256 * (vec ? 16 : 1);
+    const int64_t width = vec ? 256 * 16 : mt::q8::kDequantWidth;
     const dim3 grid((unsigned)((K + width - 1) / width), grid_of(M, 65535));
     if (type == MT_F32) {
         float* f = static_cast<float*>(out);

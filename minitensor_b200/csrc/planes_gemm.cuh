@@ -42,7 +42,7 @@ constexpr uint32_t RING_BYTES = STAGE_BYTES * STAGES;
 constexpr float kCodeUnit = 2048.f;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
-constexpr uint32_t EPI_BYTES = EPI_WARPS * 32 * 33 * 4;
+constexpr uint32_t EPI_BYTES = EPI_WARPS * 32 * 20 * 4;
 constexpr uint32_t BAR_BYTES = 8 * (2 * STAGES + 4) + 16;
 constexpr uint32_t SMEM_BYTES = 1024 + RING_BYTES + EPI_BYTES + BAR_BYTES;
 static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
@@ -202,7 +202,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         }
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;
-        float* buf = epi + (warp - 2) * 32 * 33;
+        float* buf = epi + (warp - 2) * 32 * 20;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * 128;
         const uint32_t empty_bar[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
         int n = 0;
@@ -262,18 +262,30 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         if (col0 + j < p.C) o[(int64_t)(col0 + j) * os_c] = acc[j];
                 }
             } else {
-                // 32 x 32 blocks turned in shared memory: lanes along c.
+                // 32 x 16 blocks turned in shared memory (rows of 20 floats: 16-byte accesses of
+                // 8 lanes fall on different banks), then 4 lanes along c and 8 rows at a time.
+                const bool vec = os_c == 1 && os_r % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 8; ++c) {
                     __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) buf[lane * 33 + j] = acc[c * 32 + j];
+                    for (int j = 0; j < 16; j += 4)
+                        *reinterpret_cast<float4*>(buf + lane * 20 + j) =
+                            make_float4(acc[c * 16 + j], acc[c * 16 + j + 1], acc[c * 16 + j + 2], acc[c * 16 + j + 3]);
                     __syncwarp();
-                    const int col = col0 + c * 32 + lane;
-                    if (col < p.C) {
-                        const int rows = min(32, p.R - row0);
-                        float* o = out + (int64_t)row0 * os_r + (int64_t)col * os_c;
-                        for (int i = 0; i < rows; ++i) o[(int64_t)i * os_r] = buf[i * 33 + lane];
+                    if (vec && col0 + c * 16 + 16 <= p.C) {
+                        const int r = lane >> 2, col = col0 + c * 16 + (lane & 3) * 4;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            if (row0 + i + r < p.R)
+                                *reinterpret_cast<float4*>(out + (int64_t)(row0 + i + r) * os_r + col) =
+                                    *reinterpret_cast<const float4*>(buf + (i + r) * 20 + (lane & 3) * 4);
+                    } else {
+                        const int r = lane >> 4, col = col0 + c * 16 + (lane & 15);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2)
+                            if (row0 + i + r < p.R && col < p.C)
+                                out[(int64_t)(row0 + i + r) * os_r + (int64_t)col * os_c] = buf[(i + r) * 20 + (lane & 15)];
                     }
                 }
             }
@@ -410,30 +422,43 @@ __global__ void __launch_bounds__(256) expand_q4_kernel(q4::Weight q, __nv_bfloa
     }
 }
 
-// A for the weight gradient: out[k][m] = code value of (m, k), m padded with zeros to `pitch`.
+// A for the weight gradient: out[k][m] = value of (m, k), m padded with zeros to `pitch`. A thread
+// takes 16 features of a row (VEC: one 16-byte load; rows of codes on 16-byte boundaries).
+template <bool VEC>
 __global__ void __launch_bounds__(256) expand_q8_kernel(lowbit::Q8 q, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch) {
     __shared__ uint16_t s[64][66];
     const int64_t k0 = (int64_t)blockIdx.x * 64;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int row = threadIdx.x & 63, part = threadIdx.x >> 6;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int64_t mt = blockIdx.y; mt * 64 < pitch; mt += gridDim.y) {
-        const int64_t m0 = mt * 64;
+        const int64_t m0 = mt * 64, k = k0 + part * 16;
+        uint32_t w[4] = {0, 0, 0, 0};
+        float scale = 0.f;
+        if (m0 + row < M && k < K) {
+            const uint8_t* c = q.codes + (m0 + row) * q.cp + k;
+            scale = lowbit::scale_value(q.scales[(m0 + row) * q.sp + k / lowbit::kBlock]);
+            if (VEC && k + 16 <= K) {
+                const uint4 v = *reinterpret_cast<const uint4*>(c);
+                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (k + i < K) w[i / 4] |= (uint32_t)c[i] << (8 * (i % 4));
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int64_t m = m0 + ty + 4 * i, k = k0 + tx;
-            float v = 0.f;
-            if (m < M && k < K)
-                v = lowbit::code_value(q.codes[m * q.cp + k], q.fmt) * lowbit::scale_value(q.scales[m * q.sp + k / lowbit::kBlock]);
-            s[tx][ty + 4 * i] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+            const float v = lowbit::code_value((w[i / 4] >> (8 * (i % 4))) & 0xFFu, q.fmt) * scale;
+            s[part * 16 + i][row] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
         }
         __syncthreads();
         const int64_t m = m0 + 2 * lane;
         if (m < pitch) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int64_t k = k0 + warp * 8 + i;
-                if (k >= K) break;
-                *reinterpret_cast<uint32_t*>(out + k * pitch + m) = *reinterpret_cast<const uint32_t*>(&s[warp * 8 + i][2 * lane]);
+                const int64_t ko = k0 + warp * 8 + i;
+                if (ko >= K) break;
+                *reinterpret_cast<uint32_t*>(out + ko * pitch + m) = *reinterpret_cast<const uint32_t*>(&s[warp * 8 + i][2 * lane]);
             }
         }
         __syncthreads();

@@ -12,6 +12,7 @@ using lowbit::Q8;
 
 constexpr int kWarps = 8;
 constexpr int kRows = 4;   // rows in flight per warp
+constexpr int kDequantWidth = 8 * 256;   // features per CTA of the scalar dequantisation
 
 // A warp takes a chunk of 32 * VEC features of kRows rows at a time (VEC = 4: 16-byte loads).
 template <int VEC>
@@ -25,7 +26,8 @@ __global__ void __launch_bounds__(32 * kWarps) quantize_kernel(Mat x, Q8 q, int6
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
             if (in && r0 + j < rows) {
-                lowbit::load_row<VEC>(v[j], x, r0 + j, f);
+                if (VEC == 4) lowbit::load_row<VEC>(v[j], x, r0 + j, f);
+                else v[j][0] = x.p[(r0 + j) * x.rs + f * x.cs];
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) v[j][i] = 0.f;
@@ -40,26 +42,37 @@ __global__ void __launch_bounds__(32 * kWarps) quantize_kernel(Mat x, Q8 q, int6
 __device__ __forceinline__ void put(float* o, float v) { *o = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* o, float v) { *o = __float2bfloat16_rn(v); }
 
-// N = 16: 16 codes (half a block) per thread, 16-byte accesses; N = 1: any pitch and length.
+// N = 16: 16 codes (half a block) per thread, 16-byte accesses. N = 1: any pitch and length, 8 codes
+// of a thread in flight, 256 apart.
 template <typename T, int N>
 __global__ void __launch_bounds__(256) dequantize_kernel(Q8 q, T* out, int64_t pitch, int64_t rows, int64_t K) {
-    const int64_t f = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
-    if (f >= K) return;
-    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-        const float s = lowbit::scale_value(q.scales[row * q.sp + f / lowbit::kBlock]);
-        const uint8_t* c = q.codes + row * q.cp + f;
-        T* o = out + row * pitch + f;
-        if (N == 16) {
-            const uint4 w = *reinterpret_cast<const uint4*>(c);
+    if (N == 16) {
+        const int64_t f = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
+        if (f >= K) return;
+        for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+            const float s = lowbit::scale_value(q.scales[row * q.sp + f / lowbit::kBlock]);
+            const uint4 w = *reinterpret_cast<const uint4*>(q.codes + row * q.cp + f);
             const uint32_t u[4] = {w.x, w.y, w.z, w.w};
             alignas(16) T t[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) put(&t[i], lowbit::code_value((u[i / 4] >> (8 * (i % 4))) & 0xFFu, q.fmt) * s);
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T); ++i)
-                reinterpret_cast<uint4*>(o)[i] = reinterpret_cast<const uint4*>(t)[i];
-        } else {
-            put(o, lowbit::code_value(*c, q.fmt) * s);
+                reinterpret_cast<uint4*>(out + row * pitch + f)[i] = reinterpret_cast<const uint4*>(t)[i];
+        }
+    } else {
+        const int64_t f0 = (int64_t)blockIdx.x * kDequantWidth + threadIdx.x;
+        for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+            uint8_t c[8], b[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t f = f0 + i * 256;
+                c[i] = f < K ? q.codes[row * q.cp + f] : 0;
+                b[i] = f < K ? q.scales[row * q.sp + f / lowbit::kBlock] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (f0 + i * 256 < K) put(out + row * pitch + f0 + i * 256, lowbit::code_value(c[i], q.fmt) * lowbit::scale_value(b[i]));
         }
     }
 }

@@ -7,9 +7,9 @@
 //
 // Both directions are bound by memory: a row is read once and held in registers between its
 // reduction and its use. WPR warps share a row; each lane holds V pieces of VEC features
-// (VEC = 4: 16-byte accesses, for unit-stride rows on 16-byte boundaries; VEC = 1: any
-// strides). Rows longer than the largest variant go through the *_long kernels, which read
-// them twice. Statistics and sums are float; the sum over rows for dgamma is one partial per
+// (VEC = 4: 16-byte accesses, for rows on 16-byte boundaries; VEC = 1 otherwise). Rows
+// longer than the largest variant and rows whose features are not neighbours go through the
+// *_long kernels, which read them twice. Statistics and sums are float; the sum over rows for dgamma is one partial per
 // row group in a fixed order, added in order by a second kernel, so results do not depend on
 // timing.
 #pragma once
@@ -38,8 +38,11 @@ struct Bwd {
     int64_t K;
 };
 
+// CTAs per SM that the registers have to allow: x and the residual are in flight together.
+constexpr int fwd_ctas(int floats, int threads) { return threads > 256 ? 1 : floats <= 16 ? 4 : floats <= 32 ? 3 : 2; }
+
 template <int VEC, int V, int WPR, int RPC>
-__global__ void __launch_bounds__(32 * WPR * RPC) fwd_kernel(const Fwd p) {
+__global__ void __launch_bounds__(32 * WPR * RPC, fwd_ctas(VEC * V, 32 * WPR * RPC)) fwd_kernel(const Fwd p) {
     static_assert(WPR == 1 || RPC == 1, "rows that share a CTA have one warp each");
     __shared__ float red[2][WPR];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -156,16 +159,16 @@ __global__ void __launch_bounds__(32 * WPR * RPC) bwd_kernel(const Bwd p) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dg[c][i] = 0.f;
     for (int64_t row = group; row < p.rows; row += (int64_t)gridDim.x * RPC) {
-        float dy[V][VEC], xh[V][VEC];
+        float dy[V][VEC], xh[V][VEC], dh[V][VEC];
 #pragma unroll
         for (int c = 0; c < V; ++c) {
             const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) dy[c][i] = xh[c][i] = dh[c][i] = 0.f;
             if (f < p.K) {
                 lowbit::load_row<VEC>(dy[c], p.dy, row, f);
                 lowbit::load_row<VEC>(xh[c], p.h, row, f);
-            } else {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) dy[c][i] = xh[c][i] = 0.f;
+                if (p.dh.p) lowbit::load_row<VEC>(dh[c], p.dh, row, f);
             }
         }
         const float rstd = p.rstd.p[row * p.rstd.cs];
@@ -192,13 +195,7 @@ __global__ void __launch_bounds__(32 * WPR * RPC) bwd_kernel(const Bwd p) {
             if (f < p.K) {
                 float d[VEC];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) d[i] = rstd * fmaf(-xh[c][i], dot, dy[c][i]);
-                if (p.dh.p) {
-                    float e[VEC];
-                    lowbit::load_row<VEC>(e, p.dh, row, f);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) d[i] += e[i];
-                }
+                for (int i = 0; i < VEC; ++i) d[i] = fmaf(rstd, fmaf(-xh[c][i], dot, dy[c][i]), dh[c][i]);
                 lowbit::store_row<VEC>(d, p.dx, row, f);
             }
         }
@@ -244,18 +241,20 @@ __global__ void __launch_bounds__(256) dgamma_long_kernel(const Bwd p) {
     p.part[(int64_t)blockIdx.y * p.K + f] = s;
 }
 
-// out[f] = sum over g of part[g][f]: 8 sums over g = i (mod 8), each ascending, added in order.
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int64_t groups, int64_t K, Mat out) {
-    __shared__ float s[8][32];
+// out[f] = sum over g of part[g][f]: 32 sums over g = i (mod 32), each ascending, added in order.
+__global__ void __launch_bounds__(1024) sum_parts_kernel(const float* part, int64_t groups, int64_t K, Mat out) {
+    __shared__ float s[32][33];
     const int64_t f = (int64_t)blockIdx.x * 32 + threadIdx.x;
     float a = 0.f;
-    if (f < K)
-        for (int64_t g = threadIdx.y; g < groups; g += 8) a += part[g * K + f];
+    if (f < K) {
+#pragma unroll 4
+        for (int64_t g = threadIdx.y; g < groups; g += 32) a += part[g * K + f];
+    }
     s[threadIdx.y][threadIdx.x] = a;
     __syncthreads();
     if (threadIdx.y == 0 && f < K) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) a += s[i][threadIdx.x];
+        for (int i = 1; i < 32; ++i) a += s[i][threadIdx.x];
         out.p[f * out.cs] = a;
     }
 }

@@ -20,12 +20,13 @@ allocated for that stream; the caller orders other streams' use of operands and 
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import engine
-from .engine import MODE_DEFAULT, MtTensor, _check, _gpu_present, gemm, linear_forward, view
+from .engine import MAX_DIMS, MODE_DEFAULT, _check, _gpu_present, gemm, linear_forward
 
 Q8_BLOCK = 32
 Q8_FORMATS = {"int8": 0, "e4m3": 1}
@@ -54,8 +55,7 @@ def _lowbit_lib():
     global _lib
     if _lib is None:
         L = engine.lib()
-        P, vp = ctypes.POINTER(MtTensor), ctypes.c_void_p
-        Q8, Q4 = ctypes.POINTER(MtQ8), ctypes.POINTER(MtQ4)
+        P = Q8 = Q4 = vp = ctypes.c_void_p   # structs are passed packed (_mat) or by reference
         i, u64 = ctypes.c_int, ctypes.c_uint64
         for name, args in (("mt_rms_norm", [P, P, P, P, P, P, Q8, ctypes.c_float, vp]),
                            ("mt_rms_norm_backward", [P, P, P, P, P, P, P, vp]),
@@ -111,6 +111,9 @@ class Q8Tensor:
     def device(self):
         return self.codes.device
 
+    def get_device(self) -> int:
+        return self.codes.get_device()
+
     @property
     def format(self) -> str:
         return _Q8_DTYPES[self.codes.dtype]
@@ -157,29 +160,62 @@ class Q4Weight:
     def device(self):
         return self.codes.device
 
-
-_U8 = ctypes.c_uint64 * engine.MAX_DIMS
-
-
-def _mat(t: torch.Tensor) -> MtTensor:
-    """engine.view, without its loop: these operators' smallest calls are bound by the host."""
-    if t.dtype != torch.float32 or t.dim() > 2 or not t.is_cuda:
-        return view(t)
-    return MtTensor(t.data_ptr() if t.numel() else 0, 0, t.dim(), _U8(*t.shape), _U8(*t.stride()))
+    def get_device(self) -> int:
+        return self.codes.get_device()
 
 
-def _same_device(*operands):
-    first = None
-    for o in operands:
-        if o is None:
-            continue
-        if first is None:
-            first = o.device
-        elif o.device != first:
+# An mt_tensor as bytes: these operators' smallest calls are bound by the host, and packing
+# takes a third of what filling a ctypes struct does.
+_pack = struct.Struct(f"@PQI4x{2 * MAX_DIMS}Q").pack
+_PAD = (0,) * (MAX_DIMS - 2)
+
+
+def _mat(t: torch.Tensor) -> bytes:
+    if t.dtype is not torch.float32:
+        raise ValueError(f"expected float32, got {t.dtype}")
+    dims = t.dim()
+    if dims == 2:
+        (r, c), (rs, cs) = t.shape, t.stride()
+        return _pack(t.data_ptr(), 0, 2, r, c, *_PAD, rs, cs, *_PAD)
+    if dims > MAX_DIMS:
+        raise ValueError("Exceeded MAX_DIMS")
+    pad = (0,) * (MAX_DIMS - dims)
+    return _pack(t.data_ptr(), 0, dims, *t.shape, *pad, *t.stride(), *pad)
+
+
+def _dense(t: torch.Tensor, rows: int, cols: int) -> bytes:
+    """A contiguous [rows, cols] result, whose layout is known."""
+    return _pack(t.data_ptr(), 0, 2, rows, cols, *_PAD, cols, 1, *_PAD)
+
+
+def _opt(t):
+    return None if t is None else _mat(t)
+
+
+def _same_device(first, *others):
+    """The operands' device index, -1 for host memory (which only a machine without a GPU
+    gets as far as the library's argument checks)."""
+    d = first.get_device()
+    for o in others:
+        if o is not None and o.get_device() != d:
             raise ValueError("all operands must be on the same device")
-    if first.type != "cuda" and _gpu_present():
-        raise ValueError(f"expected CUDA tensors, got some on {first}")
-    return first
+    if d < 0 and _gpu_present():
+        raise ValueError("expected CUDA tensors, got some on the host")
+    return d
+
+
+def _device(d: int):
+    return torch.device("cuda", d) if d >= 0 else torch.device("cpu")
+
+
+def _empty(like, rows, cols):
+    """An uninitialised contiguous float32 [rows, cols] on like's device."""
+    if like.dtype is torch.float32 and like.is_contiguous() and like.shape == (rows, cols):
+        return torch.empty_like(like)   # half the cost of naming everything
+    return torch.empty((rows, cols), dtype=torch.float32, device=like.device)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # current_stream(), without the object
 
 
 class _On:
@@ -190,18 +226,17 @@ class _On:
 
     def __init__(self, device, stream):
         self._ctx = None
-        if device.type != "cuda":
+        if device < 0:
             self.s = None
-            return
-        if stream is None:
-            if device.index != torch.cuda.current_device():
+        elif stream is None:
+            if device != torch.cuda.current_device():
                 self._ctx = torch.cuda.device(device)
-            self.s = torch.cuda.current_stream(device).cuda_stream
+            self.s = _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
         else:
             if not isinstance(stream, torch.cuda.Stream):
                 stream = torch.cuda.ExternalStream(int(stream), device=device)
-            elif stream.device != device:
-                raise ValueError(f"the stream belongs to {stream.device}, the operands to {device}")
+            elif stream.device.index != device:
+                raise ValueError(f"the stream belongs to {stream.device}, the operands to cuda:{device}")
             self._ctx = torch.cuda.stream(stream)
             self.s = stream.cuda_stream
 
@@ -216,14 +251,6 @@ class _On:
         return False
 
 
-def _p(v):
-    return ctypes.byref(v) if v is not None else None
-
-
-def _opt(t):
-    return ctypes.byref(_mat(t)) if t is not None else None
-
-
 def _need_2d(t, name):
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2-D, got {t.dim()}-D")
@@ -231,9 +258,10 @@ def _need_2d(t, name):
         raise ValueError(f"{name}: expected float32, got {t.dtype}")
 
 
-def _new_q8(rows, cols, fmt, device) -> Q8Tensor:
+def _new_q8(rows, cols, fmt, d) -> Q8Tensor:
     if fmt not in Q8_FORMATS:
         raise ValueError(f"8-bit format must be one of {tuple(Q8_FORMATS)}, got {fmt!r}")
+    device = _device(d)
     return Q8Tensor(torch.empty((rows, cols), dtype=_Q8_STORAGE[fmt], device=device),
                     torch.empty((rows, -(-cols // Q8_BLOCK)), dtype=torch.uint8, device=device))
 
@@ -264,12 +292,14 @@ def rms_norm(x, gamma, residual=None, eps=1e-6, q8=None, want_y=True, inplace=Fa
     dev = _same_device(x, gamma, residual)
     with _On(dev, stream) as on:
         q = _new_q8(rows, features, q8, dev) if q8 is not None else None
-        y = torch.empty((rows, features), dtype=torch.float32, device=dev) if want_y else None
-        h = x if residual is None or inplace else torch.empty((rows, features), dtype=torch.float32, device=dev)
-        rstd = torch.empty((rows,), dtype=torch.float32, device=dev)
-        _check(_lowbit_lib().mt_rms_norm(_p(_mat(x)), _opt(residual), _p(_mat(gamma)),
-                                         _p(_mat(h)) if residual is not None else None, _opt(y), _p(_mat(rstd)),
-                                         _p(q._c) if q is not None else None, float(eps), on.s))
+        y = _empty(x, rows, features) if want_y else None
+        h = x if residual is None or inplace else _empty(x, rows, features)
+        rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
+        _check(_lowbit_lib().mt_rms_norm(
+            _mat(x), _opt(residual), _mat(gamma),
+            None if residual is None else _mat(x) if inplace else _dense(h, rows, features),
+            _dense(y, rows, features) if want_y else None, _dense(rstd, 1, rows),
+            ctypes.byref(q._c) if q is not None else None, eps, on.s))
     return RmsNorm(y, h, rstd, q)
 
 
@@ -278,12 +308,14 @@ def rms_norm_backward(dy, h, gamma, rstd, dh=None, need_dgamma=True, stream=None
     gradient of x and of the residual both; ``dh``, a gradient that reaches h from the
     residual stream behind the norm, is added to it. dgamma is [features], or None."""
     _need_2d(dy, "dy")
+    rows, features = dy.shape
     dev = _same_device(dy, h, gamma, rstd, dh)
     with _On(dev, stream) as on:
-        dx = torch.empty(dy.shape, dtype=torch.float32, device=dev)
-        dgamma = torch.empty((dy.shape[1],), dtype=torch.float32, device=dev) if need_dgamma else None
-        _check(_lowbit_lib().mt_rms_norm_backward(_p(_mat(dy)), _p(_mat(h)), _p(_mat(gamma)), _p(_mat(rstd)),
-                                                  _opt(dh), _p(_mat(dx)), _opt(dgamma), on.s))
+        dx = _empty(dy, rows, features)
+        dgamma = torch.empty((features,), dtype=torch.float32, device=dy.device) if need_dgamma else None
+        _check(_lowbit_lib().mt_rms_norm_backward(
+            _mat(dy), _mat(h), _mat(gamma), _mat(rstd), _opt(dh), _dense(dx, rows, features),
+            _dense(dgamma, 1, features) if need_dgamma else None, on.s))
     return dx, dgamma
 
 
@@ -296,7 +328,7 @@ def quantize_q8(x, fmt="int8", stream=None) -> Q8Tensor:
     dev = _same_device(x)
     with _On(dev, stream) as on:
         q = _new_q8(x.shape[0], x.shape[1], fmt, dev)
-        _check(_lowbit_lib().mt_quantize_q8(_p(_mat(x)), _p(q._c), on.s))
+        _check(_lowbit_lib().mt_quantize_q8(_mat(x), ctypes.byref(q._c), on.s))
     return q
 
 
@@ -307,8 +339,8 @@ def dequantize_q8(q: Q8Tensor, dtype=torch.float32, stream=None) -> torch.Tensor
         raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
     dev = _same_device(q)
     with _On(dev, stream) as on:
-        out = torch.empty(q.shape, dtype=dtype, device=dev)
-        _check(_lowbit_lib().mt_dequantize_q8(_p(q._c), out.data_ptr(), int(dtype == torch.bfloat16),
+        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        _check(_lowbit_lib().mt_dequantize_q8(ctypes.byref(q._c), out.data_ptr(), int(dtype == torch.bfloat16),
                                               out.shape[1], on.s))
     return out
 
@@ -326,10 +358,12 @@ def linear_weight_grad_q8(xq: Q8Tensor, dY, need_db=True, stream=None):
     [1, out] = the column sums of dY (None with need_db=False)."""
     _need_2d(dY, "dY")
     dev = _same_device(xq, dY)
+    k, n = xq.shape[1], dY.shape[1]
     with _On(dev, stream) as on:
-        dW = torch.empty((xq.shape[1], dY.shape[1]), dtype=torch.float32, device=dev)
-        db = torch.empty((1, dY.shape[1]), dtype=torch.float32, device=dev) if need_db else None
-        _check(_lowbit_lib().mt_linear_wgrad_q8(_p(xq._c), _p(_mat(dY)), _p(_mat(dW)), _opt(db), on.s))
+        dW = torch.empty((k, n), dtype=torch.float32, device=dY.device)
+        db = torch.empty((1, n), dtype=torch.float32, device=dY.device) if need_db else None
+        _check(_lowbit_lib().mt_linear_wgrad_q8(ctypes.byref(xq._c), _mat(dY), _dense(dW, k, n),
+                                                _dense(db, 1, n) if need_db else None, on.s))
     return dW, db
 
 
@@ -339,7 +373,7 @@ def linear_backward_q8(xq: Q8Tensor, W, dY, mode=MODE_DEFAULT, stream=None):
     _need_2d(dY, "dY")
     dev = _same_device(xq, W, dY)
     with _On(dev, stream):
-        dX = torch.empty((dY.shape[0], W.shape[0]), dtype=torch.float32, device=dev)
+        dX = torch.empty((dY.shape[0], W.shape[0]), dtype=torch.float32, device=dY.device)
         gemm(dY, W.t(), dX, mode=mode)
         dW, db = linear_weight_grad_q8(xq, dY)
     return dX, dW, db
@@ -356,9 +390,9 @@ def quantize_q4(W, group=64, stream=None) -> Q4Weight:
     dev = _same_device(W)
     k, n = W.shape
     with _On(dev, stream) as on:
-        q = Q4Weight(torch.empty((n, 64 * (-(-k // Q4_SPAN))), dtype=torch.uint8, device=dev),
-                     torch.empty((n, -(-k // group)), dtype=torch.bfloat16, device=dev), k, group)
-        _check(_lowbit_lib().mt_quantize_q4(_p(_mat(W)), _p(q._c), on.s))
+        q = Q4Weight(torch.empty((n, 64 * (-(-k // Q4_SPAN))), dtype=torch.uint8, device=W.device),
+                     torch.empty((n, -(-k // group)), dtype=torch.bfloat16, device=W.device), k, group)
+        _check(_lowbit_lib().mt_quantize_q4(_mat(W), ctypes.byref(q._c), on.s))
     return q
 
 
@@ -366,8 +400,8 @@ def dequantize_q4(w: Q4Weight, stream=None) -> torch.Tensor:
     """The float32 weight [in, out] that ``w`` stands for."""
     dev = _same_device(w)
     with _On(dev, stream) as on:
-        W = torch.empty((w.in_features, w.out_features), dtype=torch.float32, device=dev)
-        _check(_lowbit_lib().mt_dequantize_q4(_p(w._c), _p(_mat(W)), on.s))
+        W = torch.empty((w.in_features, w.out_features), dtype=torch.float32, device=w.device)
+        _check(_lowbit_lib().mt_dequantize_q4(ctypes.byref(w._c), _mat(W), on.s))
     return W
 
 
@@ -376,7 +410,9 @@ def linear_forward_q4(x, w: Q4Weight, bias=None, relu=False, stream=None) -> tor
     ReLU)."""
     _need_2d(x, "x")
     dev = _same_device(x, w, bias)
+    rows, n = x.shape[0], w.codes.shape[0]
     with _On(dev, stream) as on:
-        Y = torch.empty((x.shape[0], w.out_features), dtype=torch.float32, device=dev)
-        _check(_lowbit_lib().mt_linear_fwd_q4(_p(_mat(x)), _p(w._c), _opt(bias), _p(_mat(Y)), int(bool(relu)), on.s))
+        Y = torch.empty((rows, n), dtype=torch.float32, device=x.device)
+        _check(_lowbit_lib().mt_linear_fwd_q4(_mat(x), ctypes.byref(w._c), _opt(bias), _dense(Y, rows, n),
+                                              1 if relu else 0, on.s))
     return Y
