@@ -113,8 +113,12 @@ __device__ __forceinline__ void store_q8(const float (&v)[VEC], const Q8& q, int
     uint32_t a = 0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) a = max(a, abs_bits(v[i]));
+    if (VEC == 1) {
+        a = __reduce_max_sync(0xffffffffu, a);
+    } else {
 #pragma unroll
-    for (int o = 16 / VEC; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+        for (int o = 16 / VEC; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    }
     const uint32_t b = scale_byte(a, q.fmt);
     const float inv = inv_scale(b);
     if (!in) return;

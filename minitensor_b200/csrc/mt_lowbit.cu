@@ -202,7 +202,7 @@ int run_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
     if (pieces <= 32) return launch_fwd<VEC, 4, 8, 1>(p, st);
     if (!few && pieces <= 64) return launch_fwd<VEC, 8, 8, 1>(p, st);
     if constexpr (VEC == 1) {
-        if (!few) return pieces <= 128 ? launch_fwd<1, 16, 8, 1>(p, st) : launch_fwd<1, 32, 8, 1>(p, st);
+        if (!few) return pieces <= 128 ? launch_fwd<1, 8, 16, 1>(p, st) : launch_fwd<1, 16, 16, 1>(p, st);
     }
     if (pieces <= 128) return launch_fwd<VEC, 4, 32, 1>(p, st);
     return launch_fwd<VEC, 8, 32, 1>(p, st);
@@ -270,19 +270,27 @@ struct Scratch {
     }
 };
 
-// Splits of the sum over k: the least of rounds x length, a 64-deep block of a pair tile
-// taking about 1,600 cycles and the partials' way through memory about 3,000 bytes a cycle.
-int pick_splits(int64_t tiles, int64_t kblocks, int64_t chunk_blocks, int64_t clusters, int64_t out_bytes) {
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, kblocks / chunk_blocks));
-    int best = 1;
-    double least = 1e300;
-    for (int64_t s = 1; s <= most; ++s) {
-        const int64_t len = (kblocks / chunk_blocks + s - 1) / s * chunk_blocks;
-        const double cost = (double)((tiles * s + clusters - 1) / clusters) * len * 1600. +
-                            (s > 1 ? (2. * s + 1.) * out_bytes / 3000. + 4000. : 0.);
-        if (cost < least * 0.98) { least = cost; best = (int)s; }
+// How many tiles are done at once, and in how many parts of k the others: a full round of
+// clusters takes whole tiles, the tiles of a last round that would leave clusters idle are
+// split between them. A 64-deep block of a pair tile takes about 1,600 cycles; a split costs
+// another kernel and its parts' way through memory, about 4,000 bytes a cycle.
+void pick_splits(mt::planes::Params& p, int64_t tiles, int64_t chunk_blocks, int64_t clusters) {
+    p.whole = (int)tiles;
+    p.splits = 1;
+    const int64_t rest = tiles % clusters;
+    if (rest == 0) return;
+    const int64_t nb = (p.kblocks + chunk_blocks - 1) / chunk_blocks;
+    double least = (double)nb * chunk_blocks * 1600.;   // the last round as it is
+    const int64_t most = std::min<int64_t>(64, std::min(nb, clusters / rest));
+    for (int64_t s = 2; s <= most; ++s) {
+        const double cost = (double)((nb + s - 1) / s * chunk_blocks) * 1600. +
+                            (double)(2 * s + 1) * rest * (mt::planes::BM * mt::planes::BN * 4) / 4000. + 5000.;
+        if (cost < least) {
+            least = cost;
+            p.splits = (int)s;
+            p.whole = (int)(tiles - rest);
+        }
     }
-    return best;
 }
 
 // D = A * B^T over `kpitch` padded values of k: a [R][kpitch], b [3][C][kpitch], both bfloat16.
@@ -298,10 +306,11 @@ int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16
     p.tiles_c = (p.C + BN - 1) / BN;
     const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c;
     if (tiles > INT32_MAX / 64) return fail(MT_EUNSUPPORTED, "%s: too many output tiles", who);
-    p.splits = pick_splits(tiles, p.kblocks, p.spc == 8 ? 2 : 1, clusters, (int64_t)p.R * p.C * 4);
-    p.units = (int)tiles * p.splits;
+    pick_splits(p, tiles, p.spc == 8 ? 2 : 1, clusters);
+    const int64_t in_parts = tiles - p.whole;
+    p.units = (int)(p.whole + in_parts * p.splits);
     Scratch part(st);
-    if (p.splits > 1) MT_TRY(part.take((size_t)p.splits * p.R * p.C * sizeof(float), who));
+    if (in_parts) MT_TRY(part.take((size_t)in_parts * p.splits * BM * BN * sizeof(float), who));
     p.part = static_cast<float*>(part.p);
     CUtensorMap ta, tb;
     const uint64_t da[3] = {(uint64_t)kpitch, (uint64_t)p.R, 1}, db[3] = {(uint64_t)kpitch, (uint64_t)p.C, 3};
@@ -321,12 +330,12 @@ int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16
     const unsigned grid = 2 * (unsigned)std::min<int64_t>(p.units, clusters);
     gemm_kernel<SCALED><<<grid, THREADS, SMEM_BYTES, st>>>(ta, tb, p);
     MT_TRY(launched(who));
-    if (p.splits > 1) {
-        join_kernel<<<grid_of(((int64_t)p.R * p.C + 255) / 256, 16LL * sms), 256, 0, st>>>(p);
+    if (in_parts) {
+        join_kernel<<<dim3((unsigned)in_parts, BM / 8), 256, 0, st>>>(p);
         MT_TRY(launched(who));
     }
     char path[96];
-    snprintf(path, sizeof path, "%s planes splits=%d", who, p.splits);
+    snprintf(path, sizeof path, "%s planes whole=%d splits=%d", who, p.whole, p.splits);
     mt::host::set_path(path);
     return MT_OK;
 }
@@ -342,20 +351,17 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     __nv_bfloat16* a = static_cast<__nv_bfloat16*>(ws.p);
     __nv_bfloat16* b = a + a_bytes / 2;
     float* sums = db.p ? reinterpret_cast<float*>(b + b_bytes / 2) : nullptr;
-    if (K > 0) {
-        const bool vec = (reinterpret_cast<uintptr_t>(q.codes) & 15) == 0 && (M == 1 || q.cp % 16 == 0);
-        const dim3 grid((unsigned)((K + 63) / 64), grid_of(tiles_m, 65535));
-        if (vec) mt::planes::expand_q8_kernel<true><<<grid, 256, 0, st>>>(q, a, M, K, pitch);
-        else mt::planes::expand_q8_kernel<false><<<grid, 256, 0, st>>>(q, a, M, K, pitch);
-        MT_TRY(launched(who));
-    }
-    mt::planes::split_rows_kernel<<<dim3((unsigned)((N + 63) / 64), grid_of(tiles_m, 65535)), 256, 0, st>>>(dy, b, M, N, pitch, sums);
+    const bool vec = (reinterpret_cast<uintptr_t>(q.codes) & 15) == 0 && (M == 1 || q.cp % 16 == 0);
+    const int64_t blocks_a = (K + 63) / 64, blocks_b = (N + 63) / 64;
+    const dim3 grid((unsigned)(blocks_a + blocks_b), grid_of(tiles_m, 65535));
+    if (vec) mt::planes::prepare_q8_kernel<true><<<grid, 256, 0, st>>>(q, a, K, dy, b, N, sums, M, pitch, (int)blocks_b);
+    else mt::planes::prepare_q8_kernel<false><<<grid, 256, 0, st>>>(q, a, K, dy, b, N, sums, M, pitch, (int)blocks_b);
     MT_TRY(launched(who));
-    if (db.p) {
+    if (K == 0) {   // the bias gradient alone
+        if (!db.p) return MT_OK;
         mt::rms::sum_parts_kernel<<<(unsigned)((N + 31) / 32), dim3(32, 32), 0, st>>>(sums, tiles_m, N, db);
-        MT_TRY(launched(who));
+        return launched(who);
     }
-    if (K == 0) return MT_OK;
     mt::planes::Params p{};
     p.R = (int)K;
     p.C = (int)N;
@@ -363,10 +369,14 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     p.out = dw.p;
     p.os_r = dw.rs;
     p.os_c = dw.cs;
+    p.col_sums = sums;
+    p.db_tiles = db.p ? (int)tiles_m : 0;
+    p.db = db.p;
+    p.db_cs = db.cs;
     return run_planes<false>(p, a, b, pitch, st, who);
 }
 
-int linear_q4_planes(const Mat& x, const mt::q4::Weight& w, const float* bias, const Mat& y, int64_t M, int relu,
+int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias, const Mat& y, int64_t M, int relu,
                      cudaStream_t st, const char* who) {
     const int64_t pitch = round_up(w.K, mt::q4::kSpan);
     const size_t a_bytes = w.N * pitch * 2, b_bytes = 3 * M * pitch * 2;
@@ -374,9 +384,9 @@ int linear_q4_planes(const Mat& x, const mt::q4::Weight& w, const float* bias, c
     MT_TRY(ws.take(a_bytes + b_bytes, who));
     __nv_bfloat16* a = static_cast<__nv_bfloat16*>(ws.p);
     __nv_bfloat16* b = a + a_bytes / 2;
-    mt::planes::expand_q4_kernel<<<dim3((unsigned)((pitch / 8 + 255) / 256), grid_of(w.N, 65535)), 256, 0, st>>>(w, a, pitch);
-    MT_TRY(launched(who));
-    mt::planes::split_cols_kernel<<<dim3((unsigned)((pitch / 4 + 255) / 256), grid_of(M, 65535)), 256, 0, st>>>(x, b, M, w.K, pitch);
+    const int64_t blocks_a = (pitch / 8 + 255) / 256, blocks_b = (pitch / 4 + 255) / 256;
+    mt::planes::prepare_q4_kernel<<<dim3((unsigned)(blocks_a + blocks_b), grid_of((std::max(w.N, M) + 7) / 8, 65535)), 256, 0, st>>>(
+        w, a, x.m, vec4(x), b, M, pitch, (int)blocks_b);
     MT_TRY(launched(who));
     mt::planes::Params p{};
     p.R = (int)w.N;
@@ -747,7 +757,7 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     const int64_t M = vx.rows;
     if (M * w.N == 0) return MT_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (M > 64 && w.K > 0) return linear_q4_planes(vx.m, w, vb.m.p, vy.m, M, relu, st, who);
+    if (M > 64 && w.K > 0) return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
     return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
 }
 

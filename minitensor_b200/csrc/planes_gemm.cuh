@@ -51,32 +51,48 @@ struct Params {
     int R, C;                    // rows of A, rows of B
     int kblocks;                 // 64-deep blocks of k
     int spc;                     // k16-steps per chunk: 2, 4 or 8
-    int tiles_r, tiles_c, splits;
-    int units;                   // tiles * splits
+    int tiles_r, tiles_c;
+    int whole, splits;           // tiles [0, whole) are done at once, the others in `splits` parts of k
+    int units;                   // whole + splits * (tiles - whole)
     float* out;                  // D[r][c] at out + r * os_r + c * os_c
     int64_t os_r, os_c;
-    float* part;                 // splits > 1: partial s of D at part + s * R * C, row-major
+    float* part;                 // part s of tile t at ((t - whole) * splits + s) * 256 * 256
     const __nv_bfloat16* scales; // SCALED: scale of row r, chunk j at r * sp + j
     int64_t sp;
     int groups;                  // scales per row; chunks behind them have no codes
     const float* bias;           // per row r, may be null (SCALED)
     int relu;
+    // Not SCALED, db_tiles > 0: db[c] at db + c * db_cs = the sum over t of col_sums[t * C + c].
+    const float* col_sums;
+    int db_tiles;
+    float* db;
+    int64_t db_cs;
 };
 
-// Unit u -> tile and the k-blocks [kb0, kb1) of its split; a split begins on a chunk.
-// Row blocks go in groups of 8, so that clusters at work share rows of A and B in L2.
-__device__ __forceinline__ void unit_of(const Params& p, int u, int& rb, int& cb, int& sp, int& kb0, int& kb1) {
-    sp = u % p.splits;
-    const int t = u / p.splits;
+// Tile t -> blocks of rows and columns. Row blocks go in groups of 8, so that clusters at work
+// share rows of A and B in L2.
+__device__ __forceinline__ void tile_of(const Params& p, int t, int& rb, int& cb) {
     const int per = 8 * p.tiles_c;
     const int g = t / per, in = t - g * per;
     const int rows = min(8, p.tiles_r - g * 8);
     cb = in / rows;
     rb = g * 8 + in - cb * rows;
+}
+// Unit u -> tile, part and the k-blocks [kb0, kb1) of the part, which begins on a chunk. sp < 0: whole.
+__device__ __forceinline__ int unit_of(const Params& p, int u, int& sp, int& kb0, int& kb1) {
+    if (u < p.whole) {
+        sp = -1;
+        kb0 = 0;
+        kb1 = p.kblocks;
+        return u;
+    }
+    const int t = (u - p.whole) / p.splits;
+    sp = u - p.whole - t * p.splits;
     const int cpb = p.spc == 8 ? 2 : 1;                        // k-blocks per chunk boundary
     const int nb = (p.kblocks + cpb - 1) / cpb;
     kb0 = (int)((long long)nb * sp / p.splits) * cpb;
     kb1 = min(p.kblocks, (int)((long long)nb * (sp + 1) / p.splits) * cpb);
+    return p.whole + t;
 }
 
 // kind::f16 instruction descriptor: bfloat16 operands, K-major, float accumulate.
@@ -144,7 +160,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             int s = 0;
             uint32_t ph = 0;
             for (int u = first; u < p.units; u += step) {
-                unit_of(p, u, rb, cb, sp, kb0, kb1);
+                tile_of(p, unit_of(p, u, sp, kb0, kb1), rb, cb);
                 const int r0 = rb * BM + (int)rank * 128, c0 = cb * BN + (int)rank * 128;
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!mbar_wait_cl(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) goto done;
@@ -164,7 +180,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             int s = 0, n = 0;          // stage, chunks begun
             uint32_t ph = 0;
             for (int u = first; u < p.units; u += step) {
-                unit_of(p, u, rb, cb, sp, kb0, kb1);
+                unit_of(p, u, sp, kb0, kb1);
                 int in_chunk = 0;
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!mbar_wait_cl(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) goto done;
@@ -206,8 +222,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * 128;
         const uint32_t empty_bar[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
         int n = 0;
+        if (!SCALED && p.db_tiles > 0) {
+            // The bias gradient, while the first tiles load.
+            for (int64_t c = (int64_t)blockIdx.x * (32 * EPI_WARPS) + (int)threadIdx.x - 64; c < p.C; c += (int64_t)gridDim.x * (32 * EPI_WARPS)) {
+                float s = 0.f;
+#pragma unroll 8
+                for (int t = 0; t < p.db_tiles; ++t) s += p.col_sums[(int64_t)t * p.C + c];
+                p.db[c * p.db_cs] = s;
+            }
+        }
         for (int u = first; u < p.units; u += step) {
-            unit_of(p, u, rb, cb, sp, kb0, kb1);
+            const int tile = unit_of(p, u, sp, kb0, kb1);
+            tile_of(p, tile, rb, cb);
             const int row0 = rb * BM + (int)rank * 128 + q * 32;
             const int col0 = cb * BN + half * 128;
             const int chunks = ((kb1 - kb0) * 4 + p.spc - 1) / p.spc;
@@ -241,11 +267,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                                                  : acc[c * 16 + j] + __uint_as_float(r[j]);
                 }
             }
-            float* out = p.splits > 1 ? p.part + (int64_t)sp * p.R * p.C : p.out;
-            const int64_t os_r = p.splits > 1 ? p.C : p.os_r, os_c = p.splits > 1 ? 1 : p.os_c;
+            const bool whole = sp < 0;
+            // The parts of a tile are stored as whole 256 x 256 tiles, along r or c as D is.
+            const bool along_r = p.os_r == 1;
+            const int pr = (int)rank * 128 + q * 32, pc = half * 128;
+            float* out = whole ? p.out + (int64_t)row0 * p.os_r + (int64_t)col0 * p.os_c
+                               : p.part + ((int64_t)(tile - p.whole) * p.splits + sp) * (BM * BN) + (along_r ? pc * BM + pr : pr * BN + pc);
+            const int64_t os_r = whole ? p.os_r : along_r ? 1 : BN, os_c = whole ? p.os_c : along_r ? BM : 1;
+            const int rows = whole ? min(32, p.R - row0) : 32, cols = whole ? min(128, p.C - col0) : 128;
             if (SCALED) {
                 const int row = row0 + lane;
-                const bool whole = p.splits == 1;
                 const float b = whole && p.bias && row < p.R ? p.bias[row] : 0.f;
 #pragma unroll
                 for (int j = 0; j < 128; ++j) {
@@ -255,37 +286,36 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
             if (os_r == 1) {
                 // Lanes are neighbours in memory: one 128-byte line per column.
-                if (row0 + lane < p.R) {
-                    float* o = out + row0 + lane;
+                if (lane < rows) {
+                    float* o = out + lane;
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
-                        if (col0 + j < p.C) o[(int64_t)(col0 + j) * os_c] = acc[j];
+                    for (int j = 0; j < 128; ++j) {
+                        if (j < cols) *o = acc[j];
+                        o += os_c;
+                    }
                 }
             } else {
                 // 32 x 16 blocks turned in shared memory (rows of 20 floats: 16-byte accesses of
                 // 8 lanes fall on different banks), then 4 lanes along c and 8 rows at a time.
                 const bool vec = os_c == 1 && os_r % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < 128; c += 16) {
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 16; j += 4)
-                        *reinterpret_cast<float4*>(buf + lane * 20 + j) =
-                            make_float4(acc[c * 16 + j], acc[c * 16 + j + 1], acc[c * 16 + j + 2], acc[c * 16 + j + 3]);
+                        *reinterpret_cast<float4*>(buf + lane * 20 + j) = make_float4(acc[c + j], acc[c + j + 1], acc[c + j + 2], acc[c + j + 3]);
                     __syncwarp();
-                    if (vec && col0 + c * 16 + 16 <= p.C) {
-                        const int r = lane >> 2, col = col0 + c * 16 + (lane & 3) * 4;
+                    if (vec && c + 16 <= cols) {
+                        const int r = lane >> 2, j = (lane & 3) * 4;
 #pragma unroll
                         for (int i = 0; i < 32; i += 8)
-                            if (row0 + i + r < p.R)
-                                *reinterpret_cast<float4*>(out + (int64_t)(row0 + i + r) * os_r + col) =
-                                    *reinterpret_cast<const float4*>(buf + (i + r) * 20 + (lane & 3) * 4);
+                            if (i + r < rows)
+                                *reinterpret_cast<float4*>(out + (i + r) * os_r + c + j) = *reinterpret_cast<const float4*>(buf + (i + r) * 20 + j);
                     } else {
-                        const int r = lane >> 4, col = col0 + c * 16 + (lane & 15);
+                        const int r = lane >> 4, j = lane & 15;
 #pragma unroll
                         for (int i = 0; i < 32; i += 2)
-                            if (row0 + i + r < p.R && col < p.C)
-                                out[(int64_t)(row0 + i + r) * os_r + (int64_t)col * os_c] = buf[(i + r) * 20 + (lane & 15)];
+                            if (i + r < rows && c + j < cols) out[(i + r) * os_r + (c + j) * os_c] = buf[(i + r) * 20 + j];
                     }
                 }
             }
@@ -307,17 +337,25 @@ done:
     }
 }
 
-// D = sum of the splits' partials in order (+ bias per row, ReLU).
+// The tiles that were done in parts: the sum of the parts in order (+ bias per row, ReLU). A thread
+// has one column (or row, where rows are neighbours in D) of 8 rows (columns).
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
-    const int64_t n = (int64_t)p.R * p.C;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        // Neighbouring threads along the output's unit stride.
-        const int64_t r = p.os_r == 1 ? i % p.R : i / p.C, c = p.os_r == 1 ? i / p.R : i % p.C;
-        float v = p.part[r * p.C + c];
-        for (int s = 1; s < p.splits; ++s) v += p.part[s * n + r * p.C + c];
-        if (p.bias) v += p.bias[r];
-        if (p.relu) v = v > 0.f ? v : 0.f;
-        p.out[r * p.os_r + c * p.os_c] = v;
+    const int t = blockIdx.x;
+    int rb, cb;
+    tile_of(p, p.whole + t, rb, cb);
+    const bool along_r = p.os_r == 1;
+    const float* part = p.part + (int64_t)t * p.splits * (BM * BN);
+    for (int i = 0; i < 8; ++i) {
+        const int a = blockIdx.y * 8 + i, r = along_r ? threadIdx.x : a, c = along_r ? a : threadIdx.x;
+        const float* at = part + (along_r ? c * BM + r : r * BN + c);
+        float v = *at;
+        for (int s = 1; s < p.splits; ++s) v += at[s * (BM * BN)];
+        const int64_t row = (int64_t)rb * BM + r, col = (int64_t)cb * BN + c;
+        if (row < p.R && col < p.C) {
+            if (p.bias) v += p.bias[row];
+            if (p.relu) v = v > 0.f ? v : 0.f;
+            p.out[row * p.os_r + col * p.os_c] = v;
+        }
     }
 }
 
@@ -342,11 +380,9 @@ __device__ __forceinline__ void split3(float x, uint16_t (&o)[3]) {
 // Planes of B for a sum over rows of x [M, N]: out[plane][n][m], m padded with zeros to `pitch`.
 // 64 x 64 tiles turned in shared memory. col_sums, if not null: sums of each tile's columns
 // at [tile][N], for the bias gradient.
-__global__ void __launch_bounds__(256) split_rows_kernel(Mat x, __nv_bfloat16* out, int64_t M, int64_t N, int64_t pitch,
-                                                         float* col_sums) {
-    __shared__ float s[64][65];
-    __shared__ float cs[4][64];
-    const int64_t n0 = (int64_t)blockIdx.x * 64;
+__device__ __forceinline__ void split_rows(const Mat& x, __nv_bfloat16* out, int64_t M, int64_t N, int64_t pitch,
+                                           float* col_sums, int block, float (*s)[65], float (*cs)[64]) {
+    const int64_t n0 = (int64_t)block * 64;
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int64_t mt = blockIdx.y; mt * 64 < pitch; mt += gridDim.y) {
@@ -384,13 +420,22 @@ __global__ void __launch_bounds__(256) split_rows_kernel(Mat x, __nv_bfloat16* o
 
 // Planes of B for a sum over columns of x [M, K]: out[plane][m][k], k padded with zeros to `pitch`
 // (a multiple of 4).
-__global__ void __launch_bounds__(256) split_cols_kernel(Mat x, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch) {
-    const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+__device__ __forceinline__ void split_cols(const Mat& x, bool vec, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch, int block) {
+    const int64_t k = ((int64_t)block * 256 + threadIdx.x) * 4;
     if (k >= pitch) return;
+#pragma unroll 4
     for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
         uint16_t o[4][3];
+        if (vec && k + 4 <= K) {
+            const float4 v = *reinterpret_cast<const float4*>(x.p + m * x.rs + k);
+            split3(v.x, o[0]);
+            split3(v.y, o[1]);
+            split3(v.z, o[2]);
+            split3(v.w, o[3]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split3(k + i < K ? x.p[m * x.rs + (k + i) * x.cs] : 0.f, o[i]);
+            for (int i = 0; i < 4; ++i) split3(k + i < K ? x.p[m * x.rs + (k + i) * x.cs] : 0.f, o[i]);
+        }
 #pragma unroll
         for (int pl = 0; pl < 3; ++pl)
             *reinterpret_cast<uint2*>(out + (pl * M + m) * pitch + k) =
@@ -402,13 +447,14 @@ __global__ void __launch_bounds__(256) split_cols_kernel(Mat x, __nv_bfloat16* o
 // thread takes a word: 128 + c is a bfloat16 with c in its low bits, and 136 comes off exactly.
 // The unit keeps the sum over a group, at most 128 * 8 times the largest x, within x's range
 // until the group's scale meets it; the tile is multiplied by it when it is done.
-__global__ void __launch_bounds__(256) expand_q4_kernel(q4::Weight q, __nv_bfloat16* out, int64_t pitch) {
-    const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+__device__ __forceinline__ void expand_q4(const q4::Weight& q, __nv_bfloat16* out, int64_t pitch, int block) {
+    const int64_t k = ((int64_t)block * 256 + threadIdx.x) * 8;
     if (k >= pitch) return;
     const int64_t in = k % q4::kSpan;
     const int64_t w = k / q4::kSpan * q4::kSpanWords + in % 32 / 8 * 4 + in / 32;
     const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
     const __nv_bfloat162 unit = __floats2bfloat162_rn(1.f / kCodeUnit, 1.f / kCodeUnit);
+#pragma unroll 4
     for (int64_t n = blockIdx.y; n < q.N; n += gridDim.y) {
         const uint32_t word = q.codes[n * q.cp + w];
         uint32_t o[4];
@@ -425,9 +471,9 @@ __global__ void __launch_bounds__(256) expand_q4_kernel(q4::Weight q, __nv_bfloa
 // A for the weight gradient: out[k][m] = value of (m, k), m padded with zeros to `pitch`. A thread
 // takes 16 features of a row (VEC: one 16-byte load; rows of codes on 16-byte boundaries).
 template <bool VEC>
-__global__ void __launch_bounds__(256) expand_q8_kernel(lowbit::Q8 q, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch) {
-    __shared__ uint16_t s[64][66];
-    const int64_t k0 = (int64_t)blockIdx.x * 64;
+__device__ __forceinline__ void expand_q8(const lowbit::Q8& q, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch,
+                                          int block, uint16_t (*s)[66]) {
+    const int64_t k0 = (int64_t)block * 64;
     const int row = threadIdx.x & 63, part = threadIdx.x >> 6;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int64_t mt = blockIdx.y; mt * 64 < pitch; mt += gridDim.y) {
@@ -463,6 +509,25 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(lowbit::Q8 q, __nv_bfloa
         }
         __syncthreads();
     }
+}
+
+// Both operands of the weight gradient in one launch: blocks [0, blocks_b) of x do dY, the others
+// the checkpoint.
+template <bool VEC>
+__global__ void __launch_bounds__(256) prepare_q8_kernel(lowbit::Q8 q, __nv_bfloat16* a, int64_t K, Mat dy, __nv_bfloat16* b,
+                                                         int64_t N, float* col_sums, int64_t M, int64_t pitch, int blocks_b) {
+    __shared__ union {
+        struct { float s[64][65], cs[4][64]; } rows;
+        uint16_t codes[64][66];
+    } sm;
+    if ((int)blockIdx.x < blocks_b) split_rows(dy, b, M, N, pitch, col_sums, blockIdx.x, sm.rows.s, sm.rows.cs);
+    else expand_q8<VEC>(q, a, M, K, pitch, blockIdx.x - blocks_b, sm.codes);
+}
+// Both operands of the 4-bit product in one launch: blocks [0, blocks_b) of x do x.
+__global__ void __launch_bounds__(256) prepare_q4_kernel(q4::Weight q, __nv_bfloat16* a, Mat x, bool vec, __nv_bfloat16* b, int64_t M,
+                                                         int64_t pitch, int blocks_b) {
+    if ((int)blockIdx.x < blocks_b) split_cols(x, vec, b, M, q.K, pitch, blockIdx.x);
+    else expand_q4(q, a, pitch, blockIdx.x - blocks_b);
 }
 
 }  // namespace planes

@@ -39,7 +39,7 @@ struct Bwd {
 };
 
 // CTAs per SM that the registers have to allow: x and the residual are in flight together.
-constexpr int fwd_ctas(int floats, int threads) { return threads > 256 ? 1 : floats <= 16 ? 4 : floats <= 32 ? 3 : 2; }
+constexpr int fwd_ctas(int floats, int threads) { return threads > 512 ? 1 : threads > 256 ? 2 : floats <= 16 ? 4 : floats <= 32 ? 3 : 2; }
 
 template <int VEC, int V, int WPR, int RPC>
 __global__ void __launch_bounds__(32 * WPR * RPC, fwd_ctas(VEC * V, 32 * WPR * RPC)) fwd_kernel(const Fwd p) {
@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(32 * WPR * RPC, fwd_ctas(VEC * V, 32 * WPR * R
         for (int c = 0; c < V; ++c) {
             const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
             const bool in = f < p.K;
+            if (f - lane * VEC >= p.K) break;   // the whole warp
             if (in) {
                 float g[VEC];
                 lowbit::load_row<VEC>(g, p.gamma, 0, f);
