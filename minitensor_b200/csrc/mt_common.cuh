@@ -81,13 +81,14 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // Bounded wait on phase `parity`. Returns false (after recording `code`) when the
 // wait ran past kWaitLimitNs or another role of this CTA already gave up (*abort).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-    if (mbar_try_wait(bar, parity)) return true;
-    uint64_t t0 = globaltimer_ns();
+    uint64_t t0 = 0;   // the clock is read from the 256th try on: it takes longer than a short wait
     for (uint32_t it = 1;; ++it) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((it & 255u) == 0) {
             if (*abort_flag) return false;
-            if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > kWaitLimitNs) {
                 atomicCAS(&g_dev_status, 0, code);
                 *abort_flag = 1;
                 return false;
@@ -201,6 +202,16 @@ __device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint64_t adesc, uint6
         : "memory");
 }
 
+// True in one lane of a converged warp. Operands of tcgen05.mma live in uniform registers: in a
+// branch on elect.sync, with addresses that all lanes share (__shfl_sync for what comes from
+// shared memory) and an unrolled loop, an MMA issues in about 10 cycles; in a branch on the
+// lane number, with addresses of its own, in 45 to 200.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // Arrive (once) on `bar` when every tcgen05 op this thread issued so far is complete.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
@@ -311,13 +322,14 @@ __device__ __forceinline__ bool mbar_try_wait_cl(uint32_t bar, uint32_t parity) 
 }
 // mbar_wait for barriers that the peer CTA (or its TMA / MMA traffic) completes.
 __device__ __forceinline__ bool mbar_wait_cl(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-    if (mbar_try_wait_cl(bar, parity)) return true;
-    uint64_t t0 = globaltimer_ns();
+    uint64_t t0 = 0;   // the clock is read from the 256th try on: it takes longer than a short wait
     for (uint32_t it = 1;; ++it) {
         if (mbar_try_wait_cl(bar, parity)) return true;
         if ((it & 255u) == 0) {
             if (*abort_flag) return false;
-            if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > kWaitLimitNs) {
                 atomicCAS(&g_dev_status, 0, code);
                 *abort_flag = 1;
                 return false;

@@ -25,6 +25,9 @@ void scratch_free(void* p, size_t bytes, cudaStream_t st);
 // cuTensorMapEncodeTiled for a 2-D or 3-D map of bfloat16 elements with 128-byte swizzle:
 // extents d[0] (contiguous) .. d[rank-1], byte strides s[0..rank-2] of dims 1.., box b.
 bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* d, const uint64_t* s, const uint32_t* b);
+// The same for a 2-D map of bytes with 64-byte swizzle: d[0] (contiguous), d[1], byte stride s of
+// dim 1, box b.
+bool encode_u8(CUtensorMap* m, const void* base, const uint64_t* d, uint64_t s, const uint32_t* b);
 
 // Device status word of mt_lowbit.cu (see mt_device_status); reset != 0 clears it.
 int lowbit_device_status(int reset);

@@ -3,12 +3,14 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
+#include <cstdlib>
 
 #include "mtgemm.h"
 #include "mt_host.h"
 #include "lowbit_common.cuh"
 #include "planes_gemm.cuh"
 #include "q4.cuh"
+#include "q4_batch.cuh"
 #include "q4_gemv.cuh"
 #include "q8.cuh"
 #include "rms_norm.cuh"
@@ -294,8 +296,8 @@ void pick_splits(mt::planes::Params& p, int64_t tiles, int64_t chunk_blocks, int
 }
 
 // D = A * B^T over `kpitch` padded values of k: a [R][kpitch], b [3][C][kpitch], both bfloat16.
-// p carries the output, the scales (SCALED), the bias and spc.
-template <bool SCALED>
+// p carries the output, the scales (SCALED) and the bias.
+template <bool SCALED, int SPC>
 int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16* b, int64_t kpitch, cudaStream_t st,
                const char* who) {
     using namespace mt::planes;
@@ -306,7 +308,7 @@ int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16
     p.tiles_c = (p.C + BN - 1) / BN;
     const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c;
     if (tiles > INT32_MAX / 64) return fail(MT_EUNSUPPORTED, "%s: too many output tiles", who);
-    pick_splits(p, tiles, p.spc == 8 ? 2 : 1, clusters);
+    pick_splits(p, tiles, SPC == 8 ? 2 : 1, clusters);
     const int64_t in_parts = tiles - p.whole;
     p.units = (int)(p.whole + in_parts * p.splits);
     Scratch part(st);
@@ -323,12 +325,12 @@ int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if (!(smem_set.load() & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<SCALED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<SCALED, SPC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
         if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
         smem_set.fetch_or(bit);
     }
     const unsigned grid = 2 * (unsigned)std::min<int64_t>(p.units, clusters);
-    gemm_kernel<SCALED><<<grid, THREADS, SMEM_BYTES, st>>>(ta, tb, p);
+    gemm_kernel<SCALED, SPC><<<grid, THREADS, SMEM_BYTES, st>>>(ta, tb, p);
     MT_TRY(launched(who));
     if (in_parts) {
         join_kernel<<<dim3((unsigned)in_parts, BM / 8), 256, 0, st>>>(p);
@@ -365,7 +367,6 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     mt::planes::Params p{};
     p.R = (int)K;
     p.C = (int)N;
-    p.spc = 8;
     p.out = dw.p;
     p.os_r = dw.rs;
     p.os_c = dw.cs;
@@ -373,7 +374,7 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     p.db_tiles = db.p ? (int)tiles_m : 0;
     p.db = db.p;
     p.db_cs = db.cs;
-    return run_planes<false>(p, a, b, pitch, st, who);
+    return run_planes<false, 8>(p, a, b, pitch, st, who);
 }
 
 int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias, const Mat& y, int64_t M, int relu,
@@ -391,7 +392,6 @@ int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias,
     mt::planes::Params p{};
     p.R = (int)w.N;
     p.C = (int)M;
-    p.spc = w.group / 16;
     p.out = y.p;
     p.os_r = y.cs;
     p.os_c = y.rs;
@@ -400,7 +400,109 @@ int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias,
     p.groups = (int)((w.K + w.group - 1) / w.group);
     p.bias = bias;
     p.relu = relu;
-    return run_planes<true>(p, a, b, pitch, st, who);
+    switch (w.group) {
+        case 32: return run_planes<true, 2>(p, a, b, pitch, st, who);
+        case 64: return run_planes<true, 4>(p, a, b, pitch, st, who);
+        default: return run_planes<true, 8>(p, a, b, pitch, st, who);
+    }
+}
+
+// ------------------------------ 4 bits, batches ---------------------------------------
+
+template <int NB, int G>
+int launch_q4b(const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, dim3 grid, int cluster, cudaStream_t st,
+               const char* who) {
+    using namespace mt::q4b;
+    static std::atomic<uint64_t> smem_set{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(smem_set.load() & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<NB, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<NB>(Cfg<NB>::COLS));
+        if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
+        smem_set.fetch_or(bit);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem_bytes<NB>(p.cols);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<NB, G>, tw, tx, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return mt::host::cuda_fail(e, who);
+    }
+    return launched(who);
+}
+template <int NB>
+int launch_q4b(int group, const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, dim3 grid, int cluster,
+               cudaStream_t st, const char* who) {
+    switch (group) {
+        case 32: return launch_q4b<NB, 32>(p, tw, tx, grid, cluster, st, who);
+        case 64: return launch_q4b<NB, 64>(p, tw, tx, grid, cluster, st, who);
+        default: return launch_q4b<NB, 128>(p, tw, tx, grid, cluster, st, who);
+    }
+}
+
+int linear_q4_batch(const View2& x, const mt::q4::Weight& w, const float* bias, const Mat& y, int64_t M, int relu,
+                    cudaStream_t st, const char* who) {
+    using namespace mt::q4b;
+    const int64_t passes = (M + kRows - 1) / kRows, rows = (M + passes - 1) / passes;
+    const int64_t pitch = round_up(w.K, mt::q4::kSpan), tiles = (w.N + 127) / 128;
+    if (passes > 65535 || tiles > INT32_MAX / 16) return fail(MT_EUNSUPPORTED, "%s: too many tiles", who);
+    Scratch ws(st);
+    MT_TRY(ws.take((size_t)passes * 3 * rows * pitch * 2, who));
+    __nv_bfloat16* parts = static_cast<__nv_bfloat16*>(ws.p);
+    split_passes_kernel<<<dim3((unsigned)((pitch / 4 + 255) / 256), (unsigned)rows, (unsigned)passes), 256, 0, st>>>(
+        x.m, vec4(x), parts, M, w.K, pitch, (int)rows);
+    MT_TRY(launched(who));
+    Params p{};
+    p.N = w.N;
+    p.M = M;
+    p.rows = (int)rows;
+    p.cols = (int)round_up(3 * rows, 16);
+    p.spans = (int)(pitch / mt::q4::kSpan);
+    p.groups = (int)((w.K + w.group - 1) / w.group);
+    p.scales = w.scales;
+    p.sp = w.sp;
+    p.bias = bias;
+    p.y = y;
+    p.relu = relu;
+    p.stage_bytes = stage_bytes(p.cols);
+    CUtensorMap tw, tx;
+    const uint64_t dw[2] = {(uint64_t)p.spans * 64, (uint64_t)w.N}, dx[2] = {(uint64_t)pitch, (uint64_t)(passes * 3 * rows)};
+    const uint64_t sx[1] = {(uint64_t)pitch * 2};
+    const uint32_t bw[2] = {64, 128}, bx[2] = {64, (uint32_t)p.cols};
+    if (!mt::host::encode_u8(&tw, w.codes, dw, (uint64_t)w.cp * 4, bw) || !mt::host::encode_bf16(&tx, parts, 2, dx, sx, bx))
+        return fail(MT_ECUDA, "%s: tensor map encoding failed", who);
+    // CTAs of a cluster, which split k: rounds x (spans of a CTA, and what its start and end take:
+    // about ten spans' time, two more for the cluster's sum).
+    const int nb = (int)(rows + 15) / 16;
+    const int64_t slots = mt::host::sm_count();
+    int cluster = 1;
+    int64_t least = INT64_MAX;
+    for (int s = 1; s <= 8 && s <= p.spans; s *= 2) {
+        const int64_t cost = (tiles * passes * s + slots - 1) / slots * ((p.spans + s - 1) / s + 10 + (s > 1 ? 2 : 0));
+        if (cost < least) { least = cost; cluster = s; }
+    }
+    const dim3 grid((unsigned)(tiles * cluster), (unsigned)passes);
+    switch (nb) {
+        case 1: MT_TRY(launch_q4b<1>(w.group, p, tw, tx, grid, cluster, st, who)); break;
+        case 2: MT_TRY(launch_q4b<2>(w.group, p, tw, tx, grid, cluster, st, who)); break;
+        case 3: MT_TRY(launch_q4b<3>(w.group, p, tw, tx, grid, cluster, st, who)); break;
+        default: MT_TRY(launch_q4b<4>(w.group, p, tw, tx, grid, cluster, st, who)); break;
+    }
+    char path[96];
+    snprintf(path, sizeof path, "%s batch rows=%d x %d cluster=%d", who, p.rows, (int)passes, cluster);
+    mt::host::set_path(path);
+    return MT_OK;
 }
 
 // ------------------------------- 4 bits, few rows -------------------------------------
@@ -757,7 +859,14 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     const int64_t M = vx.rows;
     if (M * w.N == 0) return MT_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (M > 64 && w.K > 0) return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
+    static const char* force = getenv("MT_Q4");
+    if (force && w.K > 0) {
+        if (force[0] == 'b') return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
+        if (force[0] == 'p') return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
+        return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
+    }
+    if (M > 256 && w.K > 0) return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
+    if (M > 8 && w.K > 0) return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
     return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
 }
 

@@ -11,7 +11,7 @@
 //
 // Accumulation. The tensor core adds into its accumulator by truncation, so a long sum
 // drifts towards zero by about one part in 2^24 per step; over thousands of rows that
-// exceeds a float sum's error. The accumulator is therefore drained every `spc` k-steps
+// exceeds a float sum's error. The accumulator is therefore drained every SPC k-steps
 // (32 to 128 values of k) into registers that add with rounding, while the next chunk goes
 // into the other half of TMEM. The 4-bit product multiplies by the group's scale there, once
 // per group instead of once per weight.
@@ -50,7 +50,6 @@ static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 struct Params {
     int R, C;                    // rows of A, rows of B
     int kblocks;                 // 64-deep blocks of k
-    int spc;                     // k16-steps per chunk: 2, 4 or 8
     int tiles_r, tiles_c;
     int whole, splits;           // tiles [0, whole) are done at once, the others in `splits` parts of k
     int units;                   // whole + splits * (tiles - whole)
@@ -79,6 +78,7 @@ __device__ __forceinline__ void tile_of(const Params& p, int t, int& rb, int& cb
     rb = g * 8 + in - cb * rows;
 }
 // Unit u -> tile, part and the k-blocks [kb0, kb1) of the part, which begins on a chunk. sp < 0: whole.
+template <int SPC>
 __device__ __forceinline__ int unit_of(const Params& p, int u, int& sp, int& kb0, int& kb1) {
     if (u < p.whole) {
         sp = -1;
@@ -88,7 +88,7 @@ __device__ __forceinline__ int unit_of(const Params& p, int u, int& sp, int& kb0
     }
     const int t = (u - p.whole) / p.splits;
     sp = u - p.whole - t * p.splits;
-    const int cpb = p.spc == 8 ? 2 : 1;                        // k-blocks per chunk boundary
+    constexpr int cpb = SPC == 8 ? 2 : 1;                      // k-blocks per chunk boundary
     const int nb = (p.kblocks + cpb - 1) / cpb;
     kb0 = (int)((long long)nb * sp / p.splits) * cpb;
     kb1 = min(p.kblocks, (int)((long long)nb * (sp + 1) / p.splits) * cpb);
@@ -109,7 +109,8 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t adesc, 
         : "memory");
 }
 
-template <bool SCALED>
+// SPC: k16-steps per chunk, 2, 4 or 8.
+template <bool SCALED, int SPC>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
     extern __shared__ uint8_t smem_raw[];
@@ -152,7 +153,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     tc_fence_before();
     cluster_sync_all();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     int rb, cb, sp, kb0, kb1;
     if (warp == 0) {
@@ -160,7 +161,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             int s = 0;
             uint32_t ph = 0;
             for (int u = first; u < p.units; u += step) {
-                tile_of(p, unit_of(p, u, sp, kb0, kb1), rb, cb);
+                tile_of(p, unit_of<SPC>(p, u, sp, kb0, kb1), rb, cb);
                 const int r0 = rb * BM + (int)rank * 128, c0 = cb * BN + (int)rank * 128;
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!mbar_wait_cl(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) goto done;
@@ -174,44 +175,49 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        if (leader && elect_one()) {
             constexpr uint32_t idesc = idesc_bf16(BM, BN);
-            const int nsub = p.spc == 2 ? 2 : 1, steps = 4 / nsub;
+            constexpr int STEPS = SPC == 2 ? 2 : 4;    // of a chunk in one stage
+            const uint64_t a0 = umma_desc(smem_u32(ring), 16, 1024, kLayoutSw128);
+            const uint32_t peer = 1;
             int s = 0, n = 0;          // stage, chunks begun
             uint32_t ph = 0;
-            for (int u = first; u < p.units; u += step) {
-                unit_of(p, u, sp, kb0, kb1);
+            bool ok = true;
+            for (int u = first; u < p.units && ok; u += step) {
+                unit_of<SPC>(p, u, sp, kb0, kb1);
                 int in_chunk = 0;
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait_cl(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) goto done;
+                    ok = mbar_wait_cl(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(ring + s * STAGE_BYTES);
-                    for (int sub = 0; sub < nsub; ++sub) {
+                    const uint64_t sa = a0 + s * (STAGE_BYTES >> 4);
+#pragma unroll
+                    for (int sub = 0; sub < 4; sub += STEPS) {
                         const int a = n & 1;
                         if (in_chunk == 0) {
-                            if (!mbar_wait_cl(smem_u32(&acc_empty[a]), ((n >> 1) & 1) ^ 1, abort_flag, kDevTimeoutAccEmpty))
-                                goto done;
+                            ok = mbar_wait_cl(smem_u32(&acc_empty[a]), ((n >> 1) & 1) ^ 1, abort_flag, kDevTimeoutAccEmpty);
+                            if (!ok) break;
                             tc_fence_after();
                         }
+                        const uint32_t more = in_chunk > 0 ? 1u : 0u;
                         // Smallest plane first: its sums meet a small accumulator.
-                        for (int pl = 2; pl >= 0; --pl) {
-                            const uint32_t sb = sa + A_BYTES + pl * B_BYTES;
-                            for (int k = sub * steps; k < (sub + 1) * steps; ++k) {
-                                umma_bf16_pair(tmem_base + a * BN, umma_desc(sa + k * 32, 16, 1024, kLayoutSw128),
-                                               umma_desc(sb + k * 32, 16, 1024, kLayoutSw128), idesc,
-                                               in_chunk > 0 || pl < 2 || k > sub * steps ? 1u : 0u);
-                            }
-                        }
-                        in_chunk += steps;
-                        if (in_chunk == p.spc || (kb == kb1 - 1 && sub == nsub - 1)) {
+#pragma unroll
+                        for (int pl = 2; pl >= 0; --pl)
+#pragma unroll
+                            for (int k = sub; k < sub + STEPS; ++k)
+                                umma_bf16_pair(tmem_base + a * BN, sa + k * 2, sa + ((A_BYTES + pl * B_BYTES) >> 4) + k * 2, idesc,
+                                               pl < 2 || k > sub ? 1u : more);
+                        in_chunk += STEPS;
+                        if (in_chunk == SPC || (kb == kb1 - 1 && sub + STEPS == 4)) {
                             umma_commit_pair(smem_u32(&acc_full[a]));
-                            umma_commit_pair(mapa_shared(smem_u32(&acc_full[a]), 1));
+                            umma_commit_pair(mapa_shared(smem_u32(&acc_full[a]), peer));
                             ++n;
                             in_chunk = 0;
                         }
                     }
+                    if (!ok) break;
                     umma_commit_pair(smem_u32(&empty[s]));
-                    umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 1));
+                    umma_commit_pair(mapa_shared(smem_u32(&empty[s]), peer));
                     if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
             }
@@ -232,13 +238,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
         }
         for (int u = first; u < p.units; u += step) {
-            const int tile = unit_of(p, u, sp, kb0, kb1);
+            const int tile = unit_of<SPC>(p, u, sp, kb0, kb1);
             tile_of(p, tile, rb, cb);
             const int row0 = rb * BM + (int)rank * 128 + q * 32;
             const int col0 = cb * BN + half * 128;
-            const int chunks = ((kb1 - kb0) * 4 + p.spc - 1) / p.spc;
+            const int chunks = ((kb1 - kb0) * 4 + SPC - 1) / SPC;
             const __nv_bfloat16* sc = nullptr;
-            const int g0 = kb0 * 4 / p.spc;
+            const int g0 = kb0 * 4 / SPC;
             if (SCALED) sc = p.scales + (int64_t)min(row0 + lane, p.R - 1) * p.sp;
             float acc[128];
 #pragma unroll
@@ -418,9 +424,10 @@ __device__ __forceinline__ void split_rows(const Mat& x, __nv_bfloat16* out, int
     }
 }
 
-// Planes of B for a sum over columns of x [M, K]: out[plane][m][k], k padded with zeros to `pitch`
-// (a multiple of 4).
-__device__ __forceinline__ void split_cols(const Mat& x, bool vec, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch, int block) {
+// Planes of B for a sum over columns of x [M, K]: out[plane][m][k], planes of plane_rows rows, k
+// padded with zeros to `pitch` (a multiple of 4).
+__device__ __forceinline__ void split_cols(const Mat& x, bool vec, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch, int block,
+                                           int64_t plane_rows) {
     const int64_t k = ((int64_t)block * 256 + threadIdx.x) * 4;
     if (k >= pitch) return;
 #pragma unroll 4
@@ -438,7 +445,7 @@ __device__ __forceinline__ void split_cols(const Mat& x, bool vec, __nv_bfloat16
         }
 #pragma unroll
         for (int pl = 0; pl < 3; ++pl)
-            *reinterpret_cast<uint2*>(out + (pl * M + m) * pitch + k) =
+            *reinterpret_cast<uint2*>(out + (pl * plane_rows + m) * pitch + k) =
                 make_uint2(o[0][pl] | ((uint32_t)o[1][pl] << 16), o[2][pl] | ((uint32_t)o[3][pl] << 16));
     }
 }
@@ -526,7 +533,7 @@ __global__ void __launch_bounds__(256) prepare_q8_kernel(lowbit::Q8 q, __nv_bflo
 // Both operands of the 4-bit product in one launch: blocks [0, blocks_b) of x do x.
 __global__ void __launch_bounds__(256) prepare_q4_kernel(q4::Weight q, __nv_bfloat16* a, Mat x, bool vec, __nv_bfloat16* b, int64_t M,
                                                          int64_t pitch, int blocks_b) {
-    if ((int)blockIdx.x < blocks_b) split_cols(x, vec, b, M, q.K, pitch, blockIdx.x);
+    if ((int)blockIdx.x < blocks_b) split_cols(x, vec, b, M, q.K, pitch, blockIdx.x, M);
     else expand_q4(q, a, pitch, blockIdx.x - blocks_b);
 }
 

@@ -1,0 +1,361 @@
+// q4_batch.cuh -- y = x W + b with 4-bit weights for batches of rows: tcgen05 with the unpacked
+// weights in tensor memory.
+//
+// Mathematics: x = h + m + l exactly, three bfloat16 parts (split3), as in planes_gemm.cuh. The
+// parts of up to 64 rows stand side by side as the columns of one MMA tile,
+//   D[n][part, row] = sum over a group of (c[n][k] - 8) / kCodeUnit * part[row][k],
+// and y gathers scale[n] * (h + m + l) group by group in registers, added with rounding.
+//
+// Why this shape. Up to some hundred rows the weights' bytes bound the product (0.5 byte per
+// weight at 6.5 TB/s: 8192 weights of a 128 x 64 step in 182 cycles of an SM). Unpacked to
+// bfloat16 in shared memory, a weight would cost 2 bytes written and 2 read for every MMA on it,
+// 128 bytes a cycle being all there is. So a thread unpacks its row of the step into 32
+// registers (11 instructions per 8 weights) and stores them to tensor memory, from where the
+// MMA takes them; shared memory carries only the packed codes and the parts of x.
+//
+// Work. A CTA has 128 weight rows and a range of spans of 128 k; the CTAs of a cluster share
+// the rows and split k, and add their sums through distributed shared memory in order. Warp 0
+// loads by TMA (codes and x parts of a span per stage), warp 1 issues the MMAs, warps 2-9
+// unpack (lane quarter = warp & 3; the first four the first 64 k of a span, the others the
+// rest), warps 10-17 drain the accumulator of every group, half of the rows of x each.
+// Steps are short (a 64-deep one is 182 cycles of memory), so what bounds them is the
+// hand-over between the roles: all of tensor memory goes into unpacked steps and accumulators
+// in flight. blockIdx.y takes up to 64 rows of x each.
+#pragma once
+
+#include "planes_gemm.cuh"
+
+namespace mt {
+namespace q4b {
+
+using lowbit::Mat;
+
+constexpr int kRows = 64;                 // rows of x per blockIdx.y, at most
+constexpr int THREADS = 32 * 18;
+constexpr int EPI_WARPS = 8;
+constexpr uint32_t CODE_BYTES = 128 * 64; // a span of 128 weight rows
+
+// Sizes by NB, the blocks of 8 rows of x per drain warp: 16 NB rows of x at most.
+template <int NB>
+struct Cfg {
+    static constexpr int ROWS = 16 * NB;
+    static constexpr int COLS = 48 * NB;                       // columns of the MMA tile at most
+    static constexpr int ACC = NB == 1 ? 4 : NB == 2 ? 3 : 2;  // accumulators
+    static constexpr int A_STAGES = NB == 1 ? 8 : NB <= 3 ? 6 : 4;   // unpacked 64-deep steps of 32 columns
+    static constexpr int STAGES = NB <= 2 ? 6 : NB == 3 ? 4 : 3;
+    static_assert(ACC * COLS + 32 * A_STAGES <= 512, "tensor memory");
+    static_assert(A_STAGES % 2 == 0, "each half of a span has its own steps");
+};
+
+struct Params {
+    int64_t N;                   // weight rows (outputs)
+    int64_t M;
+    int rows;                    // of x per blockIdx.y
+    int cols;                    // MMA tile width: 3 rows, rounded up to 16
+    int spans, groups;
+    const __nv_bfloat16* scales;
+    int64_t sp;
+    const float* bias;
+    Mat y;
+    int relu;
+    uint32_t stage_bytes;
+};
+
+__host__ __device__ constexpr uint32_t stage_bytes(int cols) { return CODE_BYTES + 2u * cols * 128u; }
+template <int NB>
+__host__ __device__ constexpr uint32_t smem_bytes(int cols) {
+    return 1024 + Cfg<NB>::STAGES * stage_bytes(cols) + 8 * (2 * Cfg<NB>::STAGES + 2 * Cfg<NB>::A_STAGES + 2 * Cfg<NB>::ACC) + 16;
+}
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+// D (+)= A[tmem] * B[smem]^T, bfloat16, one CTA.
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// (c - 8) / kCodeUnit of a word's 8 codes, in order, as four pairs: 128 + c is a bfloat16 with c
+// in its low bits, and one multiply-add takes 128 + 8 off and scales, exactly.
+__device__ __forceinline__ void unpack8(uint32_t w, uint32_t* o) {
+    const __nv_bfloat162 unit = __floats2bfloat162_rn(1.f / planes::kCodeUnit, 1.f / planes::kCodeUnit);
+    const __nv_bfloat162 off = __floats2bfloat162_rn(-136.f / planes::kCodeUnit, -136.f / planes::kCodeUnit);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+        const __nv_bfloat162 d = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v), unit, off);
+        o[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+}
+
+template <int NB, int G>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Params p) {
+    using C = Cfg<NB>;
+    constexpr int SPC = G / 16;               // k16-steps per group
+    constexpr int CHUNKS = 128 / G;           // groups per span
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * p.stage_bytes);
+    uint64_t* full = bars;
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* a_full = empty + C::STAGES;
+    uint64_t* a_empty = a_full + C::A_STAGES;
+    uint64_t* acc_full = a_empty + C::A_STAGES;
+    uint64_t* acc_empty = acc_full + C::ACC;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(acc_empty + C::ACC);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_empty + C::ACC) + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank(), ranks = (int)cluster_nctarank();
+    const int tile = (int)blockIdx.x / ranks;
+    const int s0 = (int)((int64_t)p.spans * rank / ranks), s1 = (int)((int64_t)p.spans * (rank + 1) / ranks);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 9);            // eight unpacking warps, the MMAs
+        }
+        for (int s = 0; s < C::A_STAGES; ++s) {
+            mbar_init(smem_u32(&a_full[s]), 4);
+            mbar_init(smem_u32(&a_empty[s]), 1);
+        }
+        for (int a = 0; a < C::ACC; ++a) {
+            mbar_init(smem_u32(&acc_full[a]), 1);
+            mbar_init(smem_u32(&acc_empty[a]), EPI_WARPS);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmX);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32((const void*)tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const uint32_t tmem_a = tmem_base + C::ACC * C::COLS;
+    float* red = reinterpret_cast<float*>(smem);          // [rows of x][128], once the ring is idle
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            for (int i = s0; i < s1; ++i) {
+                if (!mbar_wait(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
+                const uint32_t to = smem_u32(smem + s * p.stage_bytes), bar = smem_u32(&full[s]);
+                mbar_arrive_expect_tx(bar, p.stage_bytes);
+                tma_load_2d(to + 2 * p.cols * 128, &tmW, bar, i * 64, tile * 128);
+                tma_load_2d(to, &tmX, bar, i * 128, (int)blockIdx.y * 3 * p.rows);
+                tma_load_2d(to + p.cols * 128, &tmX, bar, i * 128 + 64, (int)blockIdx.y * 3 * p.rows);
+                if (++s == C::STAGES) { s = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t idesc = planes::idesc_bf16(128, p.cols);
+            const uint64_t b0 = umma_desc(smem_u32(smem), 16, 1024, kLayoutSw128);
+            const uint32_t stage_step = p.stage_bytes >> 4, half_step = (uint32_t)p.cols * 128 >> 4;
+            int s = 0, ab = 0, n = 0;
+            uint32_t ph = 0, aph = 0, nph = 0;
+            bool ok = true;
+            for (int i = s0; i < s1; ++i) {
+                if (!mbar_wait(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) break;
+#pragma unroll
+                for (int step = 0; step < 8; ++step) {
+                    if (step % SPC == 0) ok = mbar_wait(smem_u32(&acc_empty[n]), nph ^ 1, abort_flag, kDevTimeoutAccEmpty);
+                    if (step % 4 == 0 && ok) ok = mbar_wait(smem_u32(&a_full[ab]), aph, abort_flag, kDevTimeoutMisc);
+                    if (!ok) break;
+                    if (step % SPC == 0 || step % 4 == 0) tc_fence_after();
+                    umma_bf16_ts(tmem_base + n * C::COLS, tmem_a + ab * 32 + step % 4 * 8,
+                                 b0 + s * stage_step + step / 4 * half_step + step % 4 * 2, idesc, step % SPC ? 1u : 0u);
+                    if (step % SPC == SPC - 1) {
+                        umma_commit(smem_u32(&acc_full[n]));
+                        if (++n == C::ACC) { n = 0; nph ^= 1; }
+                    }
+                    if (step % 4 == 3) {
+                        umma_commit(smem_u32(&a_empty[ab]));
+                        if (++ab == C::A_STAGES) { ab = 0; aph ^= 1; }
+                    }
+                }
+                if (!ok) break;
+                umma_commit(smem_u32(&empty[s]));
+                if (++s == C::STAGES) { s = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp < 10) {
+        // Row `row` of the weight tile, one half of each span. TMA puts 16-byte piece t of a row
+        // at piece t ^ (row / 2 % 4).
+        const int q = warp & 3, row = q * 32 + lane, half = (warp - 2) >> 2;
+        int s = 0, ab = half;
+        uint32_t ph = 0, aph = 0;
+        for (int i = s0; i < s1; ++i) {
+            if (!mbar_wait_warp(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) break;
+            const uint8_t* codes = smem + s * p.stage_bytes + 2 * p.cols * 128 + row * 64 + half * 8;
+            uint2 w[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint2*>(codes + ((t ^ ((row >> 1) & 3)) << 4));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+            if (++s == C::STAGES) { s = 0; ph ^= 1; }
+            uint32_t r[32];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                unpack8(w[t].x, r + t * 4);
+                unpack8(w[t].y, r + 16 + t * 4);
+            }
+            if (!mbar_wait_warp(smem_u32(&a_empty[ab]), aph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
+            tc_fence_after();
+            tmem_st_32x32b_x32(tmem_a + ((uint32_t)(q * 32) << 16) + ab * 32, r);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&a_full[ab]));
+            if ((ab += 2) >= C::A_STAGES) { ab = half; aph ^= 1; }
+        }
+    } else {
+        const int q = warp & 3, half = (warp - 10) >> 2;
+        const int64_t row = (int64_t)tile * 128 + q * 32 + lane;
+        const uint16_t* sc = reinterpret_cast<const uint16_t*>(p.scales) + min(row, p.N - 1) * p.sp;
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * (8 * NB);
+        float acc[8 * NB];
+#pragma unroll
+        for (int j = 0; j < 8 * NB; ++j) acc[j] = 0.f;
+        const int g0 = s0 * CHUNKS, chunks = (s1 - s0) * CHUNKS;
+        // Scales of four groups are loaded together, while the four before them are at work: one
+        // at a time, each group would wait for a load.
+        uint16_t next[4];
+        auto load_scales = [&](int n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) next[i] = n + i < chunks && g0 + n + i < p.groups ? __ldg(sc + g0 + n + i) : (uint16_t)0;
+        };
+        load_scales(0);
+        bool ok = true;
+        int n = 0;
+        uint32_t nph = 0;
+#pragma unroll 1
+        for (int n0 = 0; n0 < chunks && ok; n0 += 4) {
+            float scale[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) scale[i] = __uint_as_float((uint32_t)next[i] << 16);
+            load_scales(n0 + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (n0 + i >= chunks) break;
+                ok = mbar_wait_warp(smem_u32(&acc_full[n]), nph, abort_flag, kDevTimeoutAccFull);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t t0 = taddr + n * C::COLS;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t h[8], m[8], l[8];
+                    tmem_ld_32x32b_x8(t0 + b * 8, h);
+                    tmem_ld_32x32b_x8(t0 + p.rows + b * 8, m);
+                    tmem_ld_32x32b_x8(t0 + 2 * p.rows + b * 8, l);
+                    tmem_ld_wait();
+                    if (b == NB - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&acc_empty[n]));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        acc[b * 8 + j] = fmaf(scale[i], __uint_as_float(h[j]) + (__uint_as_float(m[j]) + __uint_as_float(l[j])), acc[b * 8 + j]);
+                }
+                if (++n == C::ACC) { n = 0; nph ^= 1; }
+            }
+        }
+        const float bias = p.bias && row < p.N ? p.bias[row] : 0.f;
+        const int64_t m0 = (int64_t)blockIdx.y * p.rows;
+#pragma unroll
+        for (int j = 0; j < 8 * NB; ++j) {
+            const int m = half * (8 * NB) + j;
+            if (m < p.rows) {
+                if (ranks > 1) {
+                    red[m * 128 + q * 32 + lane] = acc[j];
+                } else if (m0 + m < p.M && row < p.N) {
+                    float v = fmaf(acc[j], planes::kCodeUnit, bias);
+                    if (p.relu) v = v > 0.f ? v : 0.f;
+                    p.y.p[(m0 + m) * p.y.rs + row * p.y.cs] = v;
+                }
+            }
+        }
+    }
+    if (ranks > 1) {
+        // Every rank adds its share of the rows of x, the parts of k in order.
+        cluster_sync_all();
+        const int64_t m0 = (int64_t)blockIdx.y * p.rows, n0 = (int64_t)tile * 128;
+        for (int i = threadIdx.x; i < p.rows * 128; i += THREADS) {
+            const int m = i >> 7, r = i & 127;
+            if (m % ranks != rank || m0 + m >= p.M || n0 + r >= p.N) continue;
+            float v = 0.f;
+            for (int k = 0; k < ranks; ++k) v += ld_cluster(mapa_shared(smem_u32(red + i), k));
+            v = fmaf(v, planes::kCodeUnit, p.bias ? p.bias[n0 + r] : 0.f);
+            if (p.relu) v = v > 0.f ? v : 0.f;
+            p.y.p[(m0 + m) * p.y.rs + (n0 + r) * p.y.cs] = v;
+        }
+        cluster_sync_all();   // the others have read this CTA's sums
+    }
+    if (warp == 0 && lane == 0 && *abort_flag) {
+        // Give copies already issued time to land before the CTA leaves.
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// The parts of x for q4b::gemm_kernel: out[pass][part][row of the pass][k].
+__global__ void __launch_bounds__(256) split_passes_kernel(Mat x, bool vec, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch, int rows) {
+    const int64_t m0 = (int64_t)blockIdx.z * rows;
+    const Mat part{x.p + m0 * x.rs, x.rs, x.cs};
+    planes::split_cols(part, vec, out + (int64_t)blockIdx.z * 3 * rows * pitch, min((int64_t)rows, M - m0), K, pitch, blockIdx.x, rows);
+}
+
+}  // namespace q4b
+}  // namespace mt
