@@ -97,6 +97,37 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// The same bounded wait for many roles with short steps: one try in place, and all further ones
+// in a function of their own, so that the roles' code stays small, with a suspend-time hint
+// (20 us a try), so that those who wait leave the issue slots to the others.
+static __device__ __noinline__ bool mbar_wait_more(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+    uint64_t t0 = 0;
+    for (uint32_t it = 1;; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity), "r"(20000u)
+            : "memory");
+        if (ok) return true;
+        if ((it & 63u) == 0) {
+            if (*abort_flag) return false;
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > kWaitLimitNs) {
+                atomicCAS(&g_dev_status, 0, code);
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ bool mbar_wait_short(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+    return mbar_try_wait(bar, parity) || mbar_wait_more(bar, parity, abort_flag, code);
+}
+
 // Warp-cooperative bounded wait for roles where a whole warp consumes the phase: lane 0
 // spins (a warp of spinning threads would compete with the producer and MMA threads for
 // the barrier unit), then every lane issues one try_wait of its own, which succeeds at

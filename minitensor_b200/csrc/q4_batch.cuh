@@ -15,12 +15,12 @@
 //
 // Work. A CTA has 128 weight rows and a range of spans of 128 k; the CTAs of a cluster share
 // the rows and split k, and add their sums through distributed shared memory in order. Warp 0
-// loads by TMA (codes and x parts of a span per stage), warp 1 issues the MMAs, warps 2-9
-// unpack (lane quarter = warp & 3; the first four the first 64 k of a span, the others the
-// rest), warps 10-17 drain the accumulator of every group, half of the rows of x each.
-// Steps are short (a 64-deep one is 182 cycles of memory), so what bounds them is the
-// hand-over between the roles: all of tensor memory goes into unpacked steps and accumulators
-// in flight. blockIdx.y takes up to 64 rows of x each.
+// loads by TMA (codes and x parts of a span per stage). The two 64-deep halves of a span go
+// their own ways: warps 1 and 2 issue their MMAs, warps 4-7 and 8-11 unpack (lane quarter =
+// warp & 3), each with its own accumulators and unpacked steps in tensor memory. Warps 12-19
+// drain the accumulators, half of the rows of x each. What bounds a step is the roles'
+// instructions and hand-overs (a half is 182 cycles of memory, an MMA 24 cycles at 16 rows of
+// x), hence two issuers and waits in few instructions. blockIdx.y takes up to 64 rows of x each.
 #pragma once
 
 #include "planes_gemm.cuh"
@@ -31,7 +31,7 @@ namespace q4b {
 using lowbit::Mat;
 
 constexpr int kRows = 64;                 // rows of x per blockIdx.y, at most
-constexpr int THREADS = 32 * 18;
+constexpr int THREADS = 32 * 20;
 constexpr int EPI_WARPS = 8;
 constexpr uint32_t CODE_BYTES = 128 * 64; // a span of 128 weight rows
 
@@ -40,11 +40,10 @@ template <int NB>
 struct Cfg {
     static constexpr int ROWS = 16 * NB;
     static constexpr int COLS = 48 * NB;                       // columns of the MMA tile at most
-    static constexpr int ACC = NB == 1 ? 4 : NB == 2 ? 3 : 2;  // accumulators
-    static constexpr int A_STAGES = NB == 1 ? 8 : NB <= 3 ? 6 : 4;   // unpacked 64-deep steps of 32 columns
+    static constexpr int ACC = NB == 1 ? 3 : NB == 2 ? 2 : 1;       // accumulators of a half
+    static constexpr int A_STAGES = NB <= 1 ? 3 : NB == 2 ? 2 : 3 - (NB == 4);   // unpacked steps of a half, 32 columns each
     static constexpr int STAGES = NB <= 2 ? 6 : NB == 3 ? 4 : 3;
-    static_assert(ACC * COLS + 32 * A_STAGES <= 512, "tensor memory");
-    static_assert(A_STAGES % 2 == 0, "each half of a span has its own steps");
+    static_assert(2 * ACC * COLS + 64 * A_STAGES <= 512, "tensor memory");
 };
 
 struct Params {
@@ -64,7 +63,7 @@ struct Params {
 __host__ __device__ constexpr uint32_t stage_bytes(int cols) { return CODE_BYTES + 2u * cols * 128u; }
 template <int NB>
 __host__ __device__ constexpr uint32_t smem_bytes(int cols) {
-    return 1024 + Cfg<NB>::STAGES * stage_bytes(cols) + 8 * (2 * Cfg<NB>::STAGES + 2 * Cfg<NB>::A_STAGES + 2 * Cfg<NB>::ACC) + 16;
+    return 1024 + Cfg<NB>::STAGES * stage_bytes(cols) + 8 * (2 * Cfg<NB>::STAGES + 4 * Cfg<NB>::A_STAGES + 4 * Cfg<NB>::ACC) + 16;
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
@@ -128,19 +127,19 @@ template <int NB, int G>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Params p) {
     using C = Cfg<NB>;
-    constexpr int SPC = G / 16;               // k16-steps per group
-    constexpr int CHUNKS = 128 / G;           // groups per span
+    constexpr int SPC = G == 32 ? 2 : 4;      // k16-steps per accumulator: a group, or half of one
+    constexpr int CHUNKS = 4 / SPC;           // accumulators per half of a span
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * p.stage_bytes);
     uint64_t* full = bars;
     uint64_t* empty = full + C::STAGES;
     uint64_t* a_full = empty + C::STAGES;
-    uint64_t* a_empty = a_full + C::A_STAGES;
-    uint64_t* acc_full = a_empty + C::A_STAGES;
-    uint64_t* acc_empty = acc_full + C::ACC;
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(acc_empty + C::ACC);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_empty + C::ACC) + 1;
+    uint64_t* a_empty = a_full + 2 * C::A_STAGES;          // [half][step]
+    uint64_t* acc_full = a_empty + 2 * C::A_STAGES;
+    uint64_t* acc_empty = acc_full + 2 * C::ACC;           // [half][accumulator]
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(acc_empty + 2 * C::ACC);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_empty + 2 * C::ACC) + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank(), ranks = (int)cluster_nctarank();
@@ -150,13 +149,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
             mbar_init(smem_u32(&full[s]), 1);
-            mbar_init(smem_u32(&empty[s]), 9);            // eight unpacking warps, the MMAs
+            mbar_init(smem_u32(&empty[s]), 10);           // eight unpacking warps, two issuers
         }
-        for (int s = 0; s < C::A_STAGES; ++s) {
+        for (int s = 0; s < 2 * C::A_STAGES; ++s) {
             mbar_init(smem_u32(&a_full[s]), 4);
             mbar_init(smem_u32(&a_empty[s]), 1);
         }
-        for (int a = 0; a < C::ACC; ++a) {
+        for (int a = 0; a < 2 * C::ACC; ++a) {
             mbar_init(smem_u32(&acc_full[a]), 1);
             mbar_init(smem_u32(&acc_empty[a]), EPI_WARPS);
         }
@@ -175,15 +174,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const uint32_t tmem_a = tmem_base + C::ACC * C::COLS;
+    const uint32_t tmem_a = tmem_base + 2 * C::ACC * C::COLS;
     float* red = reinterpret_cast<float*>(smem);          // [rows of x][128], once the ring is idle
 
+    float acc[8 * NB];   // of the draining warps
     if (warp == 0) {
         if (lane == 0) {
             int s = 0;
             uint32_t ph = 0;
             for (int i = s0; i < s1; ++i) {
-                if (!mbar_wait(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
+                if (!mbar_wait_short(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
                 const uint32_t to = smem_u32(smem + s * p.stage_bytes), bar = smem_u32(&full[s]);
                 mbar_arrive_expect_tx(bar, p.stage_bytes);
                 tma_load_2d(to + 2 * p.cols * 128, &tmW, bar, i * 64, tile * 128);
@@ -192,46 +192,50 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
                 if (++s == C::STAGES) { s = 0; ph ^= 1; }
             }
         }
-    } else if (warp == 1) {
+    } else if (warp <= 2) {
+        const int half = __shfl_sync(0xffffffffu, warp, 0) - 1;
         if (elect_one()) {
             const uint32_t idesc = planes::idesc_bf16(128, p.cols);
-            const uint64_t b0 = umma_desc(smem_u32(smem), 16, 1024, kLayoutSw128);
-            const uint32_t stage_step = p.stage_bytes >> 4, half_step = (uint32_t)p.cols * 128 >> 4;
+            uint64_t b = umma_desc(smem_u32(smem) + half * p.cols * 128, 16, 1024, kLayoutSw128);
+            const uint32_t acc0 = tmem_base + half * C::ACC * C::COLS, a0 = tmem_a + half * C::A_STAGES * 32;
+            const uint32_t a_bar = smem_u32(a_full + half * C::A_STAGES), acc_bar = smem_u32(acc_full + half * C::ACC);
             int s = 0, ab = 0, n = 0;
             uint32_t ph = 0, aph = 0, nph = 0;
-            bool ok = true;
             for (int i = s0; i < s1; ++i) {
-                if (!mbar_wait(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) break;
+                if (!mbar_wait_short(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) break;
+                if (!mbar_wait_short(a_bar + ab * 8, aph, abort_flag, kDevTimeoutMisc)) break;
+                bool ok = true;
 #pragma unroll
-                for (int step = 0; step < 8; ++step) {
-                    if (step % SPC == 0) ok = mbar_wait(smem_u32(&acc_empty[n]), nph ^ 1, abort_flag, kDevTimeoutAccEmpty);
-                    if (step % 4 == 0 && ok) ok = mbar_wait(smem_u32(&a_full[ab]), aph, abort_flag, kDevTimeoutMisc);
-                    if (!ok) break;
-                    if (step % SPC == 0 || step % 4 == 0) tc_fence_after();
-                    umma_bf16_ts(tmem_base + n * C::COLS, tmem_a + ab * 32 + step % 4 * 8,
-                                 b0 + s * stage_step + step / 4 * half_step + step % 4 * 2, idesc, step % SPC ? 1u : 0u);
-                    if (step % SPC == SPC - 1) {
-                        umma_commit(smem_u32(&acc_full[n]));
-                        if (++n == C::ACC) { n = 0; nph ^= 1; }
+                for (int step = 0; step < 4; ++step) {
+                    if (step % SPC == 0) {
+                        ok = mbar_wait_short(acc_bar + (2 * C::ACC + n) * 8, nph ^ 1, abort_flag, kDevTimeoutAccEmpty);
+                        if (!ok) break;
+                        tc_fence_after();
                     }
-                    if (step % 4 == 3) {
-                        umma_commit(smem_u32(&a_empty[ab]));
-                        if (++ab == C::A_STAGES) { ab = 0; aph ^= 1; }
+                    umma_bf16_ts(acc0 + n * C::COLS, a0 + ab * 32 + step * 8, b + step * 2, idesc, step % SPC ? 1u : 0u);
+                    if (step % SPC == SPC - 1) {
+                        umma_commit(acc_bar + n * 8);
+                        if (++n == C::ACC) { n = 0; nph ^= 1; }
                     }
                 }
                 if (!ok) break;
+                umma_commit(a_bar + (2 * C::A_STAGES + ab) * 8);
                 umma_commit(smem_u32(&empty[s]));
-                if (++s == C::STAGES) { s = 0; ph ^= 1; }
+                if (++ab == C::A_STAGES) { ab = 0; aph ^= 1; }
+                b += p.stage_bytes >> 4;
+                if (++s == C::STAGES) { s = 0; ph ^= 1; b -= C::STAGES * (p.stage_bytes >> 4); }
             }
         }
-    } else if (warp < 10) {
+    } else if (warp >= 4 && warp < 12) {
         // Row `row` of the weight tile, one half of each span. TMA puts 16-byte piece t of a row
         // at piece t ^ (row / 2 % 4).
-        const int q = warp & 3, row = q * 32 + lane, half = (warp - 2) >> 2;
-        int s = 0, ab = half;
+        const int q = warp & 3, row = q * 32 + lane, half = (warp - 4) >> 2;
+        const uint32_t a_bar = smem_u32(a_full + half * C::A_STAGES);
+        const uint32_t a0 = tmem_a + ((uint32_t)(q * 32) << 16) + half * C::A_STAGES * 32;
+        int s = 0, ab = 0;
         uint32_t ph = 0, aph = 0;
         for (int i = s0; i < s1; ++i) {
-            if (!mbar_wait_warp(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) break;
+            if (!mbar_wait_short(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) break;
             const uint8_t* codes = smem + s * p.stage_bytes + 2 * p.cols * 128 + row * 64 + half * 8;
             uint2 w[4];
 #pragma unroll
@@ -245,63 +249,66 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
                 unpack8(w[t].x, r + t * 4);
                 unpack8(w[t].y, r + 16 + t * 4);
             }
-            if (!mbar_wait_warp(smem_u32(&a_empty[ab]), aph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
+            if (!mbar_wait_short(a_bar + (2 * C::A_STAGES + ab) * 8, aph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
             tc_fence_after();
-            tmem_st_32x32b_x32(tmem_a + ((uint32_t)(q * 32) << 16) + ab * 32, r);
+            tmem_st_32x32b_x32(a0 + ab * 32, r);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&a_full[ab]));
-            if ((ab += 2) >= C::A_STAGES) { ab = half; aph ^= 1; }
+            if (lane == 0) mbar_arrive(a_bar + ab * 8);
+            if (++ab == C::A_STAGES) { ab = 0; aph ^= 1; }
         }
-    } else {
-        const int q = warp & 3, half = (warp - 10) >> 2;
+    } else if (warp >= 12) {
+        const int q = warp & 3, half = (warp - 12) >> 2;   // here of the rows of x
         const int64_t row = (int64_t)tile * 128 + q * 32 + lane;
         const uint16_t* sc = reinterpret_cast<const uint16_t*>(p.scales) + min(row, p.N - 1) * p.sp;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * (8 * NB);
-        float acc[8 * NB];
+        const uint32_t acc_bar = smem_u32(acc_full);
 #pragma unroll
         for (int j = 0; j < 8 * NB; ++j) acc[j] = 0.f;
-        const int g0 = s0 * CHUNKS, chunks = (s1 - s0) * CHUNKS;
-        // Scales of four groups are loaded together, while the four before them are at work: one
-        // at a time, each group would wait for a load.
-        uint16_t next[4];
-        auto load_scales = [&](int n) {
+        // The scales of a span are loaded while the one before it is at work.
+        constexpr int GROUPS = 128 / G;
+        uint16_t next[GROUPS];
+        auto load_scales = [&](int i) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) next[i] = n + i < chunks && g0 + n + i < p.groups ? __ldg(sc + g0 + n + i) : (uint16_t)0;
+            for (int k = 0; k < GROUPS; ++k) next[k] = i < s1 && i * GROUPS + k < p.groups ? __ldg(sc + i * GROUPS + k) : (uint16_t)0;
         };
-        load_scales(0);
+        load_scales(s0);
         bool ok = true;
         int n = 0;
         uint32_t nph = 0;
 #pragma unroll 1
-        for (int n0 = 0; n0 < chunks && ok; n0 += 4) {
-            float scale[4];
+        for (int i = s0; i < s1 && ok; ++i) {
+            float scale[GROUPS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) scale[i] = __uint_as_float((uint32_t)next[i] << 16);
-            load_scales(n0 + 4);
+            for (int k = 0; k < GROUPS; ++k) scale[k] = __uint_as_float((uint32_t)next[k] << 16);
+            load_scales(i + 1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (n0 + i >= chunks) break;
-                ok = mbar_wait_warp(smem_u32(&acc_full[n]), nph, abort_flag, kDevTimeoutAccFull);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t t0 = taddr + n * C::COLS;
+            for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    uint32_t h[8], m[8], l[8];
-                    tmem_ld_32x32b_x8(t0 + b * 8, h);
-                    tmem_ld_32x32b_x8(t0 + p.rows + b * 8, m);
-                    tmem_ld_32x32b_x8(t0 + 2 * p.rows + b * 8, l);
-                    tmem_ld_wait();
-                    if (b == NB - 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&acc_empty[n]));
+                for (int h = 0; h < 2; ++h) {
+                    const int at = h * C::ACC + n;
+                    const float sca = scale[(h * CHUNKS + c) * GROUPS / (2 * CHUNKS)];
+                    ok = ok && mbar_wait_short(acc_bar + at * 8, nph, abort_flag, kDevTimeoutAccFull);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t t0 = taddr + at * C::COLS;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        uint32_t hi[8], mi[8], lo[8];
+                        tmem_ld_32x32b_x8(t0 + b * 8, hi);
+                        tmem_ld_32x32b_x8(t0 + p.rows + b * 8, mi);
+                        tmem_ld_32x32b_x8(t0 + 2 * p.rows + b * 8, lo);
+                        tmem_ld_wait();
+                        if (b == NB - 1) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(acc_bar + (2 * C::ACC + at) * 8);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            acc[b * 8 + j] = fmaf(sca, __uint_as_float(hi[j]) + (__uint_as_float(mi[j]) + __uint_as_float(lo[j])), acc[b * 8 + j]);
                     }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        acc[b * 8 + j] = fmaf(scale[i], __uint_as_float(h[j]) + (__uint_as_float(m[j]) + __uint_as_float(l[j])), acc[b * 8 + j]);
                 }
                 if (++n == C::ACC) { n = 0; nph ^= 1; }
             }
