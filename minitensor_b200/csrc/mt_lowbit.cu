@@ -3,7 +3,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
-#include <cstdlib>
 
 #include "mtgemm.h"
 #include "mt_host.h"
@@ -409,31 +408,54 @@ int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias,
 
 // ------------------------------ 4 bits, batches ---------------------------------------
 
+// Sets *cluster to the number of CTAs that split k.
 template <int NB, int G>
-int launch_q4b(const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, dim3 grid, int cluster, cudaStream_t st,
-               const char* who) {
+int launch_q4b(const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, int64_t tiles, int64_t passes, int* cluster,
+               cudaStream_t st, const char* who) {
     using namespace mt::q4b;
     static std::atomic<uint64_t> smem_set{0};
+    static std::atomic<int> resident[4];   // clusters of 1, 2, 4 and 8 CTAs at once
     int dev = 0;
     cudaGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (!(smem_set.load() & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<NB, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<NB>(Cfg<NB>::COLS));
-        if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
-        smem_set.fetch_or(bit);
-    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3(8);
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem_bytes<NB>(p.cols);
+    cfg.dynamicSmemBytes = smem_bytes<NB>(Cfg<NB>::COLS);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)cluster;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(smem_set.load() & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<NB, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+        if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
+        for (int i = 0; i < 4; ++i) {
+            attr[0].val.clusterDim.x = 1u << i;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, gemm_kernel<NB, G>, &cfg) != cudaSuccess || n < 1) {
+                cudaGetLastError();
+                n = std::max(1, mt::host::sm_count() >> i);
+            }
+            resident[i].store(n);
+        }
+        smem_set.fetch_or(bit);
+    }
+    // Rounds x (spans of a CTA, and what its start and end take: about ten spans' time, two more
+    // for the cluster's sum).
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int i = 0; i < 4 && (1 << i) <= std::max(1, p.spans); ++i) {
+        const int64_t n = resident[i].load();
+        const int64_t cost = (tiles * passes + n - 1) / n * (((p.spans - 1) >> i) + 1 + 10 + (i ? 2 : 0));
+        if (cost < least) { least = cost; best = i; }
+    }
+    *cluster = 1 << best;
+    attr[0].val.clusterDim.x = 1u << best;
+    cfg.gridDim = dim3((unsigned)(tiles << best), (unsigned)passes);
+    cfg.dynamicSmemBytes = smem_bytes<NB>(p.cols);
     cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<NB, G>, tw, tx, p);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -442,12 +464,12 @@ int launch_q4b(const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMa
     return launched(who);
 }
 template <int NB>
-int launch_q4b(int group, const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, dim3 grid, int cluster,
-               cudaStream_t st, const char* who) {
+int launch_q4b(int group, const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, int64_t tiles, int64_t passes,
+               int* cluster, cudaStream_t st, const char* who) {
     switch (group) {
-        case 32: return launch_q4b<NB, 32>(p, tw, tx, grid, cluster, st, who);
-        case 64: return launch_q4b<NB, 64>(p, tw, tx, grid, cluster, st, who);
-        default: return launch_q4b<NB, 128>(p, tw, tx, grid, cluster, st, who);
+        case 32: return launch_q4b<NB, 32>(p, tw, tx, tiles, passes, cluster, st, who);
+        case 64: return launch_q4b<NB, 64>(p, tw, tx, tiles, passes, cluster, st, who);
+        default: return launch_q4b<NB, 128>(p, tw, tx, tiles, passes, cluster, st, who);
     }
 }
 
@@ -482,22 +504,12 @@ int linear_q4_batch(const View2& x, const mt::q4::Weight& w, const float* bias, 
     const uint32_t bw[2] = {64, 128}, bx[2] = {64, (uint32_t)p.cols};
     if (!mt::host::encode_u8(&tw, w.codes, dw, (uint64_t)w.cp * 4, bw) || !mt::host::encode_bf16(&tx, parts, 2, dx, sx, bx))
         return fail(MT_ECUDA, "%s: tensor map encoding failed", who);
-    // CTAs of a cluster, which split k: rounds x (spans of a CTA, and what its start and end take:
-    // about ten spans' time, two more for the cluster's sum).
-    const int nb = (int)(rows + 15) / 16;
-    const int64_t slots = mt::host::sm_count();
     int cluster = 1;
-    int64_t least = INT64_MAX;
-    for (int s = 1; s <= 8 && s <= p.spans; s *= 2) {
-        const int64_t cost = (tiles * passes * s + slots - 1) / slots * ((p.spans + s - 1) / s + 10 + (s > 1 ? 2 : 0));
-        if (cost < least) { least = cost; cluster = s; }
-    }
-    const dim3 grid((unsigned)(tiles * cluster), (unsigned)passes);
-    switch (nb) {
-        case 1: MT_TRY(launch_q4b<1>(w.group, p, tw, tx, grid, cluster, st, who)); break;
-        case 2: MT_TRY(launch_q4b<2>(w.group, p, tw, tx, grid, cluster, st, who)); break;
-        case 3: MT_TRY(launch_q4b<3>(w.group, p, tw, tx, grid, cluster, st, who)); break;
-        default: MT_TRY(launch_q4b<4>(w.group, p, tw, tx, grid, cluster, st, who)); break;
+    switch ((rows + 15) / 16) {
+        case 1: MT_TRY(launch_q4b<1>(w.group, p, tw, tx, tiles, passes, &cluster, st, who)); break;
+        case 2: MT_TRY(launch_q4b<2>(w.group, p, tw, tx, tiles, passes, &cluster, st, who)); break;
+        case 3: MT_TRY(launch_q4b<3>(w.group, p, tw, tx, tiles, passes, &cluster, st, who)); break;
+        default: MT_TRY(launch_q4b<4>(w.group, p, tw, tx, tiles, passes, &cluster, st, who)); break;
     }
     char path[96];
     snprintf(path, sizeof path, "%s batch rows=%d x %d cluster=%d", who, p.rows, (int)passes, cluster);
@@ -859,13 +871,10 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     const int64_t M = vx.rows;
     if (M * w.N == 0) return MT_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    static const char* force = getenv("MT_Q4");
-    if (force && w.K > 0) {
-        if (force[0] == 'b') return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
-        if (force[0] == 'p') return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
-        return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
-    }
-    if (M > 256 && w.K > 0) return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
+    // Few rows in integers, batches with the weights in tensor memory, prompts as a product of
+    // unpacked operands. Microseconds on weights of 4096 x 16384 (group 64), either side: 8 rows
+    // 23 and 27, 12 rows 29 and 27; 192 rows 105 and 107, 224 rows 134 and 108.
+    if (M > 192 && w.K > 0) return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
     if (M > 8 && w.K > 0) return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
     return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
 }
