@@ -371,6 +371,9 @@ def linear_backward_q8(xq: Q8Tensor, W, dY, mode=MODE_DEFAULT, stream=None):
     """``linear_backward`` with Linear's input in 8 bits: (dX, dW, db). dX = dY W^T does not
     use the input and is the float product in ``mode``."""
     _need_2d(dY, "dY")
+    if tuple(W.shape) != (xq.shape[1], dY.shape[1]):
+        raise ValueError(f"W must be [{xq.shape[1]}, {dY.shape[1]}] for a {tuple(xq.shape)} input and a {tuple(dY.shape)} "
+                         f"gradient, got {tuple(W.shape)}")
     dev = _same_device(xq, W, dY)
     with _On(dev, stream):
         dX = torch.empty((dY.shape[0], W.shape[0]), dtype=torch.float32, device=dY.device)

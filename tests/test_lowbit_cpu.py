@@ -162,6 +162,8 @@ def test_quantize_q8_refusals():
 def test_linear_q8_refusals():
     refuses("rows", mt.linear_weight_grad_q8, q8(3, 40), t(4, 5))
     refuses("2-D", mt.linear_weight_grad_q8, q8(3, 40), t(3))
+    refuses("W must be", mt.linear_backward_q8, q8(3, 40), t(41, 5), t(3, 5))
+    refuses("W must be", mt.linear_backward_q8, q8(3, 40), t(40, 6), t(3, 5))
     L = lowbit._lowbit_lib()
     q = q8(3, 40)
     dy, dw, db = t(3, 5), t(40, 5), t(5)

@@ -426,7 +426,7 @@ def test_linear_forward_q4_range_of_x(mt):
     """Blocks of x from 2^-120 to 2^125 in one call."""
     K, N = 512, 48
     g = gen(5)
-    for M in (1, 6, 20):
+    for M in (1, 6, 20, 200):
         for top in (125, 100):
             x, codes, s = q4_case(g, M, K, N, 64)
             e = torch.randint(-120, top, (M, K // 32), generator=g).repeat_interleave(32, 1)
@@ -462,7 +462,7 @@ def test_linear_forward_q4_non_finite(mt):
     codes = torch.full((N, K), 9, dtype=torch.int64)
     s = torch.ones(N, 4, dtype=torch.bfloat16)
     s[7, 2] = float("nan")
-    for M in (3, 40):
+    for M in (3, 40, 200):
         x = torch.ones(M, K)
         x[0, 5], x[1, 200] = float("nan"), float("inf")
         w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, 64)
@@ -494,3 +494,178 @@ def test_decoding_step(mt):
     n2 = mt.rms_norm(y, gamma.cuda(), residual=n.h, inplace=True)
     h, rstd, want = R.rms_norm(host(n2.h), None, gamma, 1e-6)
     assert R.worst(host(n2.y) - want, want) <= norm_bound(K) + 1
+
+
+# ---- how calls are made: graphs, streams, memory shared on purpose, far offsets ------------
+
+def calls(mt, g):
+    """name -> (inputs, call) for every operator; the call reads its inputs afresh."""
+    M, K, N = 40, 160, 132
+    x, r, dh, dy = (rand(g, M, K).cuda() for _ in range(4))
+    gamma = (1 + rand(g, K, scale=0.1)).cuda()
+    rstd = torch.rand(M, generator=g).cuda() + 0.5
+    dY = rand(g, M, N).cuda()
+    W = rand(g, K, N, scale=0.1).cuda()
+    q = mt.quantize_q8(x, "int8")
+    w = mt.quantize_q4(W, 32)
+    wide = rand(g, 300, K).cuda()
+
+    def flat(v):
+        if isinstance(v, torch.Tensor):
+            return [v]
+        if isinstance(v, mt.Q8Tensor):
+            return [v.codes.view(torch.uint8), v.scales]
+        if isinstance(v, mt.Q4Weight):
+            return [v.codes, v.scales.view(torch.int16)]
+        return [t for e in v if e is not None for t in flat(e)]
+
+    return {
+        "norm": ([x, r, gamma], lambda **k: flat(mt.rms_norm(x, gamma, residual=r, q8="e4m3", **k))),
+        "norm backward": ([dy, x, gamma, rstd, dh], lambda **k: flat(mt.rms_norm_backward(dy, x, gamma, rstd, dh=dh, **k))),
+        "quantize": ([x], lambda **k: flat(mt.quantize_q8(x, **k))),
+        "dequantize": ([q.codes], lambda **k: flat(mt.dequantize_q8(q, dtype=torch.bfloat16, **k))),
+        "weight grad": ([q.codes, dY], lambda **k: flat(mt.linear_weight_grad_q8(q, dY, **k))),
+        "forward and checkpoint": ([x, W], lambda **k: flat(mt.linear_forward_q8(x, W, **k))),
+        "backward": ([q.codes, W, dY], lambda **k: flat(mt.linear_backward_q8(q, W, dY, **k))),
+        "quantize 4": ([W], lambda **k: flat(mt.quantize_q4(W, 32, **k))),
+        "dequantize 4": ([w.codes], lambda **k: flat(mt.dequantize_q4(w, **k))),
+        "4 bits, one row": ([x], lambda **k: flat(mt.linear_forward_q4(x[:1], w, **k))),
+        "4 bits, batch": ([x], lambda **k: flat(mt.linear_forward_q4(x, w, **k))),
+        "4 bits, prompt": ([wide], lambda **k: flat(mt.linear_forward_q4(wide, w, **k))),
+    }
+
+
+NAMES = ["norm", "norm backward", "quantize", "dequantize", "weight grad", "forward and checkpoint", "backward", "quantize 4",
+         "dequantize 4", "4 bits, one row", "4 bits, batch", "4 bits, prompt"]
+
+
+def change(inputs):
+    for t in inputs:
+        if t.dtype == torch.float32:
+            t.mul_(1.5)
+        else:
+            t.copy_(t.flip(0))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_captured_call_reads_its_inputs_at_replay(mt, name):
+    inputs, call = calls(mt, gen(1))[name]
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for _ in range(2):
+        change(inputs)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("name", ["norm backward", "weight grad", "4 bits, batch", "4 bits, prompt"])
+def test_two_graphs_at_once_have_scratch_of_their_own(mt, name):
+    sides = []
+    for seed in (2, 3):
+        _, call = calls(mt, gen(seed))[name]
+        want = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = [call() for _ in range(3)]
+        sides.append((graph, out, want, torch.cuda.Stream(), call))   # call holds the graph's inputs
+    for _ in range(5):
+        for graph, _, _, stream, _ in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, out, want, _, _ in sides:
+        for o in out:
+            assert all(torch.equal(a, b) for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_stream_argument_and_repeated_calls(mt, name):
+    _, call = calls(mt, gen(4))[name]
+    want = call()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    a = call(stream=stream)
+    b = call(stream=stream.cuda_stream)
+    stream.synchronize()
+    for o in (a, b):
+        assert all(torch.equal(x, y) for x, y in zip(o, want))
+    assert mt.engine.device_status() == 0
+
+
+def test_norm_gradient_in_place_of_its_inputs(mt):
+    """dx over dy, and over dh, through the C entry; a residual without h."""
+    import ctypes
+    from minitensor_b200 import engine, lowbit
+    L = lowbit._lowbit_lib()
+    g = gen(6)
+    v, b = engine.view, ctypes.byref
+    for M, K in ((9, 260), (3, 33), (2, 40004)):
+        h, gamma, dy, dh = rand(g, M, K).cuda(), rand(g, K).cuda(), rand(g, M, K).cuda(), rand(g, M, K).cuda()
+        rstd = torch.rand(M, generator=g).cuda() + 0.5
+        want, want_g = mt.rms_norm_backward(dy, h, gamma, rstd, dh=dh)
+        for over in ("dy", "dh"):
+            a, c = dy.clone(), dh.clone()
+            dx = a if over == "dy" else c
+            dgamma = torch.empty(K, device="cuda")
+            assert L.mt_rms_norm_backward(b(v(a)), b(v(h)), b(v(gamma)), b(v(rstd)), b(v(c)), b(v(dx)), b(v(dgamma)), None) == 0
+            torch.cuda.synchronize()
+            assert torch.equal(dx, want) and torch.equal(dgamma, want_g)
+        r = rand(g, M, K).cuda()
+        y = torch.empty(M, K, device="cuda")
+        assert L.mt_rms_norm(b(v(h)), b(v(r)), b(v(gamma)), None, b(v(y)), None, None, 1e-6, None) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(y, mt.rms_norm(h, gamma, residual=r).y)
+
+
+def test_broadcast_inputs(mt):
+    g = gen(7)
+    row = rand(g, 1, 96)
+    x = row.cuda().expand(5, 96)
+    gamma = torch.tensor([1.25], device="cuda").expand(96)
+    out = mt.rms_norm(x, gamma, q8="int8")
+    h, rstd, y = R.rms_norm(row.expand(5, 96), None, torch.full((96,), 1.25), 1e-6)
+    assert R.worst(host(out.y) - y, y) <= norm_bound(96) + 1
+    q = mt.quantize_q8(x)
+    assert torch.equal(mt.dequantize_q8(q)[3], mt.dequantize_q8(mt.quantize_q8(row.cuda()))[0])
+    dY = torch.tensor([[2.0]], device="cuda").expand(5, 70)
+    check_wgrad(q, host(dY).contiguous(), *mt.linear_weight_grad_q8(q, dY))
+    W = rand(g, 96, 40)
+    w = mt.quantize_q4(W.cuda(), 32)
+    codes, s = R.q4_quantize(W, 32)
+    check_q4(mt.linear_forward_q4(x, w), row.expand(5, 96), codes, s, 32, None, False)
+
+
+def test_offsets_beyond_32_bits(mt):
+    """Rows 2^30 floats (and codes 2^31 bytes) apart."""
+    g = gen(8)
+    M, K, N = 3, 256, 64
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    base = torch.empty((M - 1) * 2 ** 30 + K, device="cuda")
+    far = base.as_strided((M, K), (2 ** 30, 1))
+    x, dY = rand(g, M, K), rand(g, M, N)
+    far.copy_(x.cuda())
+    gamma = torch.ones(K, device="cuda")
+    near = mt.rms_norm(x.cuda(), gamma, q8="int8")
+    got = mt.rms_norm(far, gamma, q8="int8")
+    assert torch.equal(got.y, near.y) and torch.equal(got.q8.codes, near.q8.codes)
+    rstd = near.rstd
+    assert torch.equal(mt.rms_norm_backward(far, far, gamma, rstd)[0], mt.rms_norm_backward(x.cuda(), x.cuda(), gamma, rstd)[0])
+    w = mt.quantize_q4(rand(g, K, N).cuda(), 64)
+    for rows in (1, 3):
+        assert torch.equal(mt.linear_forward_q4(far[3 - rows:], w), mt.linear_forward_q4(x[3 - rows:].cuda(), w))
+    q = mt.quantize_q8(far)
+    assert torch.equal(q.codes, mt.quantize_q8(x.cuda()).codes)
+    store = torch.empty((M - 1) * 2 ** 31 + K, dtype=torch.int8, device="cuda")
+    codes = store.as_strided((M, K), (2 ** 31, 1))
+    codes.copy_(q.codes)
+    far_q = mt.Q8Tensor(codes, q.scales)
+    assert torch.equal(mt.dequantize_q8(far_q), mt.dequantize_q8(q))
+    a, b = mt.linear_weight_grad_q8(far_q, dY.cuda()), mt.linear_weight_grad_q8(q, dY.cuda())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
