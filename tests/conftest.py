@@ -17,8 +17,11 @@ def pytest_collection_modifyitems(config, items):
     # Tests still waiting for their first pass on a GPU run after the established suite, so
     # that a failure among them (under -x) cannot hide the results of the others. They
     # still run and still fail the suite. The no-allocation entry point's file
-    # (test_zz_no_alloc.py) always runs last of all.
-    items.sort(key=lambda it: (os.path.basename(str(it.fspath)).startswith("test_zz_"),
+    # (test_zz_no_alloc.py) always runs last of all. The drop-in binary can only be built beside
+    # the reference checkout; where it is missing its test fails behind all others.
+    dropin = os.path.exists(os.path.join(ROOT, "minitensor_b200", "overlay", "_build", "dropin_test"))
+    items.sort(key=lambda it: (not dropin and os.path.basename(str(it.fspath)) == "test_dropin_gpu.py",
+                               os.path.basename(str(it.fspath)).startswith("test_zz_"),
                                it.get_closest_marker("first_gpu_run") is not None))
 
 
