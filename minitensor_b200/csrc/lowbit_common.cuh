@@ -90,26 +90,27 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[WPR], int& buf) {
     return warp_sum(s);
 }
 
-// VEC features of a row of unit stride.
+// VEC features of a row of unit stride that begins at `row`.
 template <int VEC>
-__device__ __forceinline__ void load_row(float (&v)[VEC], const Mat& m, int64_t row, int64_t f) {
+__device__ __forceinline__ void load_row(float (&v)[VEC], const float* row, int f) {
     if (VEC == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(m.p + row * m.rs + f);
+        const float4 x = *reinterpret_cast<const float4*>(row + f);
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
     } else {
-        v[0] = m.p[row * m.rs + f];
+        v[0] = row[f];
     }
 }
 template <int VEC>
-__device__ __forceinline__ void store_row(const float (&v)[VEC], const Mat& m, int64_t row, int64_t f) {
-    if (VEC == 4) *reinterpret_cast<float4*>(m.p + row * m.rs + f) = make_float4(v[0], v[1], v[2], v[3]);
-    else m.p[row * m.rs + f] = v[0];
+__device__ __forceinline__ void store_row(const float (&v)[VEC], float* row, int f) {
+    if (VEC == 4) *reinterpret_cast<float4*>(row + f) = make_float4(v[0], v[1], v[2], v[3]);
+    else row[f] = v[0];
 }
 
-// Quantises VEC values per lane, feature f of row `row` first; 32 / VEC lanes share a block.
-// Lanes behind the row's end pass zeros and in = false. All 32 lanes call it.
+// Quantises VEC values per lane, the first of feature f, into a row of codes and its scales;
+// 32 / VEC lanes share a block. Lanes behind the row's end pass zeros and in = false. All 32
+// lanes call it.
 template <int VEC>
-__device__ __forceinline__ void store_q8(const float (&v)[VEC], const Q8& q, int64_t row, int64_t f, bool in) {
+__device__ __forceinline__ void store_q8(const float (&v)[VEC], uint8_t* codes, uint8_t* scales, int fmt, int f, bool in) {
     uint32_t a = 0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) a = max(a, abs_bits(v[i]));
@@ -119,19 +120,23 @@ __device__ __forceinline__ void store_q8(const float (&v)[VEC], const Q8& q, int
 #pragma unroll
         for (int o = 16 / VEC; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
     }
-    const uint32_t b = scale_byte(a, q.fmt);
+    const uint32_t b = scale_byte(a, fmt);
     const float inv = inv_scale(b);
     if (!in) return;
-    uint8_t* c = q.codes + row * q.cp + f;
     if (VEC == 4) {
         uint32_t w = 0;
+        if (fmt == kInt8) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) w |= encode8(v[i], inv, q.fmt) << (8 * i);
-        *reinterpret_cast<uint32_t*>(c) = w;
+            for (int i = 0; i < VEC; ++i) w |= encode8(v[i], inv, kInt8) << (8 * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) w |= encode8(v[i], inv, kE4M3) << (8 * i);
+        }
+        *reinterpret_cast<uint32_t*>(codes + f) = w;
     } else {
-        *c = (uint8_t)encode8(v[0], inv, q.fmt);
+        codes[f] = (uint8_t)(fmt == kInt8 ? encode8(v[0], inv, kInt8) : encode8(v[0], inv, kE4M3));
     }
-    if (f % kBlock == 0) q.scales[row * q.sp + f / kBlock] = (uint8_t)b;
+    if ((f & (kBlock - 1)) == 0) scales[(uint32_t)f / kBlock] = (uint8_t)b;
 }
 
 }  // namespace lowbit

@@ -21,7 +21,7 @@ using mt::host::launched;
 using mt::lowbit::Mat;
 using mt::lowbit::Q8;
 
-constexpr int64_t kMaxExtent = INT32_MAX;   // rows or features of one operand
+constexpr int64_t kMaxExtent = INT32_MAX - 4096;   // rows or features of one operand
 
 // A checked 2-D view; is1d: a vector, as one row.
 struct View2 {
@@ -34,7 +34,7 @@ int to_mat(const mt_tensor* t, const char* who, const char* name, View2& v) {
     if (!t) return fail(MT_EINVAL, "%s: %s is null", who, name);
     if (t->ndim != 2) return fail(MT_EINVAL, "%s: %s must be 2-D, got %u-D", who, name, t->ndim);
     if (t->shape[0] > (uint64_t)kMaxExtent || t->shape[1] > (uint64_t)kMaxExtent)
-        return fail(MT_EUNSUPPORTED, "%s: %s has an extent beyond 2^31", who, name);
+        return fail(MT_EUNSUPPORTED, "%s: %s has an extent beyond 2^31 - 4097", who, name);
     v.rows = (int64_t)t->shape[0];
     v.cols = (int64_t)t->shape[1];
     if (v.rows * v.cols > 0 && !t->data) return fail(MT_EINVAL, "%s: %s has a null data pointer", who, name);
@@ -121,7 +121,7 @@ int to_q8(const mt_q8* q, const char* who, Q8& o, int64_t& rows, int64_t& cols) 
     if (!q) return fail(MT_EINVAL, "%s: the 8-bit tensor is null", who);
     if (q->format != MT_Q8_INT8 && q->format != MT_Q8_E4M3) return fail(MT_EINVAL, "%s: bad 8-bit format %d", who, q->format);
     if (q->rows > (uint64_t)kMaxExtent || q->cols > (uint64_t)kMaxExtent)
-        return fail(MT_EUNSUPPORTED, "%s: the 8-bit tensor has an extent beyond 2^31", who);
+        return fail(MT_EUNSUPPORTED, "%s: the 8-bit tensor has an extent beyond 2^31 - 4097", who);
     rows = (int64_t)q->rows;
     cols = (int64_t)q->cols;
     if (rows * cols > 0 && (!q->codes || !q->scales)) return fail(MT_EINVAL, "%s: the 8-bit tensor has a null pointer", who);
@@ -139,8 +139,8 @@ int to_q4(const mt_q4* q, const char* who, mt::q4::Weight& o) {
     if (!q) return fail(MT_EINVAL, "%s: the 4-bit weight is null", who);
     if (q->group != 32 && q->group != 64 && q->group != 128)
         return fail(MT_EINVAL, "%s: group must be 32, 64 or 128, got %llu", who, (unsigned long long)q->group);
-    if (q->in > (uint64_t)kMaxExtent - 127 || q->out > (uint64_t)kMaxExtent)
-        return fail(MT_EUNSUPPORTED, "%s: the 4-bit weight has an extent beyond 2^31", who);
+    if (q->in > (uint64_t)kMaxExtent || q->out > (uint64_t)kMaxExtent)
+        return fail(MT_EUNSUPPORTED, "%s: the 4-bit weight has an extent beyond 2^31 - 4097", who);
     const uint64_t spans = (q->in + 127) / 128, groups = (q->in + q->group - 1) / q->group;
     if (q->in * q->out > 0) {
         if (!q->codes || !q->scales) return fail(MT_EINVAL, "%s: the 4-bit weight has a null pointer", who);

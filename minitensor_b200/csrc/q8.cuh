@@ -18,15 +18,16 @@ constexpr int kDequantWidth = 8 * 256;   // features per CTA of the scalar dequa
 template <int VEC>
 __global__ void __launch_bounds__(32 * kWarps) quantize_kernel(Mat x, Q8 q, int64_t rows, int64_t K) {
     const int lane = threadIdx.x & 31;
-    const int64_t f = (((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * 32 + lane) * VEC;
-    if (f - lane * VEC >= K) return;   // the whole warp
+    const int64_t first = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * 32 * VEC;
+    if (first >= K) return;   // the whole warp
+    const int f = (int)first + lane * VEC;
     const bool in = f < K;
     for (int64_t r0 = (int64_t)blockIdx.y * kRows; r0 < rows; r0 += (int64_t)gridDim.y * kRows) {
         float v[kRows][VEC];
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
             if (in && r0 + j < rows) {
-                if (VEC == 4) lowbit::load_row<VEC>(v[j], x, r0 + j, f);
+                if (VEC == 4) lowbit::load_row<VEC>(v[j], x.p + (r0 + j) * x.rs, f);
                 else v[j][0] = x.p[(r0 + j) * x.rs + f * x.cs];
             } else {
 #pragma unroll
@@ -35,7 +36,7 @@ __global__ void __launch_bounds__(32 * kWarps) quantize_kernel(Mat x, Q8 q, int6
         }
 #pragma unroll
         for (int j = 0; j < kRows; ++j)
-            if (r0 + j < rows) lowbit::store_q8<VEC>(v[j], q, r0 + j, f, in);
+            if (r0 + j < rows) lowbit::store_q8<VEC>(v[j], q.codes + (r0 + j) * q.cp, q.scales + (r0 + j) * q.sp, q.fmt, f, in);
     }
 }
 
@@ -62,17 +63,27 @@ __global__ void __launch_bounds__(256) dequantize_kernel(Q8 q, T* out, int64_t p
         }
     } else {
         const int64_t f0 = (int64_t)blockIdx.x * kDequantWidth + threadIdx.x;
+        const int left = (int)min(K - f0, (int64_t)kDequantWidth);   // columns from this thread's first on
         for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+            const uint8_t* cr = q.codes + row * q.cp + f0;
+            const uint8_t* sr = q.scales + row * q.sp + f0 / lowbit::kBlock;
+            T* o = out + row * pitch + f0;
             uint8_t c[8], b[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int64_t f = f0 + i * 256;
-                c[i] = f < K ? q.codes[row * q.cp + f] : 0;
-                b[i] = f < K ? q.scales[row * q.sp + f / lowbit::kBlock] : 0;
+                const bool in = i * 256 < left;
+                c[i] = in ? cr[i * 256] : 0;
+                b[i] = in ? sr[i * 256 / lowbit::kBlock] : 0;
             }
+            if (q.fmt == lowbit::kInt8) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (f0 + i * 256 < K) put(out + row * pitch + f0 + i * 256, lowbit::code_value(c[i], q.fmt) * lowbit::scale_value(b[i]));
+                for (int i = 0; i < 8; ++i)
+                    if (i * 256 < left) put(o + i * 256, lowbit::code_value(c[i], lowbit::kInt8) * lowbit::scale_value(b[i]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i * 256 < left) put(o + i * 256, lowbit::code_value(c[i], lowbit::kE4M3) * lowbit::scale_value(b[i]));
+            }
         }
     }
 }

@@ -53,9 +53,9 @@ __global__ void __launch_bounds__(32 * WPR * RPC, fwd_ctas(VEC * V, 32 * WPR * R
         float ss = 0.f;
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
+            const int f = ((c * WPR + w) * 32 + lane) * VEC;
             if (f < p.K) {
-                lowbit::load_row<VEC>(v[c], p.x, row, f);
+                lowbit::load_row<VEC>(v[c], p.x.p + row * p.x.rs, f);
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) v[c][i] = 0.f;
@@ -65,23 +65,23 @@ __global__ void __launch_bounds__(32 * WPR * RPC, fwd_ctas(VEC * V, 32 * WPR * R
             float r[V][VEC];
 #pragma unroll
             for (int c = 0; c < V; ++c) {
-                const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
-                if (f < p.K) lowbit::load_row<VEC>(r[c], p.r, row, f);
+                const int f = ((c * WPR + w) * 32 + lane) * VEC;
+                if (f < p.K) lowbit::load_row<VEC>(r[c], p.r.p + row * p.r.rs, f);
             }
 #pragma unroll
             for (int c = 0; c < V; ++c) {
-                const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
+                const int f = ((c * WPR + w) * 32 + lane) * VEC;
                 if (f < p.K) {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) v[c][i] += r[c][i];
-                    if (p.h.p) lowbit::store_row<VEC>(v[c], p.h, row, f);
+                    if (p.h.p) lowbit::store_row<VEC>(v[c], p.h.p + row * p.h.rs, f);
                 }
             }
         } else if (p.h.p) {
 #pragma unroll
             for (int c = 0; c < V; ++c) {
-                const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
-                if (f < p.K) lowbit::store_row<VEC>(v[c], p.h, row, f);
+                const int f = ((c * WPR + w) * 32 + lane) * VEC;
+                if (f < p.K) lowbit::store_row<VEC>(v[c], p.h.p + row * p.h.rs, f);
             }
         }
 #pragma unroll
@@ -93,17 +93,17 @@ __global__ void __launch_bounds__(32 * WPR * RPC, fwd_ctas(VEC * V, 32 * WPR * R
         if (p.rstd.p && lane == 0 && w == 0) p.rstd.p[row * p.rstd.cs] = rstd;
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
+            const int f = ((c * WPR + w) * 32 + lane) * VEC;
             const bool in = f < p.K;
             if (f - lane * VEC >= p.K) break;   // the whole warp
             if (in) {
                 float g[VEC];
-                lowbit::load_row<VEC>(g, p.gamma, 0, f);
+                lowbit::load_row<VEC>(g, p.gamma.p, f);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * rstd * g[i];
-                if (p.y.p) lowbit::store_row<VEC>(v[c], p.y, row, f);
+                if (p.y.p) lowbit::store_row<VEC>(v[c], p.y.p + row * p.y.rs, f);
             }
-            if (p.q.codes) lowbit::store_q8<VEC>(v[c], p.q, row, f, in);
+            if (p.q.codes) lowbit::store_q8<VEC>(v[c], p.q.codes + row * p.q.cp, p.q.scales + row * p.q.sp, p.q.fmt, f, in);
         }
     }
 }
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(32 * kLongWarps) fwd_long_kernel(const Fwd p) 
                 v[0] = v[0] * rstd * p.gamma.p[f * p.gamma.cs];
                 if (p.y.p) p.y.p[row * p.y.rs + f * p.y.cs] = v[0];
             }
-            if (p.q.codes) lowbit::store_q8<1>(v, p.q, row, f, in);
+            if (p.q.codes) lowbit::store_q8<1>(v, p.q.codes + row * p.q.cp, p.q.scales + row * p.q.sp, p.q.fmt, (int)f, in);
         }
     }
 }
@@ -163,23 +163,23 @@ __global__ void __launch_bounds__(32 * WPR * RPC) bwd_kernel(const Bwd p) {
         float dy[V][VEC], xh[V][VEC], dh[V][VEC];
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
+            const int f = ((c * WPR + w) * 32 + lane) * VEC;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) dy[c][i] = xh[c][i] = dh[c][i] = 0.f;
             if (f < p.K) {
-                lowbit::load_row<VEC>(dy[c], p.dy, row, f);
-                lowbit::load_row<VEC>(xh[c], p.h, row, f);
-                if (p.dh.p) lowbit::load_row<VEC>(dh[c], p.dh, row, f);
+                lowbit::load_row<VEC>(dy[c], p.dy.p + row * p.dy.rs, f);
+                lowbit::load_row<VEC>(xh[c], p.h.p + row * p.h.rs, f);
+                if (p.dh.p) lowbit::load_row<VEC>(dh[c], p.dh.p + row * p.dh.rs, f);
             }
         }
         const float rstd = p.rstd.p[row * p.rstd.cs];
         float dot = 0.f;
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
+            const int f = ((c * WPR + w) * 32 + lane) * VEC;
             if (f < p.K) {
                 float g[VEC];
-                lowbit::load_row<VEC>(g, p.gamma, 0, f);
+                lowbit::load_row<VEC>(g, p.gamma.p, f);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     xh[c][i] *= rstd;
@@ -192,19 +192,19 @@ __global__ void __launch_bounds__(32 * WPR * RPC) bwd_kernel(const Bwd p) {
         dot = lowbit::row_sum<WPR>(dot, red, buf) / (float)p.K;
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
+            const int f = ((c * WPR + w) * 32 + lane) * VEC;
             if (f < p.K) {
                 float d[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) d[i] = fmaf(rstd, fmaf(-xh[c][i], dot, dy[c][i]), dh[c][i]);
-                lowbit::store_row<VEC>(d, p.dx, row, f);
+                lowbit::store_row<VEC>(d, p.dx.p + row * p.dx.rs, f);
             }
         }
     }
     if (p.part) {
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            const int64_t f = ((int64_t)(c * WPR + w) * 32 + lane) * VEC;
+            const int f = ((c * WPR + w) * 32 + lane) * VEC;
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
                 if (f + i < p.K) p.part[group * p.K + f + i] = dg[c][i];
