@@ -233,6 +233,12 @@ __device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint64_t adesc, uint6
         : "memory");
 }
 
+// Programmatic dependent launch: a kernel launched with that attribute begins while the one before
+// it on the stream still runs; what it reads of that one's results comes behind pdl_wait.
+// pdl_start lets the dependent kernel begin once every CTA has called it.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // True in one lane of a converged warp. Operands of tcgen05.mma live in uniform registers: in a
 // branch on elect.sync, with addresses that all lanes share (__shfl_sync for what comes from
 // shared memory) and an unrolled loop, an MMA issues in about 10 cycles; in a branch on the

@@ -294,6 +294,32 @@ void pick_splits(mt::planes::Params& p, int64_t tiles, int64_t chunk_blocks, int
     }
 }
 
+// Launches a kernel that calls pdl_wait before it reads what the kernel before it wrote.
+template <typename... Args>
+int launch_after(void (*kern)(Args...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, const char* who,
+                 const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;   // 0: the kernel's own cluster shape
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return mt::host::cuda_fail(e, who);
+    }
+    return launched(who);
+}
+
 // D = A * B^T over `kpitch` padded values of k: a [R][kpitch], b [3][C][kpitch], both bfloat16.
 // p carries the output, the scales (SCALED) and the bias.
 template <bool SCALED, int SPC>
@@ -329,12 +355,8 @@ int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16
         smem_set.fetch_or(bit);
     }
     const unsigned grid = 2 * (unsigned)std::min<int64_t>(p.units, clusters);
-    gemm_kernel<SCALED, SPC><<<grid, THREADS, SMEM_BYTES, st>>>(ta, tb, p);
-    MT_TRY(launched(who));
-    if (in_parts) {
-        join_kernel<<<dim3((unsigned)in_parts, BM / 8), 256, 0, st>>>(p);
-        MT_TRY(launched(who));
-    }
+    MT_TRY(launch_after(gemm_kernel<SCALED, SPC>, dim3(grid), dim3(THREADS), SMEM_BYTES, 0, st, who, ta, tb, p));
+    if (in_parts) MT_TRY(launch_after(join_kernel, dim3((unsigned)in_parts, BM / 8), dim3(256), 0, 0, st, who, p));
     char path[96];
     snprintf(path, sizeof path, "%s planes whole=%d splits=%d", who, p.whole, p.splits);
     mt::host::set_path(path);
@@ -453,15 +475,8 @@ int launch_q4b(const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMa
         if (cost < least) { least = cost; best = i; }
     }
     *cluster = 1 << best;
-    attr[0].val.clusterDim.x = 1u << best;
-    cfg.gridDim = dim3((unsigned)(tiles << best), (unsigned)passes);
-    cfg.dynamicSmemBytes = smem_bytes<NB>(p.cols);
-    cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<NB, G>, tw, tx, p);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return mt::host::cuda_fail(e, who);
-    }
-    return launched(who);
+    return launch_after(gemm_kernel<NB, G>, dim3((unsigned)(tiles << best), (unsigned)passes), dim3(THREADS), smem_bytes<NB>(p.cols),
+                        *cluster, st, who, tw, tx, p);
 }
 template <int NB>
 int launch_q4b(int group, const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, int64_t tiles, int64_t passes,

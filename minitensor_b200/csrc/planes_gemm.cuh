@@ -156,8 +156,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     int rb, cb, sp, kb0, kb1;
+    pdl_start();   // the kernel that joins split tiles
     if (warp == 0) {
         if (lane == 0) {
+            pdl_wait();
             int s = 0;
             uint32_t ph = 0;
             for (int u = first; u < p.units; u += step) {
@@ -229,6 +231,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         const uint32_t empty_bar[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
         int n = 0;
         if (!SCALED && p.db_tiles > 0) {
+            pdl_wait();
             // The bias gradient, while the first tiles load.
             for (int64_t c = (int64_t)blockIdx.x * (32 * EPI_WARPS) + (int)threadIdx.x - 64; c < p.C; c += (int64_t)gridDim.x * (32 * EPI_WARPS)) {
                 float s = 0.f;
@@ -347,6 +350,7 @@ done:
 // has one column (or row, where rows are neighbours in D) of 8 rows (columns).
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
     const int t = blockIdx.x;
+    pdl_wait();
     int rb, cb;
     tile_of(p, p.whole + t, rb, cb);
     const bool along_r = p.os_r == 1;
@@ -527,12 +531,14 @@ __global__ void __launch_bounds__(256) prepare_q8_kernel(lowbit::Q8 q, __nv_bflo
         struct { float s[64][65], cs[4][64]; } rows;
         uint16_t codes[64][66];
     } sm;
+    pdl_start();
     if ((int)blockIdx.x < blocks_b) split_rows(dy, b, M, N, pitch, col_sums, blockIdx.x, sm.rows.s, sm.rows.cs);
     else expand_q8<VEC>(q, a, M, K, pitch, blockIdx.x - blocks_b, sm.codes);
 }
 // Both operands of the 4-bit product in one launch: blocks [0, blocks_b) of x do x.
 __global__ void __launch_bounds__(256) prepare_q4_kernel(q4::Weight q, __nv_bfloat16* a, Mat x, bool vec, __nv_bfloat16* b, int64_t M,
                                                          int64_t pitch, int blocks_b) {
+    pdl_start();
     if ((int)blockIdx.x < blocks_b) split_cols(x, vec, b, M, q.K, pitch, blockIdx.x, M);
     else expand_q4(q, a, pitch, blockIdx.x - blocks_b);
 }

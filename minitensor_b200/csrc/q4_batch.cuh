@@ -180,13 +180,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     float acc[8 * NB];   // of the draining warps
     if (warp == 0) {
         if (lane == 0) {
+            // The codes of the first spans are on their way before x is split.
+            auto load_codes = [&](int i, int s) {
+                mbar_arrive_expect_tx(smem_u32(&full[s]), p.stage_bytes);
+                tma_load_2d(smem_u32(smem + s * p.stage_bytes) + 2 * p.cols * 128, &tmW, smem_u32(&full[s]), i * 64, tile * 128);
+            };
+            for (int i = s0; i < min(s1, s0 + C::STAGES); ++i) load_codes(i, i - s0);
+            pdl_wait();
             int s = 0;
             uint32_t ph = 0;
             for (int i = s0; i < s1; ++i) {
-                if (!mbar_wait_short(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
+                if (i >= s0 + C::STAGES) {
+                    if (!mbar_wait_short(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
+                    load_codes(i, s);
+                }
                 const uint32_t to = smem_u32(smem + s * p.stage_bytes), bar = smem_u32(&full[s]);
-                mbar_arrive_expect_tx(bar, p.stage_bytes);
-                tma_load_2d(to + 2 * p.cols * 128, &tmW, bar, i * 64, tile * 128);
                 tma_load_2d(to, &tmX, bar, i * 128, (int)blockIdx.y * 3 * p.rows);
                 tma_load_2d(to + p.cols * 128, &tmX, bar, i * 128 + 64, (int)blockIdx.y * 3 * p.rows);
                 if (++s == C::STAGES) { s = 0; ph ^= 1; }
@@ -359,6 +367,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
 
 // The parts of x for q4b::gemm_kernel: out[pass][part][row of the pass][k].
 __global__ void __launch_bounds__(256) split_passes_kernel(Mat x, bool vec, __nv_bfloat16* out, int64_t M, int64_t K, int64_t pitch, int rows) {
+    pdl_start();
     const int64_t m0 = (int64_t)blockIdx.z * rows;
     const Mat part{x.p + m0 * x.rs, x.rs, x.cs};
     planes::split_cols(part, vec, out + (int64_t)blockIdx.z * 3 * rows * pitch, min((int64_t)rows, M - m0), K, pitch, blockIdx.x, rows);
