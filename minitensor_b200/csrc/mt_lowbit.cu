@@ -296,22 +296,17 @@ void pick_splits(mt::planes::Params& p, int64_t tiles, int64_t chunk_blocks, int
 
 // Launches a kernel that calls pdl_wait before it reads what the kernel before it wrote.
 template <typename... Args>
-int launch_after(void (*kern)(Args...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, const char* who,
-                 const Args&... args) {
+int launch_after(void (*kern)(Args...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const char* who, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = cluster > 0 ? 2 : 1;   // 0: the kernel's own cluster shape
+    cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -355,8 +350,8 @@ int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16
         smem_set.fetch_or(bit);
     }
     const unsigned grid = 2 * (unsigned)std::min<int64_t>(p.units, clusters);
-    MT_TRY(launch_after(gemm_kernel<SCALED, SPC>, dim3(grid), dim3(THREADS), SMEM_BYTES, 0, st, who, ta, tb, p));
-    if (in_parts) MT_TRY(launch_after(join_kernel, dim3((unsigned)in_parts, BM / 8), dim3(256), 0, 0, st, who, p));
+    MT_TRY(launch_after(gemm_kernel<SCALED, SPC>, dim3(grid), dim3(THREADS), SMEM_BYTES, st, who, ta, tb, p));
+    if (in_parts) MT_TRY(launch_after(join_kernel, dim3((unsigned)in_parts, BM / 8), dim3(256), 0, st, who, p));
     char path[96];
     snprintf(path, sizeof path, "%s planes whole=%d splits=%d", who, p.whole, p.splits);
     mt::host::set_path(path);
@@ -430,61 +425,27 @@ int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias,
 
 // ------------------------------ 4 bits, batches ---------------------------------------
 
-// Sets *cluster to the number of CTAs that split k.
 template <int NB, int G>
-int launch_q4b(const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, int64_t tiles, int64_t passes, int* cluster,
-               cudaStream_t st, const char* who) {
+int launch_q4b(const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, int64_t ctas, cudaStream_t st, const char* who) {
     using namespace mt::q4b;
     static std::atomic<uint64_t> smem_set{0};
-    static std::atomic<int> resident[4];   // clusters of 1, 2, 4 and 8 CTAs at once
     int dev = 0;
     cudaGetDevice(&dev);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(8);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem_bytes<NB>(Cfg<NB>::COLS);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     const uint64_t bit = 1ull << (dev & 63);
     if (!(smem_set.load() & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<NB, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<NB, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<NB>(Cfg<NB>::COLS));
         if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
-        for (int i = 0; i < 4; ++i) {
-            attr[0].val.clusterDim.x = 1u << i;
-            int n = 0;
-            if (cudaOccupancyMaxActiveClusters(&n, gemm_kernel<NB, G>, &cfg) != cudaSuccess || n < 1) {
-                cudaGetLastError();
-                n = std::max(1, mt::host::sm_count() >> i);
-            }
-            resident[i].store(n);
-        }
         smem_set.fetch_or(bit);
     }
-    // Rounds x (spans of a CTA, and what its start and end take: about ten spans' time, two more
-    // for the cluster's sum).
-    int best = 0;
-    int64_t least = INT64_MAX;
-    for (int i = 0; i < 4 && (1 << i) <= std::max(1, p.spans); ++i) {
-        const int64_t n = resident[i].load();
-        const int64_t cost = (tiles * passes + n - 1) / n * (((p.spans - 1) >> i) + 1 + 10 + (i ? 2 : 0));
-        if (cost < least) { least = cost; best = i; }
-    }
-    *cluster = 1 << best;
-    return launch_after(gemm_kernel<NB, G>, dim3((unsigned)(tiles << best), (unsigned)passes), dim3(THREADS), smem_bytes<NB>(p.cols),
-                        *cluster, st, who, tw, tx, p);
+    return launch_after(gemm_kernel<NB, G>, dim3((unsigned)ctas), dim3(THREADS), smem_bytes<NB>(p.cols), st, who, tw, tx, p);
 }
 template <int NB>
-int launch_q4b(int group, const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, int64_t tiles, int64_t passes,
-               int* cluster, cudaStream_t st, const char* who) {
+int launch_q4b(int group, const mt::q4b::Params& p, const CUtensorMap& tw, const CUtensorMap& tx, int64_t ctas, cudaStream_t st,
+               const char* who) {
     switch (group) {
-        case 32: return launch_q4b<NB, 32>(p, tw, tx, tiles, passes, cluster, st, who);
-        case 64: return launch_q4b<NB, 64>(p, tw, tx, tiles, passes, cluster, st, who);
-        default: return launch_q4b<NB, 128>(p, tw, tx, tiles, passes, cluster, st, who);
+        case 32: return launch_q4b<NB, 32>(p, tw, tx, ctas, st, who);
+        case 64: return launch_q4b<NB, 64>(p, tw, tx, ctas, st, who);
+        default: return launch_q4b<NB, 128>(p, tw, tx, ctas, st, who);
     }
 }
 
@@ -493,9 +454,25 @@ int linear_q4_batch(const View2& x, const mt::q4::Weight& w, const float* bias, 
     using namespace mt::q4b;
     const int64_t passes = (M + kRows - 1) / kRows, rows = (M + passes - 1) / passes;
     const int64_t pitch = round_up(w.K, mt::q4::kSpan), tiles = (w.N + 127) / 128;
-    if (passes > 65535 || tiles > INT32_MAX / 16) return fail(MT_EUNSUPPORTED, "%s: too many tiles", who);
+    const int64_t all = passes * tiles * (pitch / mt::q4::kSpan);   // spans of all tiles
+    if (passes > 65535 || all > INT32_MAX / 2) return fail(MT_EUNSUPPORTED, "%s: too many tiles", who);
+    // Runs: either one per SM, or tiles in s equal parts, which walk along k side by side and share
+    // the parts of x in L2 while they are hot. By spans: a run's start and end take about ten, the
+    // join of cut tiles three; runs at different places of k take longer, the more rows of x the
+    // longer. 64 rows on 4096 x 16384: 148 runs 53 us, 128 whole tiles 39 us; 128 rows on
+    // 4001 x 11003: 148 runs 91 us, 172 whole tiles 108 us.
+    const int64_t sms = mt::host::sm_count(), spans = pitch / mt::q4::kSpan, nb = (rows + 15) / 16;
+    int64_t ctas = std::max<int64_t>(1, std::min(sms, all / 2));
+    double least = (double)((all + ctas - 1) / ctas) * (nb == 1 ? 1. : nb == 2 ? 1.2 : 1.5) + 13.;
+    for (int64_t s = 1; s <= 8 && spans % s == 0; s *= 2) {
+        const double cost = (double)((passes * tiles * s + sms - 1) / sms) * (double)(spans / s + 10) + (s > 1 ? 3. : 0.);
+        if (cost < least) { least = cost; ctas = passes * tiles * s; }
+    }
+    const bool cut = (all / ctas) % spans || all % ctas;
+    const size_t x_bytes = round_up(passes * 3 * rows * pitch * 2, 256);
+    const size_t part_bytes = cut ? (size_t)ctas * 2 * rows * 128 * sizeof(float) : 0;
     Scratch ws(st);
-    MT_TRY(ws.take((size_t)passes * 3 * rows * pitch * 2, who));
+    MT_TRY(ws.take(x_bytes + part_bytes, who));
     __nv_bfloat16* parts = static_cast<__nv_bfloat16*>(ws.p);
     split_passes_kernel<<<dim3((unsigned)((pitch / 4 + 255) / 256), (unsigned)rows, (unsigned)passes), 256, 0, st>>>(
         x.m, vec4(x), parts, M, w.K, pitch, (int)rows);
@@ -513,21 +490,26 @@ int linear_q4_batch(const View2& x, const mt::q4::Weight& w, const float* bias, 
     p.y = y;
     p.relu = relu;
     p.stage_bytes = stage_bytes(p.cols);
+    p.tiles = (int)tiles;
+    p.each = (int)(all / ctas);
+    p.more = (int)(all % ctas);
+    p.part = cut ? reinterpret_cast<float*>(static_cast<char*>(ws.p) + x_bytes) : nullptr;
     CUtensorMap tw, tx;
     const uint64_t dw[2] = {(uint64_t)p.spans * 64, (uint64_t)w.N}, dx[2] = {(uint64_t)pitch, (uint64_t)(passes * 3 * rows)};
     const uint64_t sx[1] = {(uint64_t)pitch * 2};
     const uint32_t bw[2] = {64, 128}, bx[2] = {64, (uint32_t)p.cols};
     if (!mt::host::encode_u8(&tw, w.codes, dw, (uint64_t)w.cp * 4, bw) || !mt::host::encode_bf16(&tx, parts, 2, dx, sx, bx))
         return fail(MT_ECUDA, "%s: tensor map encoding failed", who);
-    int cluster = 1;
-    switch ((rows + 15) / 16) {
-        case 1: MT_TRY(launch_q4b<1>(w.group, p, tw, tx, tiles, passes, &cluster, st, who)); break;
-        case 2: MT_TRY(launch_q4b<2>(w.group, p, tw, tx, tiles, passes, &cluster, st, who)); break;
-        case 3: MT_TRY(launch_q4b<3>(w.group, p, tw, tx, tiles, passes, &cluster, st, who)); break;
-        default: MT_TRY(launch_q4b<4>(w.group, p, tw, tx, tiles, passes, &cluster, st, who)); break;
+    switch (nb) {
+        case 1: MT_TRY(launch_q4b<1>(w.group, p, tw, tx, ctas, st, who)); break;
+        case 2: MT_TRY(launch_q4b<2>(w.group, p, tw, tx, ctas, st, who)); break;
+        case 3: MT_TRY(launch_q4b<3>(w.group, p, tw, tx, ctas, st, who)); break;
+        default: MT_TRY(launch_q4b<4>(w.group, p, tw, tx, ctas, st, who)); break;
     }
+    if (cut)
+        MT_TRY(launch_after(join_kernel, dim3((unsigned)(passes * tiles), (unsigned)(rows + 1) / 2), dim3(256), 0, st, who, p));
     char path[96];
-    snprintf(path, sizeof path, "%s batch rows=%d x %d cluster=%d", who, p.rows, (int)passes, cluster);
+    snprintf(path, sizeof path, "%s batch rows=%d x %d ctas=%d", who, p.rows, (int)passes, (int)ctas);
     mt::host::set_path(path);
     return MT_OK;
 }

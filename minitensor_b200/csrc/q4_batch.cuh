@@ -13,14 +13,15 @@
 // registers (11 instructions per 8 weights) and stores them to tensor memory, from where the
 // MMA takes them; shared memory carries only the packed codes and the parts of x.
 //
-// Work. A CTA has 128 weight rows and a range of spans of 128 k; the CTAs of a cluster share
-// the rows and split k, and add their sums through distributed shared memory in order. Warp 0
-// loads by TMA (codes and x parts of a span per stage). The two 64-deep halves of a span go
+// Work. The spans of 128 k of all tiles of 128 weight rows, taken tile after tile, are cut into
+// one run per CTA, so that all SMs end together; a tile inside one run is written at once, the
+// parts of a cut one go to scratch and a second kernel adds them in order. Warp 0 loads by
+// TMA (codes and x parts of a span per stage). The two 64-deep halves of a span go
 // their own ways: warps 1 and 2 issue their MMAs, warps 4-7 and 8-11 unpack (lane quarter =
 // warp & 3), each with its own accumulators and unpacked steps in tensor memory. Warps 12-19
 // drain the accumulators, half of the rows of x each. What bounds a step is the roles'
 // instructions and hand-overs (a half is 182 cycles of memory, an MMA 24 cycles at 16 rows of
-// x), hence two issuers and waits in few instructions. blockIdx.y takes up to 64 rows of x each.
+// x), hence two issuers and waits in few instructions. Up to 64 rows of x at a time ("pass").
 #pragma once
 
 #include "planes_gemm.cuh"
@@ -30,7 +31,7 @@ namespace q4b {
 
 using lowbit::Mat;
 
-constexpr int kRows = 64;                 // rows of x per blockIdx.y, at most
+constexpr int kRows = 64;                 // rows of x of a pass, at most
 constexpr int THREADS = 32 * 20;
 constexpr int EPI_WARPS = 8;
 constexpr uint32_t CODE_BYTES = 128 * 64; // a span of 128 weight rows
@@ -49,9 +50,12 @@ struct Cfg {
 struct Params {
     int64_t N;                   // weight rows (outputs)
     int64_t M;
-    int rows;                    // of x per blockIdx.y
+    int rows;                    // of x per pass
     int cols;                    // MMA tile width: 3 rows, rounded up to 16
     int spans, groups;
+    int tiles;                   // of weight rows; tile t of pass s is number s * tiles + t
+    int each, more;              // spans of a CTA's run, and how many CTAs have one more
+    float* part;                 // [CTA][first or last tile of its run][row of x][128]
     const __nv_bfloat16* scales;
     int64_t sp;
     const float* bias;
@@ -99,16 +103,8 @@ __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[
                  : "r"(taddr)
                  : "memory");
 }
-__device__ __forceinline__ uint32_t cluster_nctarank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ float ld_cluster(uint32_t a) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-}
+// The first span of CTA c's run, counted over all tiles.
+__host__ __device__ __forceinline__ int run_begin(const Params& p, int c) { return c * p.each + (c < p.more ? c : p.more); }
 
 // (c - 8) / kCodeUnit of a word's 8 codes, in order, as four pairs: 128 + c is a bfloat16 with c
 // in its low bits, and one multiply-add takes 128 + 8 off and scales, exactly.
@@ -142,9 +138,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_empty + 2 * C::ACC) + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = (int)cluster_ctarank(), ranks = (int)cluster_nctarank();
-    const int tile = (int)blockIdx.x / ranks;
-    const int s0 = (int)((int64_t)p.spans * rank / ranks), s1 = (int)((int64_t)p.spans * (rank + 1) / ranks);
+    const int begin = run_begin(p, blockIdx.x), count = run_begin(p, blockIdx.x + 1) - begin;
+    const int t_first = begin / p.spans, s_first = begin - t_first * p.spans;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -173,30 +168,41 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_start();   // the kernel that joins cut tiles
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const uint32_t tmem_a = tmem_base + 2 * C::ACC * C::COLS;
-    float* red = reinterpret_cast<float*>(smem);          // [rows of x][128], once the ring is idle
 
     float acc[8 * NB];   // of the draining warps
     if (warp == 0) {
         if (lane == 0) {
             // The codes of the first spans are on their way before x is split.
-            auto load_codes = [&](int i, int s) {
-                mbar_arrive_expect_tx(smem_u32(&full[s]), p.stage_bytes);
-                tma_load_2d(smem_u32(smem + s * p.stage_bytes) + 2 * p.cols * 128, &tmW, smem_u32(&full[s]), i * 64, tile * 128);
+            // A position in the run: tile of the pass, span, the pass's first row of x parts.
+            struct Cursor { int tile, s, row; };
+            Cursor code{t_first % p.tiles, s_first, t_first / p.tiles * 3 * p.rows}, x = code;
+            auto step = [&](Cursor& c) {
+                if (++c.s < p.spans) return;
+                c.s = 0;
+                if (++c.tile == p.tiles) { c.tile = 0; c.row += 3 * p.rows; }
             };
-            for (int i = s0; i < min(s1, s0 + C::STAGES); ++i) load_codes(i, i - s0);
+            auto load_codes = [&](int s) {
+                mbar_arrive_expect_tx(smem_u32(&full[s]), p.stage_bytes);
+                tma_load_2d(smem_u32(smem + s * p.stage_bytes) + 2 * p.cols * 128, &tmW, smem_u32(&full[s]), code.s * 64,
+                            code.tile * 128);
+                step(code);
+            };
+            for (int i = 0; i < min(count, C::STAGES); ++i) load_codes(i);
             pdl_wait();
             int s = 0;
             uint32_t ph = 0;
-            for (int i = s0; i < s1; ++i) {
-                if (i >= s0 + C::STAGES) {
+            for (int i = 0; i < count; ++i) {
+                if (i >= C::STAGES) {
                     if (!mbar_wait_short(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
-                    load_codes(i, s);
+                    load_codes(s);
                 }
                 const uint32_t to = smem_u32(smem + s * p.stage_bytes), bar = smem_u32(&full[s]);
-                tma_load_2d(to, &tmX, bar, i * 128, (int)blockIdx.y * 3 * p.rows);
-                tma_load_2d(to + p.cols * 128, &tmX, bar, i * 128 + 64, (int)blockIdx.y * 3 * p.rows);
+                tma_load_2d(to, &tmX, bar, x.s * 128, x.row);
+                tma_load_2d(to + p.cols * 128, &tmX, bar, x.s * 128 + 64, x.row);
+                step(x);
                 if (++s == C::STAGES) { s = 0; ph ^= 1; }
             }
         }
@@ -209,7 +215,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
             const uint32_t a_bar = smem_u32(a_full + half * C::A_STAGES), acc_bar = smem_u32(acc_full + half * C::ACC);
             int s = 0, ab = 0, n = 0;
             uint32_t ph = 0, aph = 0, nph = 0;
-            for (int i = s0; i < s1; ++i) {
+            for (int i = 0; i < count; ++i) {
                 if (!mbar_wait_short(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) break;
                 if (!mbar_wait_short(a_bar + ab * 8, aph, abort_flag, kDevTimeoutMisc)) break;
                 bool ok = true;
@@ -242,7 +248,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
         const uint32_t a0 = tmem_a + ((uint32_t)(q * 32) << 16) + half * C::A_STAGES * 32;
         int s = 0, ab = 0;
         uint32_t ph = 0, aph = 0;
-        for (int i = s0; i < s1; ++i) {
+        for (int i = 0; i < count; ++i) {
             if (!mbar_wait_short(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull)) break;
             const uint8_t* codes = smem + s * p.stage_bytes + 2 * p.cols * 128 + row * 64 + half * 8;
             uint2 w[4];
@@ -268,8 +274,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
         }
     } else if (warp >= 12) {
         const int q = warp & 3, half = (warp - 12) >> 2;   // here of the rows of x
-        const int64_t row = (int64_t)tile * 128 + q * 32 + lane;
-        const uint16_t* sc = reinterpret_cast<const uint16_t*>(p.scales) + min(row, p.N - 1) * p.sp;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * (8 * NB);
         const uint32_t acc_bar = smem_u32(acc_full);
 #pragma unroll
@@ -277,20 +281,33 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
         // The scales of a span are loaded while the one before it is at work.
         constexpr int GROUPS = 128 / G;
         uint16_t next[GROUPS];
-        auto load_scales = [&](int i) {
-#pragma unroll
-            for (int k = 0; k < GROUPS; ++k) next[k] = i < s1 && i * GROUPS + k < p.groups ? __ldg(sc + i * GROUPS + k) : (uint16_t)0;
+        int tile = t_first % p.tiles, s = s_first, from = s_first;   // `from`: the first span of the run in the tile
+        int64_t m0 = (int64_t)(t_first / p.tiles) * p.rows;
+        bool first = true;                                           // the run's first tile
+        const uint16_t* sc = nullptr;
+        auto scales_of = [&](int tile) {
+            sc = reinterpret_cast<const uint16_t*>(p.scales) + min((int64_t)tile * 128 + q * 32 + lane, p.N - 1) * p.sp;
         };
-        load_scales(s0);
+        auto load_scales = [&](int s) {
+#pragma unroll
+            for (int k = 0; k < GROUPS; ++k) next[k] = s * GROUPS + k < p.groups ? __ldg(sc + s * GROUPS + k) : (uint16_t)0;
+        };
+        scales_of(tile);
+        load_scales(s);
         bool ok = true;
         int n = 0;
         uint32_t nph = 0;
 #pragma unroll 1
-        for (int i = s0; i < s1 && ok; ++i) {
+        for (int i = 0; i < count && ok; ++i) {
             float scale[GROUPS];
 #pragma unroll
             for (int k = 0; k < GROUPS; ++k) scale[k] = __uint_as_float((uint32_t)next[k] << 16);
-            load_scales(i + 1);
+            if (s + 1 < p.spans) {
+                load_scales(s + 1);
+            } else if (i + 1 < count) {
+                scales_of(tile + 1 == p.tiles ? 0 : tile + 1);
+                load_scales(0);
+            }
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
@@ -320,37 +337,30 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
                 }
                 if (++n == C::ACC) { n = 0; nph ^= 1; }
             }
-        }
-        const float bias = p.bias && row < p.N ? p.bias[row] : 0.f;
-        const int64_t m0 = (int64_t)blockIdx.y * p.rows;
+            if (++s == p.spans || i == count - 1) {
+                // One store per row of x, by pointers that step from row to row.
+                const int64_t row = (int64_t)tile * 128 + q * 32 + lane;
+                const bool whole = from == 0 && s == p.spans;
+                const int rows = min(p.rows, whole ? (int)min(p.M - m0, (int64_t)kRows) : kRows) - half * (8 * NB);
+                float* to = whole ? p.y.p + (m0 + half * (8 * NB)) * p.y.rs + row * p.y.cs
+                                  : p.part + (((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * p.rows + half * (8 * NB)) * 128 + q * 32 + lane;
+                const int64_t step = whole ? p.y.rs : 128;
+                const float bias = whole && p.bias && row < p.N ? p.bias[row] : 0.f;
+                const float unit = whole ? planes::kCodeUnit : 1.f;
+                const bool mine = !whole || row < p.N, relu = whole && p.relu;
 #pragma unroll
-        for (int j = 0; j < 8 * NB; ++j) {
-            const int m = half * (8 * NB) + j;
-            if (m < p.rows) {
-                if (ranks > 1) {
-                    red[m * 128 + q * 32 + lane] = acc[j];
-                } else if (m0 + m < p.M && row < p.N) {
-                    float v = fmaf(acc[j], planes::kCodeUnit, bias);
-                    if (p.relu) v = v > 0.f ? v : 0.f;
-                    p.y.p[(m0 + m) * p.y.rs + row * p.y.cs] = v;
+                for (int j = 0; j < 8 * NB; ++j) {
+                    float v = fmaf(acc[j], unit, bias);
+                    if (relu) v = v > 0.f ? v : 0.f;
+                    if (mine && j < rows) *to = v;
+                    to += step;
+                    acc[j] = 0.f;
                 }
+                from = s = 0;
+                first = false;
+                if (++tile == p.tiles) { tile = 0; m0 += p.rows; }
             }
         }
-    }
-    if (ranks > 1) {
-        // Every rank adds its share of the rows of x, the parts of k in order.
-        cluster_sync_all();
-        const int64_t m0 = (int64_t)blockIdx.y * p.rows, n0 = (int64_t)tile * 128;
-        for (int i = threadIdx.x; i < p.rows * 128; i += THREADS) {
-            const int m = i >> 7, r = i & 127;
-            if (m % ranks != rank || m0 + m >= p.M || n0 + r >= p.N) continue;
-            float v = 0.f;
-            for (int k = 0; k < ranks; ++k) v += ld_cluster(mapa_shared(smem_u32(red + i), k));
-            v = fmaf(v, planes::kCodeUnit, p.bias ? p.bias[n0 + r] : 0.f);
-            if (p.relu) v = v > 0.f ? v : 0.f;
-            p.y.p[(m0 + m) * p.y.rs + (n0 + r) * p.y.cs] = v;
-        }
-        cluster_sync_all();   // the others have read this CTA's sums
     }
     if (warp == 0 && lane == 0 && *abort_flag) {
         // Give copies already issued time to land before the CTA leaves.
@@ -363,6 +373,27 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
+}
+
+// Tiles that several runs share: the sum of their parts in order (+ bias, ReLU). blockIdx.x: tile,
+// blockIdx.y: two rows of x.
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+    const int t = blockIdx.x, first = t * p.spans, last = first + p.spans - 1;
+    const int wide = p.more * (p.each + 1);   // spans of the runs that have one more
+    auto owner = [&](int x) { return x < wide ? x / (p.each + 1) : p.more + (x - wide) / p.each; };
+    const int c0 = owner(first), c1 = owner(last);
+    const int m = blockIdx.y * 2 + (threadIdx.x >> 7), r = threadIdx.x & 127;
+    const int64_t row = (int64_t)(t % p.tiles) * 128 + r, mm = (int64_t)(t / p.tiles) * p.rows + m;
+    pdl_wait();
+    if (c0 == c1 || m >= p.rows || row >= p.N || mm >= p.M) return;
+    float v = 0.f;
+    for (int c = c0; c <= c1; ++c) {
+        const int slot = run_begin(p, c) / p.spans == t ? 0 : 1;
+        v += p.part[(((int64_t)c * 2 + slot) * p.rows + m) * 128 + r];
+    }
+    v = fmaf(v, planes::kCodeUnit, p.bias ? p.bias[row] : 0.f);
+    if (p.relu) v = v > 0.f ? v : 0.f;
+    p.y.p[mm * p.y.rs + row * p.y.cs] = v;
 }
 
 // The parts of x for q4b::gemm_kernel: out[pass][part][row of the pass][k].
