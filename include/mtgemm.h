@@ -20,7 +20,7 @@
  *   - Launches are asynchronous on `stream` (NULL = legacy default stream, the
  *     reference's active_stream() default); nothing synchronises inside a call, so calls
  *     can be captured in CUDA graphs.
- *   - Device memory: four paths take stream-ordered scratch (cudaMallocAsync and
+ *   - Device memory: these paths take stream-ordered scratch (cudaMallocAsync and
  *     cudaFreeAsync on `stream`; inside a capture these become graph memory nodes):
  *       . a GEMM whose output has too few tiles to fill the GPU (batch 1, no extra
  *         destinations, at least 8 k-blocks): its k range is split, the fp32 partials go
@@ -29,7 +29,9 @@
  *         activation (or of dY) and the weights reordered tap by tap;
  *       . the conv weight gradient, stated below (mt_conv2d_wgrad can take a caller
  *         workspace, mt_conv2d_wgrad_noalloc a fixed library array);
- *       . mt_matmul_host without a workspace: the device copies of A, B and C.
+ *       . mt_matmul_host without a workspace: the device copies of A, B and C;
+ *       . mt_rms_norm_backward (partial sums of dgamma), mt_linear_wgrad_q8 and, from 9 rows of
+ *         X on, mt_linear_fwd_q4 (bfloat16 forms of the operands, partial tiles).
  *     Strict-fp32 calls and every other path allocate nothing.
  *   - Every function returns an mt_status and never throws; mt_last_error() gives the
  *     thread-local message of the last failure.

@@ -870,7 +870,7 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Few rows in integers, batches with the weights in tensor memory, prompts as a product of
     // unpacked operands. Microseconds on weights of 4096 x 16384 (group 64), either side: 8 rows
-    // 23 and 27, 12 rows 29 and 27; 192 rows 105 and 107, 224 rows 134 and 108.
+    // 23 and 24, 12 rows 29 and 24; 192 rows 98 and 107, 256 rows 138 and 109.
     if (M > 192 && w.K > 0) return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
     if (M > 8 && w.K > 0) return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
     return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
