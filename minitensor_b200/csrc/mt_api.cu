@@ -2257,18 +2257,26 @@ int fail(int code, const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
-    t_err = buf;
+    try {
+        t_err = buf;
+    } catch (...) {   // no memory for the text: nothing may be thrown through a C entry
+    }
     return code;
 }
-int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+int cuda_fail(cudaError_t e, const char* what) { return fail(MT_ECUDA, "%s: %s", what, cudaGetErrorString(e)); }
 int launched(const char* what) {
     cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess && e != cudaErrorStreamCaptureUnsupported) return ::cuda_fail(e, what);
+    if (e != cudaSuccess && e != cudaErrorStreamCaptureUnsupported) return cuda_fail(e, what);
     g_launches.fetch_add(1);
     return MT_OK;
 }
-void set_path(const char* path) { t_path = path; }
-int sm_count() { return dev_info().sms; }
+void set_path(const char* path) {
+    try {
+        t_path = path;
+    } catch (...) {
+    }
+}
+int sm_count() { return std::max(1, dev_info().sms); }   // a machine without a GPU gets as far as its first CUDA call
 int device_cc() { return dev_info().cc; }
 int scratch_alloc(void** p, size_t bytes, cudaStream_t st, const char* who) { return ::scratch_alloc(p, bytes, st, who); }
 void scratch_free(void* p, size_t bytes, cudaStream_t st) { ::scratch_free(p, bytes, st); }

@@ -315,25 +315,30 @@ int launch_after(void (*kern)(Args...), dim3 grid, dim3 block, size_t smem, cuda
     return launched(who);
 }
 
-// D = A * B^T over `kpitch` padded values of k: a [R][kpitch], b [3][C][kpitch], both bfloat16.
-// p carries the output, the scales (SCALED) and the bias.
-template <bool SCALED, int SPC>
-int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16* b, int64_t kpitch, cudaStream_t st,
-               const char* who) {
+// Tiles and splits of a product over `kpitch` padded values of k; *part_bytes of scratch for the
+// parts of split tiles.
+template <int SPC>
+int plan_planes(mt::planes::Params& p, int64_t kpitch, size_t* part_bytes, const char* who) {
     using namespace mt::planes;
-    const int sms = mt::host::sm_count();
-    const int64_t clusters = std::max(1, sms / 2);
     p.kblocks = (int)((kpitch + BK - 1) / BK);
     p.tiles_r = (p.R + BM - 1) / BM;
     p.tiles_c = (p.C + BN - 1) / BN;
     const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c;
     if (tiles > INT32_MAX / 64) return fail(MT_EUNSUPPORTED, "%s: too many output tiles", who);
-    pick_splits(p, tiles, SPC == 8 ? 2 : 1, clusters);
+    pick_splits(p, tiles, SPC == 8 ? 2 : 1, std::max(1, mt::host::sm_count() / 2));
     const int64_t in_parts = tiles - p.whole;
     p.units = (int)(p.whole + in_parts * p.splits);
-    Scratch part(st);
-    if (in_parts) MT_TRY(part.take((size_t)in_parts * p.splits * BM * BN * sizeof(float), who));
-    p.part = static_cast<float*>(part.p);
+    *part_bytes = (size_t)in_parts * p.splits * BM * BN * sizeof(float);
+    return MT_OK;
+}
+
+// D = A * B^T: a [R][kpitch], b [3][C][kpitch], both bfloat16. p is planned and carries the output,
+// the scales (SCALED), the bias and the scratch for parts. The kernel before it on the stream
+// made a and b.
+template <bool SCALED, int SPC>
+int run_planes(const mt::planes::Params& p, const __nv_bfloat16* a, const __nv_bfloat16* b, int64_t kpitch, cudaStream_t st,
+               const char* who) {
+    using namespace mt::planes;
     CUtensorMap ta, tb;
     const uint64_t da[3] = {(uint64_t)kpitch, (uint64_t)p.R, 1}, db[3] = {(uint64_t)kpitch, (uint64_t)p.C, 3};
     const uint64_t sa[2] = {(uint64_t)kpitch * 2, (uint64_t)kpitch * 2 * p.R}, sb[2] = {(uint64_t)kpitch * 2, (uint64_t)kpitch * 2 * p.C};
@@ -349,7 +354,8 @@ int run_planes(mt::planes::Params p, const __nv_bfloat16* a, const __nv_bfloat16
         if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
         smem_set.fetch_or(bit);
     }
-    const unsigned grid = 2 * (unsigned)std::min<int64_t>(p.units, clusters);
+    const unsigned grid = 2 * (unsigned)std::min(p.units, std::max(1, mt::host::sm_count() / 2));
+    const int in_parts = p.tiles_r * p.tiles_c - p.whole;
     MT_TRY(launch_after(gemm_kernel<SCALED, SPC>, dim3(grid), dim3(THREADS), SMEM_BYTES, st, who, ta, tb, p));
     if (in_parts) MT_TRY(launch_after(join_kernel, dim3((unsigned)in_parts, BM / 8), dim3(256), 0, st, who, p));
     char path[96];
@@ -363,12 +369,18 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     const int64_t pitch = std::max<int64_t>(8, round_up(M, 8));
     const size_t a_bytes = round_up(K * pitch * 2, 256), b_bytes = round_up(3 * N * pitch * 2, 256);
     const int64_t tiles_m = (pitch + 63) / 64;
-    const size_t s_bytes = db.p ? (size_t)tiles_m * N * sizeof(float) : 0;
+    const size_t s_bytes = db.p ? round_up(tiles_m * N * sizeof(float), 256) : 0;
+    mt::planes::Params p{};
+    p.R = (int)K;
+    p.C = (int)N;
+    size_t part_bytes = 0;
+    MT_TRY(plan_planes<8>(p, pitch, &part_bytes, who));
     Scratch ws(st);
-    MT_TRY(ws.take(a_bytes + b_bytes + s_bytes, who));
+    MT_TRY(ws.take(a_bytes + b_bytes + s_bytes + part_bytes, who));
     __nv_bfloat16* a = static_cast<__nv_bfloat16*>(ws.p);
     __nv_bfloat16* b = a + a_bytes / 2;
     float* sums = db.p ? reinterpret_cast<float*>(b + b_bytes / 2) : nullptr;
+    p.part = reinterpret_cast<float*>(static_cast<char*>(ws.p) + a_bytes + b_bytes + s_bytes);
     const bool vec = (reinterpret_cast<uintptr_t>(q.codes) & 15) == 0 && (M == 1 || q.cp % 16 == 0);
     const int64_t blocks_a = (K + 63) / 64, blocks_b = (N + 63) / 64;
     const dim3 grid((unsigned)(blocks_a + blocks_b), grid_of(tiles_m, 65535));
@@ -380,9 +392,6 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
         mt::rms::sum_parts_kernel<<<(unsigned)((N + 31) / 32), dim3(32, 32), 0, st>>>(sums, tiles_m, N, db);
         return launched(who);
     }
-    mt::planes::Params p{};
-    p.R = (int)K;
-    p.C = (int)N;
     p.out = dw.p;
     p.os_r = dw.rs;
     p.os_c = dw.cs;
@@ -393,21 +402,25 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     return run_planes<false, 8>(p, a, b, pitch, st, who);
 }
 
+template <int SPC>
 int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias, const Mat& y, int64_t M, int relu,
                      cudaStream_t st, const char* who) {
     const int64_t pitch = round_up(w.K, mt::q4::kSpan);
-    const size_t a_bytes = w.N * pitch * 2, b_bytes = 3 * M * pitch * 2;
+    const size_t a_bytes = round_up(w.N * pitch * 2, 256), b_bytes = round_up(3 * M * pitch * 2, 256);
+    mt::planes::Params p{};
+    p.R = (int)w.N;
+    p.C = (int)M;
+    size_t part_bytes = 0;
+    MT_TRY(plan_planes<SPC>(p, pitch, &part_bytes, who));
     Scratch ws(st);
-    MT_TRY(ws.take(a_bytes + b_bytes, who));
+    MT_TRY(ws.take(a_bytes + b_bytes + part_bytes, who));
     __nv_bfloat16* a = static_cast<__nv_bfloat16*>(ws.p);
     __nv_bfloat16* b = a + a_bytes / 2;
+    p.part = reinterpret_cast<float*>(static_cast<char*>(ws.p) + a_bytes + b_bytes);
     const int64_t blocks_a = (pitch / 8 + 255) / 256, blocks_b = (pitch / 4 + 255) / 256;
     mt::planes::prepare_q4_kernel<<<dim3((unsigned)(blocks_a + blocks_b), grid_of((std::max(w.N, M) + 7) / 8, 65535)), 256, 0, st>>>(
         w, a, x.m, vec4(x), b, M, pitch, (int)blocks_b);
     MT_TRY(launched(who));
-    mt::planes::Params p{};
-    p.R = (int)w.N;
-    p.C = (int)M;
     p.out = y.p;
     p.os_r = y.cs;
     p.os_c = y.rs;
@@ -416,11 +429,7 @@ int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias,
     p.groups = (int)((w.K + w.group - 1) / w.group);
     p.bias = bias;
     p.relu = relu;
-    switch (w.group) {
-        case 32: return run_planes<true, 2>(p, a, b, pitch, st, who);
-        case 64: return run_planes<true, 4>(p, a, b, pitch, st, who);
-        default: return run_planes<true, 8>(p, a, b, pitch, st, who);
-    }
+    return run_planes<true, SPC>(p, a, b, pitch, st, who);
 }
 
 // ------------------------------ 4 bits, batches ---------------------------------------
@@ -871,7 +880,13 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     // Few rows in integers, batches with the weights in tensor memory, prompts as a product of
     // unpacked operands. Microseconds on weights of 4096 x 16384 (group 64), either side: 8 rows
     // 23 and 24, 12 rows 29 and 24; 192 rows 98 and 107, 256 rows 138 and 109.
-    if (M > 192 && w.K > 0) return linear_q4_planes(vx, w, vb.m.p, vy.m, M, relu, st, who);
+    if (M > 192 && w.K > 0) {
+        switch (w.group) {   // k16-steps per group
+            case 32: return linear_q4_planes<2>(vx, w, vb.m.p, vy.m, M, relu, st, who);
+            case 64: return linear_q4_planes<4>(vx, w, vb.m.p, vy.m, M, relu, st, who);
+            default: return linear_q4_planes<8>(vx, w, vb.m.p, vy.m, M, relu, st, who);
+        }
+    }
     if (M > 8 && w.K > 0) return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
     return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
 }

@@ -4,7 +4,8 @@
 //   D[r][c] = sum_k A[r][k] * B[c][k],  A bfloat16, B float
 //
 // Mathematics. A float is the exact sum of three bfloat16 numbers: truncating it to its top
-// 8 significand bits leaves a remainder of 16 bits, truncating that leaves 8 (split3). So
+// 8 significand bits leaves a remainder of 16 bits, truncating that leaves 8 (split3; below
+// 2^-110 the last part runs out of exponents, off by at most 2^-133). So
 // A * B is the sum of three products of 8-bit by 8-bit significands, each exact in the
 // float accumulator: three kind::f16 MMAs per k-step instead of the three of 3xTF32 at half
 // their rate, twice as fast, and no bits of the operands are lost.
@@ -19,9 +20,13 @@
 // Work. A pair of CTAs shares a 256 x 256 tile (tcgen05 cta_group::2, as umma_gemm2.cuh): each
 // holds its 128 rows of A and its 128 columns of the three planes of B, 64 KB per 64-deep
 // stage, 3 stages. Warp 0 loads by TMA, warp 1 of the even CTA issues the MMAs, warps 2-9
-// drain: lane quarter = warp & 3, 128 columns each, 128 accumulators per thread. Few tiles:
-// the sum over k is split between clusters, partial tiles go to scratch and a second kernel
-// adds them in order. Bound: tensor pipe, 3 * 2 R C K operations.
+// drain: lane quarter = warp & 3, 128 columns each, 128 accumulators per thread. The tiles of a
+// last round that would leave clusters idle are split over k between them; their parts go to
+// scratch and a second kernel adds them in order. Bound: tensor pipe, 3 * 2 R C K operations: 8192^3 in 2039 us, 1617 TFLOP/s
+// of bfloat16 work, 0.97 of measured peak (one launch; 2.4 ms in a row, under the power cap).
+// Three 64-deep stages, because 64 KB a stage leave room for no fourth; 256 x 256 tiles, because
+// a CTA alone on 128 x 256 would move 112 KB through shared memory in the time that bandwidth
+// has for 190 KB of reads and writes, of which the MMAs' reads alone are 144 KB.
 #pragma once
 
 #include "lowbit_common.cuh"

@@ -22,6 +22,10 @@
 // drain the accumulators, half of the rows of x each. What bounds a step is the roles'
 // instructions and hand-overs (a half is 182 cycles of memory, an MMA 24 cycles at 16 rows of
 // x), hence two issuers and waits in few instructions. Up to 64 rows of x at a time ("pass").
+//
+// Measured on 4096 -> 16384 (group 64): 16 rows 25 us, 64 rows 36 us, 192 rows 98 us; one issuer
+// took 35 us for 16 rows, and unpacked steps and accumulators in half of tensor memory with two
+// CTAs per SM no less.
 #pragma once
 
 #include "planes_gemm.cuh"

@@ -215,3 +215,19 @@ def test_linear_q4_refusals():
         assert L.mt_linear_fwd_q4(b(x), b(bad), None, b(y), 0, None) == engine.MT_EINVAL
     assert L.mt_quantize_q4(b(v(t(99, 8))), b(c), None) == engine.MT_EINVAL
     assert L.mt_dequantize_q4(b(c), b(v(t(100, 9))), None) == engine.MT_EINVAL
+
+
+def test_valid_calls_without_a_gpu_end_in_an_error():
+    """Nothing is divided by the number of SMs of a GPU that is not there."""
+    if torch.cuda.is_available():
+        pytest.skip("needs a machine without a GPU")
+    w = q4(256, 64)
+    for rows in (1, 8, 20, 100, 300):
+        with pytest.raises(RuntimeError):
+            mt.linear_forward_q4(t(rows, 256), w)
+    for call in (lambda: mt.linear_weight_grad_q8(q8(300, 200), t(300, 70)), lambda: mt.quantize_q8(t(3, 64)),
+                 lambda: mt.dequantize_q8(q8(3, 64)), lambda: mt.quantize_q4(t(64, 8)), lambda: mt.dequantize_q4(w),
+                 lambda: mt.rms_norm(t(3, 64), t(64), q8="e4m3"), lambda: mt.rms_norm(t(3, 50000), t(50000)),
+                 lambda: mt.rms_norm_backward(t(3, 64), t(3, 64), t(64), t(3))):
+        with pytest.raises(RuntimeError):
+            call()

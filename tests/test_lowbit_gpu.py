@@ -292,6 +292,26 @@ def test_linear_weight_grad_q8_keeps_every_bit(mt, fmt):
     assert torch.equal(host(db), dy)
 
 
+def test_linear_weight_grad_q8_split_over_the_rows(mt):
+    """One tile of dW from many rows, whose sum is cut into parts."""
+    q, dy = wgrad_input(gen(9), 5000, 40, 70, "int8", mt)
+    got = mt.linear_weight_grad_q8(q, dy.cuda())
+    assert "splits=1" not in mt.engine.last_path()
+    check_wgrad(q, dy, *got)
+
+
+def test_linear_weight_grad_q8_small_gradients(mt):
+    """Gradients down to 2^-125: the third part of the smallest is off by at most 2^-133, which x,
+    a power of two here, carries into dW."""
+    g = gen(10)
+    x = torch.ones(1, 64)
+    dy = torch.ldexp(torch.rand(1, 130, generator=g) + 1, torch.randint(-125, -90, (1, 130), generator=g))
+    dW, db = mt.linear_weight_grad_q8(mt.quantize_q8(x.cuda()), dy.cuda())
+    err = (host(dW).double() - dy.double()).abs()
+    assert (err <= 2.0 ** -133 + 3 * R.U * dy.double()).all()
+    assert torch.equal(host(db), dy)
+
+
 def test_linear_weight_grad_q8_empty(mt):
     q = mt.quantize_q8(torch.empty(0, 64, device="cuda"))
     dW, db = mt.linear_weight_grad_q8(q, torch.empty(0, 40, device="cuda"))
@@ -509,6 +529,8 @@ def calls(mt, g):
     q = mt.quantize_q8(x, "int8")
     w = mt.quantize_q4(W, 32)
     wide = rand(g, 300, K).cuda()
+    long_q, long_dy = mt.quantize_q8(rand(g, 4096, 96).cuda()), rand(g, 4096, 70).cuda()
+    long_x, long_w = rand(g, 260, 8192).cuda(), mt.quantize_q4(rand(g, 8192, 64).cuda(), 64)
 
     def flat(v):
         if isinstance(v, torch.Tensor):
@@ -531,12 +553,14 @@ def calls(mt, g):
         "dequantize 4": ([w.codes], lambda **k: flat(mt.dequantize_q4(w, **k))),
         "4 bits, one row": ([x], lambda **k: flat(mt.linear_forward_q4(x[:1], w, **k))),
         "4 bits, batch": ([x], lambda **k: flat(mt.linear_forward_q4(x, w, **k))),
+        "weight grad, split": ([long_q.codes, long_dy], lambda **k: flat(mt.linear_weight_grad_q8(long_q, long_dy, **k))),
+        "4 bits, prompt, split": ([long_x], lambda **k: flat(mt.linear_forward_q4(long_x, long_w, **k))),
         "4 bits, prompt": ([wide], lambda **k: flat(mt.linear_forward_q4(wide, w, **k))),
     }
 
 
 NAMES = ["norm", "norm backward", "quantize", "dequantize", "weight grad", "forward and checkpoint", "backward", "quantize 4",
-         "dequantize 4", "4 bits, one row", "4 bits, batch", "4 bits, prompt"]
+         "dequantize 4", "4 bits, one row", "4 bits, batch", "4 bits, prompt", "weight grad, split", "4 bits, prompt, split"]
 
 
 def change(inputs):
@@ -563,7 +587,8 @@ def test_captured_call_reads_its_inputs_at_replay(mt, name):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
-@pytest.mark.parametrize("name", ["norm backward", "weight grad", "4 bits, batch", "4 bits, prompt"])
+@pytest.mark.parametrize("name", ["norm backward", "weight grad", "weight grad, split", "4 bits, batch", "4 bits, prompt",
+                                  "4 bits, prompt, split"])
 def test_two_graphs_at_once_have_scratch_of_their_own(mt, name):
     sides = []
     for seed in (2, 3):
