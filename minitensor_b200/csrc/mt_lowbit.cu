@@ -271,27 +271,31 @@ struct Scratch {
     }
 };
 
-// How many tiles are done at once, and in how many parts of k the others: a full round of
-// clusters takes whole tiles, the tiles of a last round that would leave clusters idle are
-// split between them. A 64-deep block of a pair tile takes about 1,600 cycles; a split costs
-// another kernel and its parts' way through memory, about 4,000 bytes a cycle.
-void pick_splits(mt::planes::Params& p, int64_t tiles, int64_t chunk_blocks, int64_t clusters) {
+// How a product is cut: columns of a tile, tiles done at once, and in how many parts of k the
+// others. A full round of clusters takes whole tiles; the tiles of a last round that would leave
+// clusters idle are split between them. Cycles: a 64-deep block of a 256 x 256 tile takes about
+// 1,600, of a 256 x 128 tile (bound by shared memory) 1,000; a tile's end 6,000 or 3,500; a split
+// another kernel, 4,000, and its parts' way through memory at 5,000 bytes a cycle.
+double plan_tiles(mt::planes::Params& p, int bn, int64_t chunk_blocks, int64_t clusters) {
+    const double block = bn == 256 ? 1600. : 1000., end = bn == 256 ? 6000. : 3500.;
+    p.tiles_c = (p.C + bn - 1) / bn;
+    const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c, rest = tiles % clusters;
+    const int64_t nb = (p.kblocks + chunk_blocks - 1) / chunk_blocks;
     p.whole = (int)tiles;
     p.splits = 1;
-    const int64_t rest = tiles % clusters;
-    if (rest == 0) return;
-    const int64_t nb = (p.kblocks + chunk_blocks - 1) / chunk_blocks;
-    double least = (double)nb * chunk_blocks * 1600.;   // the last round as it is
-    const int64_t most = std::min<int64_t>(64, std::min(nb, clusters / rest));
+    const double round = (double)nb * chunk_blocks * block + end;
+    double last = rest ? round : 0.;   // the last round as it is
+    const int64_t most = rest ? std::min<int64_t>(64, std::min(nb, clusters / rest)) : 1;
     for (int64_t s = 2; s <= most; ++s) {
-        const double cost = (double)((nb + s - 1) / s * chunk_blocks) * 1600. +
-                            (double)(2 * s + 1) * rest * (mt::planes::BM * mt::planes::BN * 4) / 4000. + 5000.;
-        if (cost < least) {
-            least = cost;
+        const double cost = (double)((nb + s - 1) / s * chunk_blocks) * block + end +
+                            (double)(2 * s + 1) * rest * (mt::planes::BM * bn * 4) / 5000. + 4000.;
+        if (cost < last) {
+            last = cost;
             p.splits = (int)s;
             p.whole = (int)(tiles - rest);
         }
     }
+    return (double)(tiles / clusters) * round + last;
 }
 
 // Launches a kernel that calls pdl_wait before it reads what the kernel before it wrote.
@@ -315,34 +319,38 @@ int launch_after(void (*kern)(Args...), dim3 grid, dim3 block, size_t smem, cuda
     return launched(who);
 }
 
-// Tiles and splits of a product over `kpitch` padded values of k; *part_bytes of scratch for the
-// parts of split tiles.
+// Tiles and splits of a product over `kpitch` padded values of k; *bn columns of a tile and
+// *part_bytes of scratch for the parts of split tiles.
 template <int SPC>
-int plan_planes(mt::planes::Params& p, int64_t kpitch, size_t* part_bytes, const char* who) {
+int plan_planes(mt::planes::Params& p, int64_t kpitch, int* bn, size_t* part_bytes, const char* who) {
     using namespace mt::planes;
     p.kblocks = (int)((kpitch + BK - 1) / BK);
     p.tiles_r = (p.R + BM - 1) / BM;
-    p.tiles_c = (p.C + BN - 1) / BN;
-    const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c;
-    if (tiles > INT32_MAX / 64) return fail(MT_EUNSUPPORTED, "%s: too many output tiles", who);
-    pick_splits(p, tiles, SPC == 8 ? 2 : 1, std::max(1, mt::host::sm_count() / 2));
-    const int64_t in_parts = tiles - p.whole;
+    if ((int64_t)p.tiles_r * ((p.C + 127) / 128) > INT32_MAX / 64) return fail(MT_EUNSUPPORTED, "%s: too many output tiles", who);
+    const int64_t clusters = std::max(1, mt::host::sm_count() / 2), chunk = SPC == 8 ? 2 : 1;
+    Params narrow = p;
+    *bn = 256;
+    if (plan_tiles(narrow, 128, chunk, clusters) < plan_tiles(p, 256, chunk, clusters)) {
+        p = narrow;
+        *bn = 128;
+    }
+    const int64_t in_parts = (int64_t)p.tiles_r * p.tiles_c - p.whole;
     p.units = (int)(p.whole + in_parts * p.splits);
-    *part_bytes = (size_t)in_parts * p.splits * BM * BN * sizeof(float);
+    *part_bytes = (size_t)in_parts * p.splits * BM * *bn * sizeof(float);
     return MT_OK;
 }
 
 // D = A * B^T: a [R][kpitch], b [3][C][kpitch], both bfloat16. p is planned and carries the output,
 // the scales (SCALED), the bias and the scratch for parts. The kernel before it on the stream
 // made a and b.
-template <bool SCALED, int SPC>
+template <bool SCALED, int SPC, int BN>
 int run_planes(const mt::planes::Params& p, const __nv_bfloat16* a, const __nv_bfloat16* b, int64_t kpitch, cudaStream_t st,
                const char* who) {
     using namespace mt::planes;
     CUtensorMap ta, tb;
     const uint64_t da[3] = {(uint64_t)kpitch, (uint64_t)p.R, 1}, db[3] = {(uint64_t)kpitch, (uint64_t)p.C, 3};
     const uint64_t sa[2] = {(uint64_t)kpitch * 2, (uint64_t)kpitch * 2 * p.R}, sb[2] = {(uint64_t)kpitch * 2, (uint64_t)kpitch * 2 * p.C};
-    const uint32_t ba[3] = {BK, 128, 1}, bb[3] = {BK, 128, 3};
+    const uint32_t ba[3] = {BK, 128, 1}, bb[3] = {BK, BN / 2, 3};
     if (!mt::host::encode_bf16(&ta, a, 3, da, sa, ba) || !mt::host::encode_bf16(&tb, b, 3, db, sb, bb))
         return fail(MT_ECUDA, "%s: tensor map encoding failed", who);
     static std::atomic<uint64_t> smem_set{0};
@@ -350,16 +358,16 @@ int run_planes(const mt::planes::Params& p, const __nv_bfloat16* a, const __nv_b
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if (!(smem_set.load() & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<SCALED, SPC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+        cudaError_t e = cudaFuncSetAttribute(gemm_kernel<SCALED, SPC, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<BN>::SMEM_BYTES);
         if (e != cudaSuccess) return mt::host::cuda_fail(e, who);
         smem_set.fetch_or(bit);
     }
     const unsigned grid = 2 * (unsigned)std::min(p.units, std::max(1, mt::host::sm_count() / 2));
     const int in_parts = p.tiles_r * p.tiles_c - p.whole;
-    MT_TRY(launch_after(gemm_kernel<SCALED, SPC>, dim3(grid), dim3(THREADS), SMEM_BYTES, st, who, ta, tb, p));
-    if (in_parts) MT_TRY(launch_after(join_kernel, dim3((unsigned)in_parts, BM / 8), dim3(256), 0, st, who, p));
+    MT_TRY(launch_after(gemm_kernel<SCALED, SPC, BN>, dim3(grid), dim3(THREADS), Cfg<BN>::SMEM_BYTES, st, who, ta, tb, p));
+    if (in_parts) MT_TRY(launch_after(join_kernel<BN>, dim3((unsigned)in_parts, BM * BN / 2048), dim3(256), 0, st, who, p));
     char path[96];
-    snprintf(path, sizeof path, "%s planes whole=%d splits=%d", who, p.whole, p.splits);
+    snprintf(path, sizeof path, "%s planes bn=%d whole=%d splits=%d", who, BN, p.whole, p.splits);
     mt::host::set_path(path);
     return MT_OK;
 }
@@ -373,8 +381,9 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     mt::planes::Params p{};
     p.R = (int)K;
     p.C = (int)N;
+    int bn = 0;
     size_t part_bytes = 0;
-    MT_TRY(plan_planes<8>(p, pitch, &part_bytes, who));
+    MT_TRY(plan_planes<8>(p, pitch, &bn, &part_bytes, who));
     Scratch ws(st);
     MT_TRY(ws.take(a_bytes + b_bytes + s_bytes + part_bytes, who));
     __nv_bfloat16* a = static_cast<__nv_bfloat16*>(ws.p);
@@ -399,7 +408,7 @@ int wgrad_planes(const Q8& q, const Mat& dy, const Mat& dw, const Mat& db, int64
     p.db_tiles = db.p ? (int)tiles_m : 0;
     p.db = db.p;
     p.db_cs = db.cs;
-    return run_planes<false, 8>(p, a, b, pitch, st, who);
+    return bn == 256 ? run_planes<false, 8, 256>(p, a, b, pitch, st, who) : run_planes<false, 8, 128>(p, a, b, pitch, st, who);
 }
 
 template <int SPC>
@@ -410,8 +419,9 @@ int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias,
     mt::planes::Params p{};
     p.R = (int)w.N;
     p.C = (int)M;
+    int bn = 0;
     size_t part_bytes = 0;
-    MT_TRY(plan_planes<SPC>(p, pitch, &part_bytes, who));
+    MT_TRY(plan_planes<SPC>(p, pitch, &bn, &part_bytes, who));
     Scratch ws(st);
     MT_TRY(ws.take(a_bytes + b_bytes + part_bytes, who));
     __nv_bfloat16* a = static_cast<__nv_bfloat16*>(ws.p);
@@ -429,7 +439,7 @@ int linear_q4_planes(const View2& x, const mt::q4::Weight& w, const float* bias,
     p.groups = (int)((w.K + w.group - 1) / w.group);
     p.bias = bias;
     p.relu = relu;
-    return run_planes<true, SPC>(p, a, b, pitch, st, who);
+    return bn == 256 ? run_planes<true, SPC, 256>(p, a, b, pitch, st, who) : run_planes<true, SPC, 128>(p, a, b, pitch, st, who);
 }
 
 // ------------------------------ 4 bits, batches ---------------------------------------

@@ -20,7 +20,8 @@
 // Work. A pair of CTAs shares a 256 x 256 tile (tcgen05 cta_group::2, as umma_gemm2.cuh): each
 // holds its 128 rows of A and its 128 columns of the three planes of B, 64 KB per 64-deep
 // stage, 3 stages. Warp 0 loads by TMA, warp 1 of the even CTA issues the MMAs, warps 2-9
-// drain: lane quarter = warp & 3, 128 columns each, 128 accumulators per thread. The tiles of a
+// drain: lane quarter = warp & 3, 128 columns each, 128 accumulators per thread. Products that
+// do not fill the GPU with such tiles take 256 x 128 ones (five stages). The tiles of a
 // last round that would leave clusters idle are split over k between them; their parts go to
 // scratch and a second kernel adds them in order. Bound: tensor pipe, 3 * 2 R C K operations: 8192^3 in 2039 us, 1617 TFLOP/s
 // of bfloat16 work, 0.97 of measured peak (one launch; 2.4 ms in a row, under the power cap).
@@ -37,20 +38,24 @@ namespace planes {
 
 using lowbit::Mat;
 
-constexpr int BM = 256, BN = 256;       // pair tile
+constexpr int BM = 256;                 // rows of a pair tile
 constexpr int BK = 64;                  // k per stage: 128-byte rows
-constexpr int STAGES = 3;
 constexpr uint32_t A_BYTES = 128 * BK * 2;
-constexpr uint32_t B_BYTES = 128 * BK * 2;            // one plane
-constexpr uint32_t STAGE_BYTES = A_BYTES + 3 * B_BYTES;
-constexpr uint32_t RING_BYTES = STAGE_BYTES * STAGES;
 constexpr float kCodeUnit = 2048.f;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
 constexpr uint32_t EPI_BYTES = EPI_WARPS * 32 * 20 * 4;
-constexpr uint32_t BAR_BYTES = 8 * (2 * STAGES + 4) + 16;
-constexpr uint32_t SMEM_BYTES = 1024 + RING_BYTES + EPI_BYTES + BAR_BYTES;
-static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
+
+// By the columns of a pair tile, 256 or 128.
+template <int BN>
+struct Cfg {
+    static constexpr int STAGES = BN == 256 ? 3 : 5;
+    static constexpr uint32_t B_BYTES = BN / 2 * BK * 2;       // one plane of a CTA's columns
+    static constexpr uint32_t STAGE_BYTES = A_BYTES + 3 * B_BYTES;
+    static constexpr uint32_t RING_BYTES = STAGE_BYTES * STAGES;
+    static constexpr uint32_t SMEM_BYTES = 1024 + RING_BYTES + EPI_BYTES + 8 * (2 * STAGES + 4) + 16;
+    static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
+};
 
 struct Params {
     int R, C;                    // rows of A, rows of B
@@ -60,7 +65,7 @@ struct Params {
     int units;                   // whole + splits * (tiles - whole)
     float* out;                  // D[r][c] at out + r * os_r + c * os_c
     int64_t os_r, os_c;
-    float* part;                 // part s of tile t at ((t - whole) * splits + s) * 256 * 256
+    float* part;                 // part s of tile t at ((t - whole) * splits + s) * 256 * BN
     const __nv_bfloat16* scales; // SCALED: scale of row r, chunk j at r * sp + j
     int64_t sp;
     int groups;                  // scales per row; chunks behind them have no codes
@@ -115,9 +120,12 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t adesc, 
 }
 
 // SPC: k16-steps per chunk, 2, 4 or 8.
-template <bool SCALED, int SPC>
+template <bool SCALED, int SPC, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+    using G = Cfg<BN>;
+    constexpr int STAGES = G::STAGES, HALF = BN / 2;
+    constexpr uint32_t B_BYTES = G::B_BYTES, STAGE_BYTES = G::STAGE_BYTES, RING_BYTES = G::RING_BYTES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* ring = smem;
@@ -152,7 +160,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         tma_prefetch_desc(&tmB);
     }
     if (warp == 1) {
-        tmem_alloc_pair(smem_u32((const void*)tmem_slot), 512);
+        tmem_alloc_pair(smem_u32((const void*)tmem_slot), 2 * BN);
         tmem_relinquish_pair();
     }
     tc_fence_before();
@@ -169,7 +177,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             uint32_t ph = 0;
             for (int u = first; u < p.units; u += step) {
                 tile_of(p, unit_of<SPC>(p, u, sp, kb0, kb1), rb, cb);
-                const int r0 = rb * BM + (int)rank * 128, c0 = cb * BN + (int)rank * 128;
+                const int r0 = rb * BM + (int)rank * 128, c0 = cb * BN + (int)rank * HALF;
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!mbar_wait_cl(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) goto done;
                     const uint32_t sa = smem_u32(ring + s * STAGE_BYTES);
@@ -232,31 +240,38 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;
         float* buf = epi + (warp - 2) * 32 * 20;
-        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * 128;
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * HALF;
         const uint32_t empty_bar[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
         int n = 0;
         if (!SCALED && p.db_tiles > 0) {
             pdl_wait();
-            // The bias gradient, while the first tiles load.
-            for (int64_t c = (int64_t)blockIdx.x * (32 * EPI_WARPS) + (int)threadIdx.x - 64; c < p.C; c += (int64_t)gridDim.x * (32 * EPI_WARPS)) {
+            // The bias gradient, while the first tiles load: 4 columns per warp, 8 lanes each, which
+            // take every eighth partial sum.
+            const int sub = lane & 7;
+            for (int64_t c0 = ((int64_t)blockIdx.x * EPI_WARPS + warp - 2) * 4; c0 < p.C; c0 += (int64_t)gridDim.x * EPI_WARPS * 4) {
+                const int64_t c = c0 + (lane >> 3);
                 float s = 0.f;
+                if (c < p.C) {
 #pragma unroll 8
-                for (int t = 0; t < p.db_tiles; ++t) s += p.col_sums[(int64_t)t * p.C + c];
-                p.db[c * p.db_cs] = s;
+                    for (int t = sub; t < p.db_tiles; t += 8) s += p.col_sums[(int64_t)t * p.C + c];
+                }
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (sub == 0 && c < p.C) p.db[c * p.db_cs] = s;
             }
         }
         for (int u = first; u < p.units; u += step) {
             const int tile = unit_of<SPC>(p, u, sp, kb0, kb1);
             tile_of(p, tile, rb, cb);
             const int row0 = rb * BM + (int)rank * 128 + q * 32;
-            const int col0 = cb * BN + half * 128;
+            const int col0 = cb * BN + half * HALF;
             const int chunks = ((kb1 - kb0) * 4 + SPC - 1) / SPC;
             const __nv_bfloat16* sc = nullptr;
             const int g0 = kb0 * 4 / SPC;
             if (SCALED) sc = p.scales + (int64_t)min(row0 + lane, p.R - 1) * p.sp;
-            float acc[128];
+            float acc[HALF];
 #pragma unroll
-            for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+            for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
 #pragma unroll 1
             for (int ch = 0; ch < chunks; ++ch, ++n) {
                 const int a = n & 1;
@@ -266,11 +281,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 __syncwarp();
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < HALF / 16; ++c) {
                     uint32_t r[16];
                     tmem_ld_32x32b_x16(taddr + a * BN + c * 16, r);
                     tmem_ld_wait();
-                    if (c == 7) {
+                    if (c == HALF / 16 - 1) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(empty_bar[a]);
@@ -282,18 +297,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 }
             }
             const bool whole = sp < 0;
-            // The parts of a tile are stored as whole 256 x 256 tiles, along r or c as D is.
+            // The parts of a tile are stored as whole tiles, along r or c as D is.
             const bool along_r = p.os_r == 1;
-            const int pr = (int)rank * 128 + q * 32, pc = half * 128;
+            const int pr = (int)rank * 128 + q * 32, pc = half * HALF;
             float* out = whole ? p.out + (int64_t)row0 * p.os_r + (int64_t)col0 * p.os_c
                                : p.part + ((int64_t)(tile - p.whole) * p.splits + sp) * (BM * BN) + (along_r ? pc * BM + pr : pr * BN + pc);
             const int64_t os_r = whole ? p.os_r : along_r ? 1 : BN, os_c = whole ? p.os_c : along_r ? BM : 1;
-            const int rows = whole ? min(32, p.R - row0) : 32, cols = whole ? min(128, p.C - col0) : 128;
+            const int rows = whole ? min(32, p.R - row0) : 32, cols = whole ? min(HALF, p.C - col0) : HALF;
             if (SCALED) {
                 const int row = row0 + lane;
                 const float b = whole && p.bias && row < p.R ? p.bias[row] : 0.f;
 #pragma unroll
-                for (int j = 0; j < 128; ++j) {
+                for (int j = 0; j < HALF; ++j) {
                     acc[j] = fmaf(acc[j], kCodeUnit, b);
                     if (whole && p.relu) acc[j] = acc[j] > 0.f ? acc[j] : 0.f;
                 }
@@ -303,7 +318,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 if (lane < rows) {
                     float* o = out + lane;
 #pragma unroll
-                    for (int j = 0; j < 128; ++j) {
+                    for (int j = 0; j < HALF; ++j) {
                         if (j < cols) *o = acc[j];
                         o += os_c;
                     }
@@ -313,7 +328,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 // 8 lanes fall on different banks), then 4 lanes along c and 8 rows at a time.
                 const bool vec = os_c == 1 && os_r % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
-                for (int c = 0; c < 128; c += 16) {
+                for (int c = 0; c < HALF; c += 16) {
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 16; j += 4)
@@ -347,12 +362,13 @@ done:
     cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem_base, 512);
+        tmem_dealloc_pair(tmem_base, 2 * BN);
     }
 }
 
 // The tiles that were done in parts: the sum of the parts in order (+ bias per row, ReLU). A thread
-// has one column (or row, where rows are neighbours in D) of 8 rows (columns).
+// has 8 elements.
+template <int BN>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
     const int t = blockIdx.x;
     pdl_wait();
@@ -360,8 +376,11 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
     tile_of(p, p.whole + t, rb, cb);
     const bool along_r = p.os_r == 1;
     const float* part = p.part + (int64_t)t * p.splits * (BM * BN);
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int a = blockIdx.y * 8 + i, r = along_r ? threadIdx.x : a, c = along_r ? a : threadIdx.x;
+        // 256 neighbours along r or c per step, whichever is D's unit stride.
+        const int e = (blockIdx.y * 8 + i) * 256 + threadIdx.x;
+        const int r = along_r ? e % BM : e / BN, c = along_r ? e / BM : e % BN;
         const float* at = part + (along_r ? c * BM + r : r * BN + c);
         float v = *at;
         for (int s = 1; s < p.splits; ++s) v += at[s * (BM * BN)];
