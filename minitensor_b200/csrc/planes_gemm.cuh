@@ -21,9 +21,15 @@
 // holds its 128 rows of A and its 128 columns of the three planes of B, 64 KB per 64-deep
 // stage, 3 stages. Warp 0 loads by TMA, warp 1 of the even CTA issues the MMAs, warps 2-9
 // drain: lane quarter = warp & 3, 128 columns each, 128 accumulators per thread. Products that
-// do not fill the GPU with such tiles take 256 x 128 ones (five stages). The tiles of a
-// last round that would leave clusters idle are split over k between them; their parts go to
-// scratch and a second kernel adds them in order. Bound: tensor pipe, 3 * 2 R C K operations: 8192^3 in 2039 us, 1617 TFLOP/s
+// do not fill the GPU with such tiles take 256 x 128 ones, five stages and four accumulators
+// (777 x 1001 x 1303: 25.6 -> 18 us; 8192^3 would lose a third to reads of shared memory). The
+// tiles of a last round that would leave clusters idle are split over k between them; their parts
+// go to scratch and a second kernel adds them in order.
+// Waits: what follows a wait here are copies and MMAs, or reads of tensor memory behind a
+// tcgen05 fence, and no thread's ordinary stores, so none needs an acquire at cluster scope. That
+// would empty the L1 with the scales in it at every chunk: groups of 32, 2048 x 4096 x 8192 379
+// against 337 us, 2048 x 5376 x 1536 168 against 128 us.
+// Bound: tensor pipe, 3 * 2 R C K operations: 8192^3 in 2039 us, 1617 TFLOP/s
 // of bfloat16 work, 0.97 of measured peak (one launch; 2.4 ms in a row, under the power cap).
 // Three 64-deep stages, because 64 KB a stage leave room for no fourth; 256 x 256 tiles, because
 // a CTA alone on 128 x 256 would move 112 KB through shared memory in the time that bandwidth
@@ -50,10 +56,11 @@ constexpr uint32_t EPI_BYTES = EPI_WARPS * 32 * 20 * 4;
 template <int BN>
 struct Cfg {
     static constexpr int STAGES = BN == 256 ? 3 : 5;
+    static constexpr int ACCS = 512 / BN;                      // accumulators, all of tensor memory
     static constexpr uint32_t B_BYTES = BN / 2 * BK * 2;       // one plane of a CTA's columns
     static constexpr uint32_t STAGE_BYTES = A_BYTES + 3 * B_BYTES;
     static constexpr uint32_t RING_BYTES = STAGE_BYTES * STAGES;
-    static constexpr uint32_t SMEM_BYTES = 1024 + RING_BYTES + EPI_BYTES + 8 * (2 * STAGES + 4) + 16;
+    static constexpr uint32_t SMEM_BYTES = 1024 + RING_BYTES + EPI_BYTES + 8 * (2 * STAGES + 2 * ACCS) + 16;
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 };
 
@@ -124,7 +131,7 @@ template <bool SCALED, int SPC, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
     using G = Cfg<BN>;
-    constexpr int STAGES = G::STAGES, HALF = BN / 2;
+    constexpr int STAGES = G::STAGES, ACCS = G::ACCS, HALF = BN / 2;
     constexpr uint32_t B_BYTES = G::B_BYTES, STAGE_BYTES = G::STAGE_BYTES, RING_BYTES = G::RING_BYTES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -134,9 +141,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     uint64_t* full = bars;
     uint64_t* empty = bars + STAGES;
     uint64_t* acc_full = bars + 2 * STAGES;
-    uint64_t* acc_empty = bars + 2 * STAGES + 2;
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * STAGES + 4);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * STAGES + 4) + 1;
+    uint64_t* acc_empty = acc_full + ACCS;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(acc_empty + ACCS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_empty + ACCS) + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
@@ -148,7 +155,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             mbar_init(smem_u32(&full[s]), 1);
             mbar_init(smem_u32(&empty[s]), 1);
         }
-        for (int a = 0; a < 2; ++a) {
+        for (int a = 0; a < ACCS; ++a) {
             mbar_init(smem_u32(&acc_full[a]), 1);
             mbar_init(smem_u32(&acc_empty[a]), 2 * EPI_WARPS);
         }
@@ -160,7 +167,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         tma_prefetch_desc(&tmB);
     }
     if (warp == 1) {
-        tmem_alloc_pair(smem_u32((const void*)tmem_slot), 2 * BN);
+        tmem_alloc_pair(smem_u32((const void*)tmem_slot), 512);
         tmem_relinquish_pair();
     }
     tc_fence_before();
@@ -179,7 +186,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 tile_of(p, unit_of<SPC>(p, u, sp, kb0, kb1), rb, cb);
                 const int r0 = rb * BM + (int)rank * 128, c0 = cb * BN + (int)rank * HALF;
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait_cl(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) goto done;
+                    if (!mbar_wait_short(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) goto done;
                     const uint32_t sa = smem_u32(ring + s * STAGE_BYTES);
                     if (leader) mbar_arrive_expect_tx(smem_u32(&full[s]), 2 * STAGE_BYTES);
                     const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
@@ -202,15 +209,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 unit_of<SPC>(p, u, sp, kb0, kb1);
                 int in_chunk = 0;
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    ok = mbar_wait_cl(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull);
+                    ok = mbar_wait_short(smem_u32(&full[s]), ph, abort_flag, kDevTimeoutFull);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t sa = a0 + s * (STAGE_BYTES >> 4);
 #pragma unroll
                     for (int sub = 0; sub < 4; sub += STEPS) {
-                        const int a = n & 1;
+                        const int a = n % ACCS;
                         if (in_chunk == 0) {
-                            ok = mbar_wait_cl(smem_u32(&acc_empty[a]), ((n >> 1) & 1) ^ 1, abort_flag, kDevTimeoutAccEmpty);
+                            ok = mbar_wait_short(smem_u32(&acc_empty[a]), ((n / ACCS) & 1) ^ 1, abort_flag, kDevTimeoutAccEmpty);
                             if (!ok) break;
                             tc_fence_after();
                         }
@@ -241,7 +248,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         const int q = warp & 3, half = (warp - 2) >> 2;
         float* buf = epi + (warp - 2) * 32 * 20;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + half * HALF;
-        const uint32_t empty_bar[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
+        const uint32_t empty_bar = mapa_shared(smem_u32(acc_empty), 0);
         int n = 0;
         if (!SCALED && p.db_tiles > 0) {
             pdl_wait();
@@ -274,10 +281,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
 #pragma unroll 1
             for (int ch = 0; ch < chunks; ++ch, ++n) {
-                const int a = n & 1;
+                const int a = n % ACCS;
                 float scale = 1.f;
                 if (SCALED) scale = g0 + ch < p.groups ? __bfloat162float(sc[g0 + ch]) : 0.f;
-                if (!mbar_wait_cl(smem_u32(&acc_full[a]), (n >> 1) & 1, abort_flag, kDevTimeoutAccFull)) goto done;
+                if (!mbar_wait_short(smem_u32(&acc_full[a]), (n / ACCS) & 1, abort_flag, kDevTimeoutAccFull)) goto done;
                 __syncwarp();
                 tc_fence_after();
 #pragma unroll
@@ -288,7 +295,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     if (c == HALF / 16 - 1) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(empty_bar[a]);
+                        if (lane == 0) mbar_arrive_cluster(empty_bar + a * 8);
                     }
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -362,7 +369,7 @@ done:
     cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem_base, 2 * BN);
+        tmem_dealloc_pair(tmem_base, 512);
     }
 }
 
