@@ -181,8 +181,8 @@ unsigned grid_of(int64_t n, int64_t most) { return (unsigned)std::max<int64_t>(1
 // ------------------------------------- RMS norm ---------------------------------------
 
 // Pieces of 32 lanes x VEC features in the largest row held in registers.
-constexpr int64_t kFwdPieces = 32 * 8;
-constexpr int64_t bwd_pieces(bool vec) { return vec ? 32 * 4 : 32 * 8; }
+constexpr int64_t fwd_pieces(bool vec) { return vec ? 32 * 8 : 32 * 16; }
+constexpr int64_t bwd_pieces(bool vec) { return vec ? 32 * 4 : 32 * 16; }
 
 template <int VEC, int V, int WPR, int RPC>
 int launch_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
@@ -203,6 +203,7 @@ int run_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
     if (pieces <= 32) return launch_fwd<VEC, 4, 8, 1>(p, st);
     if (!few && pieces <= 64) return launch_fwd<VEC, 8, 8, 1>(p, st);
     if constexpr (VEC == 1) {
+        if (pieces > 256) return launch_fwd<1, 16, 32, 1>(p, st);
         if (!few) return pieces <= 128 ? launch_fwd<1, 8, 16, 1>(p, st) : launch_fwd<1, 16, 16, 1>(p, st);
     }
     if (pieces <= 128) return launch_fwd<VEC, 4, 32, 1>(p, st);
@@ -240,7 +241,8 @@ int with_bwd_variant(int64_t K, F&& f) {
     if (pieces <= 32) return f.template run<VEC, 2, 16, 1>();
     if (pieces <= 64) return f.template run<VEC, 4, 16, 1>();
     if constexpr (VEC == 4) return f.template run<4, 4, 32, 1>();
-    else return pieces <= 128 ? f.template run<1, 8, 16, 1>() : f.template run<1, 8, 32, 1>();
+    else if (pieces <= 128) return f.template run<1, 8, 16, 1>();
+    else return pieces <= 256 ? f.template run<1, 8, 32, 1>() : f.template run<1, 16, 32, 1>();
 }
 struct GroupsOf {
     int64_t rows, *out;
@@ -665,7 +667,7 @@ MT_API int mt_rms_norm(const mt_tensor* x, const mt_tensor* residual, const mt_t
                      (!q8 || ((reinterpret_cast<uintptr_t>(q.codes) & 3) == 0 && (M == 1 || q.cp % 4 == 0)));
     int rc;
     const bool unit = unit_cols(vx) && unit_cols(vr) && unit_cols(vg) && unit_cols(vh) && unit_cols(vy);
-    if (!unit || (K + 32 * (vec ? 4 : 1) - 1) / (32 * (vec ? 4 : 1)) > kFwdPieces) {
+    if (!unit || (K + 32 * (vec ? 4 : 1) - 1) / (32 * (vec ? 4 : 1)) > fwd_pieces(vec)) {
         mt::rms::fwd_long_kernel<<<grid_of(M, INT32_MAX), 32 * mt::rms::kLongWarps, 0, st>>>(p);
         rc = launched("rms_norm launch");
         if (rc == MT_OK) mt::host::set_path("rms_norm long rows");
