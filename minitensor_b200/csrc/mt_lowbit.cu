@@ -891,7 +891,7 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Few rows in integers, batches with the weights in tensor memory, prompts as a product of
     // unpacked operands. Microseconds on weights of 4096 x 16384 (group 64), either side: 8 rows
-    // 23 and 24, 12 rows 29 and 24; 192 rows 98 and 107, 256 rows 138 and 109.
+    // 23 and 24, 12 rows 29 and 24; 192 rows 96 and 109, 256 rows 138 and 109.
     if (M > 192 && w.K > 0) {
         switch (w.group) {   // k16-steps per group
             case 32: return linear_q4_planes<2>(vx, w, vb.m.p, vy.m, M, relu, st, who);
