@@ -22,15 +22,16 @@
 // stage, 3 stages. Warp 0 loads by TMA, warp 1 of the even CTA issues the MMAs, warps 2-9
 // drain: lane quarter = warp & 3, 128 columns each, 128 accumulators per thread. Products that
 // do not fill the GPU with such tiles take 256 x 128 ones, five stages and four accumulators
-// (777 x 1001 x 1303: 25.6 -> 18 us; large ones stay, since 64 values of k of such a tile, bound by
-// reads of shared memory, take about 1,000 cycles, and of a 256 x 256 tile 1,600). The tiles of a last round that would leave clusters idle are split over k between them; their parts
-// go to scratch and a second kernel adds them in order.
+// (777 x 1001 x 1303: 25.6 -> 18 us; large ones stay, since 64 values of k of such a tile, bound
+// by reads of shared memory, take about 1,000 cycles, and of a 256 x 256 tile 1,600). The tiles of
+// a last round that would leave clusters idle are split over k between them; their parts go to
+// scratch and a second kernel adds them in order.
 // Waits: what follows a wait here are copies and MMAs, or reads of tensor memory behind a
 // tcgen05 fence, and no thread's ordinary stores, so none needs an acquire at cluster scope, which
 // seems to cost the L1 with the scales in it at every chunk: groups of 32, 2048 x 4096 x 8192 379
 // against 337 us, 2048 x 5376 x 1536 168 against 128 us.
-// Bound: tensor pipe, 3 * 2 R C K operations: 8192^3 in 1956 us, 1686 TFLOP/s
-// of bfloat16 work, 1.01 of the measured cuBLAS rate (one launch; 2.25 ms in a row, under the power cap).
+// Bound: tensor pipe, 3 * 2 R C K operations: 8192^3 in 1956 us, 1686 TFLOP/s of bfloat16 work,
+// 1.01 of the measured cuBLAS rate (one launch; 2.25 ms in a row, under the power cap).
 // Three 64-deep stages, because 64 KB a stage leave room for no fourth; 256 x 256 tiles, because
 // a CTA alone on 128 x 256 would move 112 KB through shared memory in the time that bandwidth
 // has for 190 KB of reads and writes, of which the MMAs' reads alone are 144 KB.

@@ -373,6 +373,17 @@ def test_quantize_q4_is_exact(mt, group, K, N):
     assert torch.equal(qt.codes, q.codes) and torch.equal(qt.scales, q.scales)
 
 
+# Sizes that are cut in every way: tiles of 128 or 256 columns, at once, in parts, or the last
+# round in parts.
+@pytest.mark.parametrize("M,K,N,cut", [(130, 260, 200, "bn=128 whole=4 splits=1"), (1100, 70, 90, "bn=128 whole=0 splits=9"),
+                                       (300, 5000, 4100, "bn=256 whole=340 splits=1"), (700, 2100, 2300, "bn=256 whole=74 splits=6")])
+def test_linear_weight_grad_q8_cuts(mt, M, K, N, cut):
+    q, dy = wgrad_input(gen(M + K + N), M, K, N, "int8", mt)
+    got = mt.linear_weight_grad_q8(q, dy.cuda())
+    assert mt.engine.last_path().endswith(cut)
+    check_wgrad(q, dy, *got)
+
+
 def q4_case(g, M, K, N, group):
     codes = torch.randint(0, 16, (N, K), generator=g)
     s = (0.01 * torch.exp(rand(g, N, -(-K // group)))).to(torch.bfloat16)
@@ -413,6 +424,19 @@ def test_linear_forward_q4(mt, M, K, N, group):
     w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, group)
     y = mt.linear_forward_q4(x.cuda(), w, bias=bias.cuda() if bias is not None else None, relu=relu)
     check_q4(y, x, codes, s, group, bias, relu)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N,cut", [(200, 300, 300, "bn=128 whole=4 splits=1"), (500, 1300, 4800, "bn=128 whole=74 splits=11"),
+                                       (1030, 700, 2600, "bn=256 whole=55 splits=1"), (200, 4000, 4097, "bn=256 whole=0 splits=4")])
+def test_linear_forward_q4_cuts(mt, M, K, N, cut, group):
+    g = gen(M + K + N + group)
+    x, codes, s = q4_case(g, M, K, N, group)
+    bias = rand(g, N)
+    w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, group)
+    y = mt.linear_forward_q4(x.cuda(), w, bias=bias.cuda(), relu=True)
+    assert mt.engine.last_path().endswith(cut)
+    check_q4(y, x, codes, s, group, bias, True)
 
 
 @pytest.mark.parametrize("layout", LAYOUTS)
