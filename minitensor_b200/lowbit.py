@@ -261,9 +261,12 @@ def _need_2d(t, name):
 def _new_q8(rows, cols, fmt, d) -> Q8Tensor:
     if fmt not in Q8_FORMATS:
         raise ValueError(f"8-bit format must be one of {tuple(Q8_FORMATS)}, got {fmt!r}")
-    device = _device(d)
-    return Q8Tensor(torch.empty((rows, cols), dtype=_Q8_STORAGE[fmt], device=device),
-                    torch.empty((rows, -(-cols // Q8_BLOCK)), dtype=torch.uint8, device=device))
+    device, blocks = _device(d), -(-cols // Q8_BLOCK)
+    q = Q8Tensor.__new__(Q8Tensor)      # dense and new: nothing for the constructor to check
+    q.codes = codes = torch.empty((rows, cols), dtype=_Q8_STORAGE[fmt], device=device)
+    q.scales = scales = torch.empty((rows, blocks), dtype=torch.uint8, device=device)
+    q._c = MtQ8(codes.data_ptr(), scales.data_ptr(), rows, cols, cols, blocks, Q8_FORMATS[fmt])
+    return q
 
 
 # ---- RMS norm ---------------------------------------------------------------------------
