@@ -62,7 +62,7 @@ def norm_bound(K):
 
 SHAPES = [(1, 1), (1, 4096), (3, 5), (5, 32), (2, 33), (7, 100), (9, 128), (300, 127), (4, 512), (130, 516), (3, 1000),
           (3, 1024), (2, 1025), (5, 4100), (320, 1028), (2, 4097), (2, 8191), (3, 16384), (2, 20000), (1, 32768), (2, 8193),
-          (2, 40004), (1, 70001)]
+          (320, 12289), (2, 16383), (2, 16385), (2, 40004), (1, 70001)]
 
 
 @pytest.mark.parametrize("rows,K", SHAPES)
