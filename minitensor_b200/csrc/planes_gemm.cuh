@@ -196,6 +196,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
             }
+            // The last releases of the stages: they are committed behind the accumulator that ends the
+            // drains' work, and those of the odd CTA come from its peer. None may arrive in shared
+            // memory that the CTA has left.
+            for (int i = 0; i < STAGES; ++i) {
+                if (!mbar_wait_short(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) goto done;
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+            }
         }
     } else if (warp == 1) {
         if (leader && elect_one()) {

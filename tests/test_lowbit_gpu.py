@@ -718,3 +718,19 @@ def test_offsets_beyond_32_bits(mt):
     assert torch.equal(mt.dequantize_q8(far_q), mt.dequantize_q8(q))
     a, b = mt.linear_weight_grad_q8(far_q, dY.cuda()), mt.linear_weight_grad_q8(q, dY.cuda())
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# ---- kernels that end with releases on their way -----------------------------------------
+
+def test_weight_grad_one_call_behind_the_other(mt):
+    """Whole tiles, split tiles and short sums in turn, each kernel's shared memory taken over by the
+    next: equal bits every time and no wait that ran out. (The stages' last releases are waited for
+    before a CTA leaves; one that arrived later would write to the next kernel's shared memory.)"""
+    g = gen(31)
+    cases = [wgrad_input(g, M, K, N, "int8", mt) for M, K, N in ((16, 64, 64), (300, 1300, 2300), (5000, 40, 70), (65, 520, 600))]
+    cases = [(q, dy.cuda()) for q, dy in cases]
+    want = [mt.linear_weight_grad_q8(q, dy) for q, dy in cases]
+    got = [[mt.linear_weight_grad_q8(q, dy) for q, dy in cases] for _ in range(30)]
+    for turn in got:
+        assert all(torch.equal(a, c) and torch.equal(b, d) for (a, b), (c, d) in zip(turn, want))
+    assert mt.engine.device_status() == 0
