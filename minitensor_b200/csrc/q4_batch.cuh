@@ -209,6 +209,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
                 step(x);
                 if (++s == C::STAGES) { s = 0; ph ^= 1; }
             }
+            // The last releases of the stages are committed behind the accumulators that end the drains'
+            // work, and must not arrive in shared memory that the CTA has left.
+            for (int i = 0; i < C::STAGES; ++i) {
+                if (!mbar_wait_short(smem_u32(&empty[s]), ph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
+                if (++s == C::STAGES) { s = 0; ph ^= 1; }
+            }
         }
     } else if (warp <= 2) {
         const int half = __shfl_sync(0xffffffffu, warp, 0) - 1;
@@ -274,6 +280,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(a_bar + ab * 8);
+            if (++ab == C::A_STAGES) { ab = 0; aph ^= 1; }
+        }
+        for (int i = 0; i < C::A_STAGES; ++i) {   // as for the stages, those of the unpacked steps
+            if (!mbar_wait_short(a_bar + (2 * C::A_STAGES + ab) * 8, aph ^ 1, abort_flag, kDevTimeoutEmpty)) break;
             if (++ab == C::A_STAGES) { ab = 0; aph ^= 1; }
         }
     } else if (warp >= 12) {

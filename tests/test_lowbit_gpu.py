@@ -734,3 +734,17 @@ def test_weight_grad_one_call_behind_the_other(mt):
     for turn in got:
         assert all(torch.equal(a, c) and torch.equal(b, d) for (a, b), (c, d) in zip(turn, want))
     assert mt.engine.device_status() == 0
+
+
+def test_batches_of_4_bit_products_one_call_behind_the_other(mt):
+    """The same for batches: runs over cut tiles, whole tiles, and runs shorter than the ring."""
+    g = gen(32)
+    cases = []
+    for M, K, N, group in ((9, 128, 16, 32), (21, 1111, 401, 32), (40, 4096, 2048, 64), (64, 512, 20000, 128), (150, 260, 300, 64)):
+        x, codes, s = q4_case(g, M, K, N, group)
+        cases.append((x.cuda(), mt.Q4Weight(pack_fast(codes, K).cuda(), s.cuda(), K, group)))
+    want = [mt.linear_forward_q4(x, w) for x, w in cases]
+    got = [[mt.linear_forward_q4(x, w) for x, w in cases] for _ in range(30)]
+    for turn in got:
+        assert all(torch.equal(a, b) for a, b in zip(turn, want))
+    assert mt.engine.device_status() == 0
