@@ -574,41 +574,45 @@ int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, c
         ++chunks;
         rows = (M + chunks - 1) / chunks;
     }
-    if (chunks > 65535) return fail(MT_EUNSUPPORTED, "%s: too many rows", who);
     const int nt = (int)(rows + 1) / 2;
     int64_t most = std::max<int64_t>(1, spans);
     while (most > 1 && gemv_smem(nt, (int)most) > kMaxSmem) most = (most + 1) / 2;
     const int sms = mt::host::sm_count();
     const int64_t ctas = std::max<int64_t>(1, sms / chunks);
     Gemv p{};
-    p.x = x.m;
     p.w = w;
     p.bias = bias;
-    p.y = y;
-    p.M = M;
     p.rows = (int)rows;
     p.relu = relu;
     const int64_t tiles = (w.N + 15) / 16;
-    const dim3 grid(grid_of(tiles, ctas), (unsigned)chunks);
+    dim3 grid(grid_of(tiles, ctas));
     p.tiles_each = (int)(tiles / grid.x);
     p.tiles_more = (int)(tiles % grid.x);
     p.xvec = vec4(x);
     const int64_t launches = spans ? (spans + most - 1) / most : 1;   // no inputs: the bias alone
-    for (int64_t i = 0; i < launches; ++i) {
-        const int64_t s0 = i * most;
-        p.span0 = (int)s0;
-        p.spans = (int)std::min(most, spans - s0);
-        p.accumulate = i > 0;
-        p.finish = i == launches - 1;
-        switch (nt) {
-            case 1: MT_TRY(launch_gemv<1>(p, grid, st, who)); break;
-            case 2: MT_TRY(launch_gemv<2>(p, grid, st, who)); break;
-            case 3: MT_TRY(launch_gemv<3>(p, grid, st, who)); break;
-            case 4: MT_TRY(launch_gemv<4>(p, grid, st, who)); break;
-            case 5: MT_TRY(launch_gemv<5>(p, grid, st, who)); break;
-            case 6: MT_TRY(launch_gemv<6>(p, grid, st, who)); break;
-            case 7: MT_TRY(launch_gemv<7>(p, grid, st, who)); break;
-            default: MT_TRY(launch_gemv<8>(p, grid, st, who)); break;
+    // Without inputs there may be more rows than a grid has chunks.
+    for (int64_t c0 = 0; c0 < chunks; c0 += 65535) {
+        const int64_t m0 = c0 * rows;
+        grid.y = (unsigned)std::min<int64_t>(65535, chunks - c0);
+        p.x = Mat{x.m.p + m0 * x.m.rs, x.m.rs, x.m.cs};
+        p.y = Mat{y.p + m0 * y.rs, y.rs, y.cs};
+        p.M = M - m0;
+        for (int64_t i = 0; i < launches; ++i) {
+            const int64_t s0 = i * most;
+            p.span0 = (int)s0;
+            p.spans = (int)std::min(most, spans - s0);
+            p.accumulate = i > 0;
+            p.finish = i == launches - 1;
+            switch (nt) {
+                case 1: MT_TRY(launch_gemv<1>(p, grid, st, who)); break;
+                case 2: MT_TRY(launch_gemv<2>(p, grid, st, who)); break;
+                case 3: MT_TRY(launch_gemv<3>(p, grid, st, who)); break;
+                case 4: MT_TRY(launch_gemv<4>(p, grid, st, who)); break;
+                case 5: MT_TRY(launch_gemv<5>(p, grid, st, who)); break;
+                case 6: MT_TRY(launch_gemv<6>(p, grid, st, who)); break;
+                case 7: MT_TRY(launch_gemv<7>(p, grid, st, who)); break;
+                default: MT_TRY(launch_gemv<8>(p, grid, st, who)); break;
+            }
         }
     }
     char path[96];

@@ -231,3 +231,12 @@ def test_valid_calls_without_a_gpu_end_in_an_error():
                  lambda: mt.rms_norm_backward(t(3, 64), t(3, 64), t(64), t(3))):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_linear_q4_without_inputs_takes_any_number_of_rows():
+    """The bias alone, on more rows than a grid has chunks: not refused (without a GPU it ends at
+    the launch)."""
+    if torch.cuda.is_available():
+        pytest.skip("needs a machine without a GPU")
+    with pytest.raises(RuntimeError, match="launch|no kernel|driver|device"):
+        mt.linear_forward_q4(t(1100000, 0), q4(0, 3), bias=t(3))

@@ -748,3 +748,10 @@ def test_batches_of_4_bit_products_one_call_behind_the_other(mt):
     for turn in got:
         assert all(torch.equal(a, b) for a, b in zip(turn, want))
     assert mt.engine.device_status() == 0
+
+
+def test_linear_forward_q4_without_inputs_takes_any_number_of_rows(mt):
+    none = mt.quantize_q4(torch.empty(0, 3, device="cuda"))
+    bias = torch.randn(3, device="cuda")
+    y = mt.linear_forward_q4(torch.empty(1100000, 0, device="cuda"), none, bias=bias, relu=True)
+    assert torch.equal(y, bias.clamp_min(0).expand(1100000, 3))
