@@ -562,21 +562,31 @@ int launch_gemv(const mt::q4::Gemv& p, dim3 grid, cudaStream_t st, const char* w
     }
 }
 
+// Rows per CTA: as many as 4, but rather 2 (their CTAs read the weights again, from L2) than K in
+// several launches of at most `most` spans.
+struct GemvPlan {
+    int64_t chunks, rows, most, launches;
+};
+GemvPlan plan_gemv(int64_t M, int64_t spans) {
+    using namespace mt::q4;
+    GemvPlan g;
+    g.chunks = (M + kGemvMaxRows - 1) / kGemvMaxRows;
+    g.rows = (M + g.chunks - 1) / g.chunks;
+    while (g.rows > 2 && gemv_smem((int)g.rows, (int)spans) > kMaxSmem) {
+        ++g.chunks;
+        g.rows = (M + g.chunks - 1) / g.chunks;
+    }
+    g.most = std::max<int64_t>(1, spans);
+    while (g.most > 1 && gemv_smem((int)g.rows, (int)g.most) > kMaxSmem) g.most = (g.most + 1) / 2;
+    g.launches = spans ? (spans + g.most - 1) / g.most : 1;   // no inputs: the bias alone
+    return g;
+}
+
 int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, const Mat& y, int64_t M, int relu,
                    cudaStream_t st, const char* who) {
     using namespace mt::q4;
     const int64_t spans = (w.K + kSpan - 1) / kSpan;
-    // Rows per CTA: as many as 16, but rather fewer (their CTAs read the weights again, from
-    // L2) than K in several launches, down to 4.
-    int64_t chunks = (M + 2 * kGemvMaxTiles - 1) / (2 * kGemvMaxTiles);
-    int64_t rows = (M + chunks - 1) / chunks;
-    while (rows > 4 && gemv_smem((int)(rows + 1) / 2, (int)spans) > kMaxSmem) {
-        ++chunks;
-        rows = (M + chunks - 1) / chunks;
-    }
-    const int nt = (int)(rows + 1) / 2;
-    int64_t most = std::max<int64_t>(1, spans);
-    while (most > 1 && gemv_smem(nt, (int)most) > kMaxSmem) most = (most + 1) / 2;
+    const auto [chunks, rows, most, launches] = plan_gemv(M, spans);
     const int sms = mt::host::sm_count();
     const int64_t ctas = std::max<int64_t>(1, sms / chunks);
     Gemv p{};
@@ -589,7 +599,6 @@ int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, c
     p.tiles_each = (int)(tiles / grid.x);
     p.tiles_more = (int)(tiles % grid.x);
     p.xvec = vec4(x);
-    const int64_t launches = spans ? (spans + most - 1) / most : 1;   // no inputs: the bias alone
     // Without inputs there may be more rows than a grid has chunks.
     for (int64_t c0 = 0; c0 < chunks; c0 += 65535) {
         const int64_t m0 = c0 * rows;
@@ -603,15 +612,11 @@ int linear_q4_gemv(const View2& x, const mt::q4::Weight& w, const float* bias, c
             p.spans = (int)std::min(most, spans - s0);
             p.accumulate = i > 0;
             p.finish = i == launches - 1;
-            switch (nt) {
+            switch (rows) {
                 case 1: MT_TRY(launch_gemv<1>(p, grid, st, who)); break;
                 case 2: MT_TRY(launch_gemv<2>(p, grid, st, who)); break;
                 case 3: MT_TRY(launch_gemv<3>(p, grid, st, who)); break;
-                case 4: MT_TRY(launch_gemv<4>(p, grid, st, who)); break;
-                case 5: MT_TRY(launch_gemv<5>(p, grid, st, who)); break;
-                case 6: MT_TRY(launch_gemv<6>(p, grid, st, who)); break;
-                case 7: MT_TRY(launch_gemv<7>(p, grid, st, who)); break;
-                default: MT_TRY(launch_gemv<8>(p, grid, st, who)); break;
+                default: MT_TRY(launch_gemv<4>(p, grid, st, who)); break;
             }
         }
     }
@@ -894,8 +899,10 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     if (M * w.N == 0) return MT_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Few rows in integers, batches with the weights in tensor memory, prompts as a product of
-    // unpacked operands. Microseconds on weights of 4096 x 16384 (group 64), either side: 8 rows
-    // 23 and 24, 12 rows 29 and 24; 192 rows 96 and 109, 256 rows 138 and 109.
+    // unpacked operands. Microseconds, either side: 192 rows on weights of 4096 x 16384 (group 64) 96
+    // and 109, 256 rows 138 and 109; 4 rows there 27 and 31, 5 rows 35 and 31. In two launches: 1 row on
+    // 20000 x 16384 63 and 86, 2 rows on 16384 x 4096 36 and 31, but 56 and 101 on 12000 x 16384 in
+    // groups of 32, which cost a batch twice the drains. In three: 1 row on 30000 x 4096 58 and 45.
     if (M > 192 && w.K > 0) {
         switch (w.group) {   // k16-steps per group
             case 32: return linear_q4_planes<2>(vx, w, vb.m.p, vy.m, M, relu, st, who);
@@ -903,7 +910,9 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
             default: return linear_q4_planes<8>(vx, w, vb.m.p, vy.m, M, relu, st, who);
         }
     }
-    if (M > 8 && w.K > 0) return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
+    const int64_t spans = (w.K + mt::q4::kSpan - 1) / mt::q4::kSpan;
+    if (w.K > 0 && (M > mt::q4::kGemvMaxRows || plan_gemv(M, spans).launches > (M == 1 || w.group == 32 ? 2 : 1)))
+        return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
     return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
 }
 

@@ -77,6 +77,20 @@ def q4_weight(codes, scales, group):
     return ((codes - 8).double() * scales.double().repeat_interleave(group, 1)[:, :K]).t()
 
 
+def q4_bound(M, K, group):
+    """What y = x W may be off in u times |x| |W|, W in 4 bits: relative to what each entry of x adds
+    itself, as for a float product, whatever the entries beside it are.
+
+    Up to 8 rows: the signed digits of an entry add up to 9 times it at most (a digit pair to 3.02 times
+    its number, the second number of an entry to half a step of the first, 0.5 to 1 times the
+    entry), and every part meets a conversion, a product with the scale, the sums over the groups,
+    over four lanes, 16 warps, 5 passes and K / 1024 launches, and the bias. More rows: a tensor-core step
+    aligns 17 terms to the largest and drops up to 2 u of it from each, 3 * group / 16 steps meet in
+    an accumulator, then come the scale, the sum over the groups and 64 parts, and the bias."""
+    few = 9 * (31 + K / group + K / 1024)
+    return max(few, 102 * group / 16 + K / group + 70) if M <= 8 else 102 * group / 16 + K / group + 70
+
+
 def rms_norm(x, residual, gamma, eps):
     h = x.double() + (residual.double() if residual is not None else 0)
     rstd = 1 / torch.sqrt((h * h).mean(1) + eps)

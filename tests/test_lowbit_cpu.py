@@ -80,6 +80,34 @@ def test_bounds_catch_planted_mistakes():
     assert R.worst(X[:299].double().t() @ DY[:299].double() - W, mag) > 308
 
 
+def digit_values(x, sets):
+    """x [K] as the sum of `sets` fixed-point numbers of steps 2^(e - 29 - 31 j), 2^e the largest entry's
+    power of two, in 64 bits where each number and its remainder are exact."""
+    e = torch.floor(torch.log2(x.abs().max().double()))
+    v, total = x.double() * 2.0 ** (29 - e), torch.zeros_like(x, dtype=torch.float64)
+    for j in range(sets):
+        X = torch.round(v)
+        assert X.abs().max() <= 2 ** 30
+        total += X * 2.0 ** (e - 29 - 31 * j)
+        v = (v - X) * 2.0 ** 31
+    return total
+
+
+def test_bounds_catch_an_entry_lost_beside_a_large_one():
+    """One fixed-point number for a span drops what lies far below its largest entry; that is beyond
+    q4_bound, which holds an error against |x| |W|. A second number reaches 2^37 below."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(128, generator=g)
+    W = torch.randint(-8, 8, (128, 40), generator=g).double()
+    W[::16] = 0
+    for top in (20, 35):
+        y = x.clone()
+        y[::16] = 2.0 ** top
+        assert R.worst((digit_values(y, 1) - y.double()) @ W, y.double().abs() @ W.abs()) > R.q4_bound(1, 128, 32)
+        near = y.abs() >= 2.0 ** (top - 36)
+        assert torch.equal(digit_values(y, 2)[near], y.double()[near])
+
+
 # ---- refusals ---------------------------------------------------------------------------
 
 def test_rms_norm_refusals():

@@ -755,3 +755,56 @@ def test_linear_forward_q4_without_inputs_takes_any_number_of_rows(mt):
     bias = torch.randn(3, device="cuda")
     y = mt.linear_forward_q4(torch.empty(1100000, 0, device="cuda"), none, bias=bias, relu=True)
     assert torch.equal(y, bias.clamp_min(0).expand(1100000, 3))
+
+# ---- 4 bits: entries of x of every size beside each other ---------------------------------
+
+def ladder(g, M, K, N, group, low, high):
+    """x whose entries' exponents are spread over [low, high], and weights that are 0 (code 8) in
+    output n for every entry above the n-th of N thresholds: y[:, n] is a sum of the entries below."""
+    e = torch.randint(low, high + 1, (M, K), generator=g)
+    e[:, 0] = high
+    x = torch.ldexp((torch.rand(M, K, generator=g) + 1) * torch.where(torch.rand(M, K, generator=g) < 0.5, -1.0, 1.0), e)
+    codes = torch.randint(0, 16, (N, K), generator=g)
+    limit = low + (high - low) * (torch.arange(N) + 1) // N
+    codes[(e.amax(0)[None, :] > limit[:, None])] = 8
+    s = (0.01 * torch.exp(rand(g, N, -(-K // group)))).to(torch.bfloat16)
+    return x, codes, s
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8, 9, 40, 200])
+@pytest.mark.parametrize("low,high", [(-14, 0), (-35, 10), (-40, 40), (-60, 120), (-85, 125)])
+@pytest.mark.parametrize("K,group", [(128, 32), (1000, 64), (4100, 128)])
+def test_linear_forward_q4_small_entries_beside_large_ones(mt, M, low, high, K, group):
+    """The error is held against |x| |W| alone: a large entry that meets weight 0 is no excuse."""
+    g = gen(M + K + high)
+    x, codes, s = ladder(g, M, K, 40, group, low, high)
+    w = mt.Q4Weight(pack_fast(codes, K).cuda(), s.cuda(), K, group)
+    W = R.q4_weight(codes, s, group)
+    err = host(mt.linear_forward_q4(x.cuda(), w)).double() - x.double() @ W
+    assert R.worst(err, x.double().abs() @ W.abs()) <= R.q4_bound(M, K, group)
+
+
+def test_linear_forward_q4_one_large_entry_on_a_zero_weight(mt):
+    """One entry of 1e12 on weight 0 beside 127 ones: the ones are the result, at any number of rows."""
+    codes = torch.full((16, 128), 9, dtype=torch.int64)
+    codes[:, 0] = 8
+    w = mt.Q4Weight(R.q4_pack(codes, 128).cuda(), torch.ones(16, 1, dtype=torch.bfloat16, device="cuda"), 128, 128)
+    for M in (1, 2, 4, 7, 8, 9, 200):
+        x = torch.ones(M, 128, device="cuda")
+        x[:, 0] = 1e12
+        assert torch.equal(host(mt.linear_forward_q4(x, w)), torch.full((M, 16), 127.0))
+
+
+@pytest.mark.parametrize("M", [1, 4, 8])
+def test_linear_forward_q4_spread_entries_in_long_rows(mt, M):
+    """Several launches over K, several passes over the digits, bias and ReLU at the end of both."""
+    g, N = gen(M), 24
+    K = 20000 if M == 1 else 14000
+    x, codes, s = ladder(g, M, K, N, 32, -60, 60)
+    bias = rand(g, N) * 2.0 ** 40
+    w = mt.Q4Weight(pack_fast(codes, K).cuda(), s.cuda(), K, 32)
+    y = host(mt.linear_forward_q4(x.cuda(), w, bias=bias.cuda(), relu=True)).double()
+    assert "gemv" in mt.engine.last_path() or M > 4
+    W = R.q4_weight(codes, s, 32)
+    want, mag = x.double() @ W + bias.double(), x.double().abs() @ W.abs() + bias.double().abs()
+    assert R.worst(y - want.clamp_min(0), mag) <= R.q4_bound(M, K, 32)
