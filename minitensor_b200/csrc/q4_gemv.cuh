@@ -187,7 +187,9 @@ __device__ __forceinline__ int gemv_stage_x(const Gemv& p, uint8_t* xs, float* f
                     *reinterpret_cast<uint32_t*>(o + 3 * (size_t)col_bytes) = __byte_perm(h0, h1, 0x7632);
                     o += 4 * (size_t)col_bytes;
                 }
-                if (lane == 0) fs[r * (spans + 1) + s] = __uint_as_float((uint32_t)max(e - 33 - 62 * max(pass - 1, 0), 1) << 23);
+                // 2^14 times the span's unit: sums in the unit itself would fall below a float's normal
+                // numbers where y does not, and with 2^16 the low digits' could overflow first.
+                if (lane == 0) fs[r * (spans + 1) + s] = __uint_as_float((uint32_t)max(e - 19 - 62 * max(pass - 1, 0), 1) << 23);
             }
         }
     }
@@ -317,8 +319,9 @@ __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
                 for (int i = 0; i < NT; ++i) tot[i][0] = tot[i][1] = 0.f;
                 const uint8_t* xl = xs + (size_t)g * col_bytes + t * 32;
                 const uint4* w = ring;
-                // A lane's digits: 2^16 for the high ones, 2^-31 for the second number, 2^-62 for later passes.
-                const float weight = (t & 1 ? 65536.f : 1.f) * (t & 2 ? 0x1p-31f : 1.f) * (pass ? 0x1p-62f : 1.f);
+                // A lane's digits: 2^16 for the high ones, 2^-31 for the second number, 2^-62 for later passes;
+                // and 2^-14 for what the spans' powers of two have too much.
+                const float weight = (t & 1 ? 4.f : 0x1p-14f) * (t & 2 ? 0x1p-31f : 1.f) * (pass ? 0x1p-62f : 1.f);
 #pragma unroll 1
                 for (int i = lo; i < hi; ++i) {
                     uint16_t ca[SEG], cb[SEG];

@@ -808,3 +808,21 @@ def test_linear_forward_q4_spread_entries_in_long_rows(mt, M):
     W = R.q4_weight(codes, s, 32)
     want, mag = x.double() @ W + bias.double(), x.double().abs() @ W.abs() + bias.double().abs()
     assert R.worst(y - want.clamp_min(0), mag) <= R.q4_bound(M, K, 32)
+
+
+@pytest.mark.parametrize("e,scale", [(-90, 0), (-118, 0), (-130, 0), (-60, -60), (-40, -80), (-20, -104)])
+def test_linear_forward_q4_tiny_results(mt, e, scale):
+    """Rows of x with a single value, y = s * (c - 8) * x down to a float's smallest numbers, by a tiny x
+    or a tiny s: at most six roundings (a conversion, the scale's product and the sum of four lanes,
+    once per number), where y is not a normal number each of them to a multiple of 2^-147 at worst."""
+    M, K, N, group = 4, 160, 40, 32
+    g = gen(-e)
+    x = torch.zeros(M, K)
+    x[torch.arange(M), torch.tensor([3, 60, 101, 159])] = torch.ldexp(torch.rand(M, generator=g) + 1, torch.tensor(e))
+    codes = torch.randint(0, 16, (N, K), generator=g)
+    s = torch.ldexp(1 + torch.rand(N, K // group, generator=g), torch.tensor(scale)).to(torch.bfloat16)
+    w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, group)
+    want = x.double() @ R.q4_weight(codes, s, group)
+    for rows in (1, 4):
+        err = (host(mt.linear_forward_q4(x[:rows].cuda(), w)).double() - want[:rows]).abs()
+        assert R.worst((err - 6 * 2.0 ** -148).clamp_min(0), want[:rows]) <= 7
