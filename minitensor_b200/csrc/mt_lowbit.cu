@@ -720,7 +720,8 @@ MT_API int mt_rms_norm_backward(const mt_tensor* dy, const mt_tensor* h, const m
     const bool is_long = !unit || (K + 32 * (vec ? 4 : 1) - 1) / (32 * (vec ? 4 : 1)) > bwd_pieces(vec);
     int64_t groups = 0;
     if (is_long) {
-        groups = std::min<int64_t>(M, std::max<int64_t>(1, 8LL * mt::host::sm_count() * 256 / K));
+        // blockIdx.y of the partial sums' kernel, of which a grid has 65,535.
+        groups = std::min<int64_t>({M, 65535, std::max<int64_t>(1, 8LL * mt::host::sm_count() * 256 / K)});
     } else {
         MT_TRY(vec ? with_bwd_variant<4>(K, GroupsOf{M, &groups}) : with_bwd_variant<1>(K, GroupsOf{M, &groups}));
     }

@@ -826,3 +826,25 @@ def test_linear_forward_q4_tiny_results(mt, e, scale):
     for rows in (1, 4):
         err = (host(mt.linear_forward_q4(x[:rows].cuda(), w)).double() - want[:rows]).abs()
         assert R.worst((err - 6 * 2.0 ** -148).clamp_min(0), want[:rows]) <= 7
+
+
+@pytest.mark.parametrize("K", [2, 3, 4, 5])
+@pytest.mark.parametrize("how", ["dy transposed", "gamma strided", "gamma broadcast"])
+def test_rms_norm_backward_many_short_strided_rows(mt, K, how):
+    """More row groups than a grid has in y."""
+    rows, g = 160000, gen(K)
+    h, gamma, dy = rand(g, rows, K, scale=2.0), 1 + rand(g, K, scale=0.1), rand(g, rows, K)
+    rstd = (1 / torch.sqrt((h.double() ** 2).mean(1) + 1e-6)).float()
+    dyd, gd = dy.cuda(), gamma.cuda()
+    if how == "dy transposed":
+        dyd = strided(dy, "transposed")
+    elif how == "gamma strided":
+        gd = gamma.repeat_interleave(2).cuda()[::2]
+    else:
+        gamma = gamma[:1].expand(K)
+        gd = gamma[:1].cuda().expand(K)
+    dx, dgamma = mt.rms_norm_backward(dyd, h.cuda(), gd, rstd.cuda())
+    want, mag, want_g, mag_g = R.rms_norm_backward(dy, h, gamma, rstd, None)
+    assert R.worst(host(dx) - want, mag) <= 50
+    assert R.worst(host(dgamma) - want_g, mag_g) <= rows + 3
+    assert torch.equal(mt.rms_norm_backward(dyd, h.cuda(), gd, rstd.cuda(), need_dgamma=False)[0], dx)
