@@ -213,16 +213,19 @@ int run_fwd(const mt::rms::Fwd& p, cudaStream_t st) {
 // Row groups whose dgamma partials are kept; the launch has one per CTA (or warp, RPC > 1).
 template <int VEC, int V, int WPR, int RPC>
 int64_t bwd_groups(int64_t rows) {
-    // As many CTAs as are resident at once.
-    static std::atomic<int> resident{0};
-    int per_sm = resident.load();
+    // As many CTAs as are resident at once, asked once per device.
+    static std::atomic<int> resident[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int per_sm = resident[dev & 63].load();
     if (per_sm == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, mt::rms::bwd_kernel<VEC, V, WPR, RPC>, 32 * WPR * RPC, 0) !=
-                cudaSuccess || per_sm < 1) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, mt::rms::bwd_kernel<VEC, V, WPR, RPC>, 32 * WPR * RPC, 0) ==
+                cudaSuccess && per_sm > 0) {
+            resident[dev & 63].store(per_sm);
+        } else {
             cudaGetLastError();
             per_sm = 1;
         }
-        resident.store(per_sm);
     }
     const int64_t ctas = std::min<int64_t>((rows + RPC - 1) / RPC, (int64_t)mt::host::sm_count() * per_sm);
     return ctas * RPC;
