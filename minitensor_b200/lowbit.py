@@ -74,10 +74,27 @@ def _lowbit_lib():
 
 # ---- operands ---------------------------------------------------------------------------
 
-class Q8Tensor:
+class _Held:
+    """Tensors with the C struct that points into their memory: no attribute can be set again,
+    since the struct would go on pointing to the memory of the tensor before."""
+
+    __slots__ = ()
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{type(self).__name__}.{name} cannot be set: make a new {type(self).__name__}")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{type(self).__name__}.{name} cannot be deleted")
+
+
+_put = object.__setattr__
+
+
+class Q8Tensor(_Held):
     """A [rows, cols] tensor in 8 bits. ``codes`` (int8 or float8_e4m3fn) [rows, cols] and
     ``scales`` (uint8) [rows, ceil(cols / 32)], both with unit column stride: the code c of
-    a block of 32 columns with scale byte b stands for c * 2^(b - 127); b = 255 is NaN."""
+    a block of 32 columns with scale byte b stands for c * 2^(b - 127); b = 255 is NaN. What the
+    tensors hold may be changed in place, the tensors not."""
 
     __slots__ = ("codes", "scales", "_c")
 
@@ -98,10 +115,11 @@ class Q8Tensor:
                 raise ValueError(f"{name} must not have overlapping or broadcast rows")
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on the same device")
-        self.codes, self.scales = codes, scales
+        _put(self, "codes", codes)
+        _put(self, "scales", scales)
         # A [n, 1] view may have any column stride; its row stride still is the pitch.
-        self._c = MtQ8(codes.data_ptr(), scales.data_ptr(), rows, cols, max(codes.stride(0), cols),
-                       max(scales.stride(0), scales.shape[1]), Q8_FORMATS[_Q8_DTYPES[codes.dtype]])
+        _put(self, "_c", MtQ8(codes.data_ptr(), scales.data_ptr(), rows, cols, max(codes.stride(0), cols),
+                              max(scales.stride(0), scales.shape[1]), Q8_FORMATS[_Q8_DTYPES[codes.dtype]]))
 
     @property
     def shape(self):
@@ -119,10 +137,11 @@ class Q8Tensor:
         return _Q8_DTYPES[self.codes.dtype]
 
 
-class Q4Weight:
+class Q4Weight(_Held):
     """A Linear weight [in_features, out_features] in 4 bits: ``codes`` (uint8)
     [out, 64 * ceil(in / 128)] and ``scales`` (bfloat16) [out, ceil(in / group)], rows =
-    output features. include/mtgemm.h (mt_q4) has the order of the codes in a row."""
+    output features. include/mtgemm.h (mt_q4) has the order of the codes in a row. What the
+    tensors hold may be changed in place, the tensors not."""
 
     __slots__ = ("codes", "scales", "in_features", "group", "_c")
 
@@ -147,10 +166,11 @@ class Q4Weight:
                 raise ValueError(f"{name} must not have overlapping or broadcast rows")
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on the same device")
-        self.codes, self.scales, self.in_features, self.group = codes, scales, in_features, group
         pitch = codes.stride(0) if out > 1 else want_c
-        self._c = MtQ4(codes.data_ptr(), scales.data_ptr(), in_features, out, group, pitch,
-                       max(scales.stride(0), want_s))
+        for name, value in (("codes", codes), ("scales", scales), ("in_features", in_features), ("group", group),
+                            ("_c", MtQ4(codes.data_ptr(), scales.data_ptr(), in_features, out, group, pitch,
+                                        max(scales.stride(0), want_s)))):
+            _put(self, name, value)
 
     @property
     def out_features(self) -> int:
@@ -263,9 +283,11 @@ def _new_q8(rows, cols, fmt, d) -> Q8Tensor:
         raise ValueError(f"8-bit format must be one of {tuple(Q8_FORMATS)}, got {fmt!r}")
     device, blocks = _device(d), -(-cols // Q8_BLOCK)
     q = Q8Tensor.__new__(Q8Tensor)      # dense and new: nothing for the constructor to check
-    q.codes = codes = torch.empty((rows, cols), dtype=_Q8_STORAGE[fmt], device=device)
-    q.scales = scales = torch.empty((rows, blocks), dtype=torch.uint8, device=device)
-    q._c = MtQ8(codes.data_ptr(), scales.data_ptr(), rows, cols, cols, blocks, Q8_FORMATS[fmt])
+    codes = torch.empty((rows, cols), dtype=_Q8_STORAGE[fmt], device=device)
+    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=device)
+    _put(q, "codes", codes)
+    _put(q, "scales", scales)
+    _put(q, "_c", MtQ8(codes.data_ptr(), scales.data_ptr(), rows, cols, cols, blocks, Q8_FORMATS[fmt]))
     return q
 
 

@@ -268,3 +268,17 @@ def test_linear_q4_without_inputs_takes_any_number_of_rows():
         pytest.skip("needs a machine without a GPU")
     with pytest.raises(RuntimeError, match="launch|no kernel|driver|device"):
         mt.linear_forward_q4(t(1100000, 0), q4(0, 3), bias=t(3))
+
+
+def test_operands_cannot_be_given_other_tensors():
+    """The library reads the memory of the tensors that an operand was made of; one set later would
+    not be it (and the first could be freed)."""
+    for v, names in ((q8(2, 40), ("codes", "scales", "_c")), (q4(100, 8), ("codes", "scales", "in_features", "group", "_c"))):
+        before = [getattr(v, n) for n in names]
+        for n in names:
+            with pytest.raises(AttributeError):
+                setattr(v, n, getattr(v, n))
+            with pytest.raises(AttributeError):
+                delattr(v, n)
+        assert all(getattr(v, n) is b for n, b in zip(names, before))
+        assert (v._c.codes, v._c.scales) == (v.codes.data_ptr(), v.scales.data_ptr())
