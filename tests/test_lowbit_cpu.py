@@ -80,6 +80,18 @@ def test_bounds_catch_planted_mistakes():
     assert R.worst(X[:299].double().t() @ DY[:299].double() - W, mag) > 308
 
 
+def test_bounds_of_single_terms_catch_a_lost_third_part():
+    """Without its third part most floats are beyond the bounds for sums of one term, whatever the other
+    operand; sums of many terms hide it."""
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(4000, generator=g) * torch.exp(5 * torch.randn(4000, generator=g))
+    high = (x.view(torch.int32) & -65536).view(torch.float32)
+    mid = ((x - high).view(torch.int32) & -65536).view(torch.float32)
+    off = (x.double() - high.double() - mid.double()).abs() / (R.U * x.double().abs())
+    assert (off > 7).double().mean() > 0.9
+    assert torch.equal((x - high - mid).to(torch.bfloat16).float(), x - high - mid)   # and the third part is all of the rest
+
+
 def digit_values(x, sets):
     """x [K] as the sum of `sets` fixed-point numbers of steps 2^(e - 29 - 31 j), 2^e the largest entry's
     power of two, in 64 bits where each number and its remainder are exact."""

@@ -848,3 +848,48 @@ def test_rms_norm_backward_many_short_strided_rows(mt, K, how):
     assert R.worst(host(dx) - want, mag) <= 50
     assert R.worst(host(dgamma) - want_g, mag_g) <= rows + 3
     assert torch.equal(mt.rms_norm_backward(dyd, h.cuda(), gd, rstd.cuda(), need_dgamma=False)[0], dx)
+
+
+# ---- no part of a float is lost, by every way through the products ------------------------
+# Sums over thousands of terms may be off by so much that a lost third part (2^-16 of an operand)
+# would pass. Here every sum has one term, at a place that differs from sum to sum.
+
+@pytest.mark.parametrize("M,K,N,cut", [(130, 260, 200, "bn=128 whole=4 splits=1"), (1100, 70, 90, "bn=128 whole=0 splits=9"),
+                                       (300, 5000, 4100, "bn=256 whole=340 splits=1"), (700, 2100, 2300, "bn=256 whole=74 splits=6")])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_linear_weight_grad_q8_keeps_every_bit_by_every_cut(mt, M, K, N, cut, fmt):
+    """dY with one value per column: the third and the second part meet in an accumulator, then the
+    first, each sum truncated (2 u); zeros are added after that."""
+    q, dy = wgrad_input(gen(M + N), M, K, N, fmt, mt)
+    at, n = (torch.arange(N) * 37 + 5) % M, torch.arange(N)
+    one = torch.zeros(M, N)
+    one[at, n] = dy[at, n]
+    dW, db = mt.linear_weight_grad_q8(q, one.cuda())
+    assert mt.engine.last_path().endswith(cut)
+    want = host(mt.dequantize_q8(q)).double()[at].t() * one[at, n].double()
+    assert R.worst(host(dW) - want, want) <= 3
+    assert torch.equal(host(db)[0], one[at, n])
+
+
+def one_value_rows(g, M, K):
+    x = torch.zeros(M, K)
+    x[torch.arange(M), (torch.arange(M) * 37 + 5) % K] = rand(g, M) * torch.exp(5 * rand(g, M))
+    return x
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N,cut", [(200, 300, 300, "bn=128 whole=4 splits=1"), (500, 1300, 4800, "bn=128 whole=74 splits=11"),
+                                       (1030, 700, 2600, "bn=256 whole=55 splits=1"), (200, 4000, 4097, "bn=256 whole=0 splits=4"),
+                                       (9, 1111, 401, "batch"), (21, 4000, 700, "batch"), (40, 300, 20000, "batch"),
+                                       (64, 1111, 401, "batch"), (150, 4000, 700, "batch")])
+def test_linear_forward_q4_keeps_every_bit_by_every_cut(mt, M, K, N, cut, group):
+    """Rows of x with one value: as above, and the product with the scale."""
+    g = gen(M + K + N + group)
+    _, codes, s = q4_case(g, 1, K, N, group)
+    x = one_value_rows(g, M, K)
+    w = mt.Q4Weight(pack_fast(codes, K).cuda(), s.cuda(), K, group)
+    y = host(mt.linear_forward_q4(x.cuda(), w))
+    assert cut in mt.engine.last_path()
+    at = x.abs().argmax(1)
+    want = x[torch.arange(M), at].double()[:, None] * R.q4_weight(codes, s, group)[at]
+    assert R.worst(y - want, want) <= 7
