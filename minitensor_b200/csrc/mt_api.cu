@@ -2277,7 +2277,6 @@ void set_path(const char* path) {
     }
 }
 int sm_count() { return std::max(1, dev_info().sms); }   // a machine without a GPU gets as far as its first CUDA call
-int device_cc() { return dev_info().cc; }
 int scratch_alloc(void** p, size_t bytes, cudaStream_t st, const char* who) { return ::scratch_alloc(p, bytes, st, who); }
 void scratch_free(void* p, size_t bytes, cudaStream_t st) { ::scratch_free(p, bytes, st); }
 bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* d, const uint64_t* s, const uint32_t* b) {

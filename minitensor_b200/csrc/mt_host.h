@@ -18,8 +18,6 @@ int cuda_fail(cudaError_t e, const char* what);
 int launched(const char* what);
 void set_path(const char* path);
 int sm_count();
-// Compute capability of the current device, major * 10 + minor.
-int device_cc();
 int scratch_alloc(void** p, size_t bytes, cudaStream_t st, const char* who);
 void scratch_free(void* p, size_t bytes, cudaStream_t st);
 // cuTensorMapEncodeTiled for a 2-D or 3-D map of bfloat16 elements with 128-byte swizzle:

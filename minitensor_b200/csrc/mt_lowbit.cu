@@ -23,7 +23,7 @@ using mt::lowbit::Q8;
 
 constexpr int64_t kMaxExtent = INT32_MAX - 4096;   // rows or features of one operand
 
-// A checked 2-D view; is1d: a vector, as one row.
+// A checked 2-D view, or a vector as one row.
 struct View2 {
     Mat m{nullptr, 0, 0};
     int64_t rows = 0, cols = 0;
