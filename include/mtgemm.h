@@ -230,8 +230,8 @@ typedef struct mt_q4 {
  * 8 bits. x, residual, h, y are [rows, features] views, gamma [features], rstd [rows].
  * residual, h, y, rstd and q8 may each be NULL (h then is x, or is not written). h may be the
  * very view that x or residual is (the addition in place), and so may y; of q8, `format`
- * says what to write. eps >= 0. Statistics are float: a row whose squares overflow (a magnitude
- * from about 2^63 on) has rstd 0. */
+ * says what to write. eps >= 0. Statistics are float: a row whose sum of squares is beyond a
+ * float's range (one magnitude of 2^64, or all of 2^64 / sqrt(features)) has rstd 0. */
 MT_API int mt_rms_norm(const mt_tensor* x, const mt_tensor* residual, const mt_tensor* gamma, const mt_tensor* h,
                        const mt_tensor* y, const mt_tensor* rstd, const mt_q8* q8, float eps, void* stream);
 

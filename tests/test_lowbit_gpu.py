@@ -893,3 +893,13 @@ def test_linear_forward_q4_keeps_every_bit_by_every_cut(mt, M, K, N, cut, group)
     at = x.abs().argmax(1)
     want = x[torch.arange(M), at].double()[:, None] * R.q4_weight(codes, s, group)[at]
     assert R.worst(y - want, want) <= 7
+
+
+@pytest.mark.parametrize("K", [64, 4096, 20000])
+def test_rms_norm_range_of_its_statistics(mt, K):
+    """Rows up to where the sum of squares is beyond a float's range, and past it."""
+    top = 2.0 ** 63.9 / K ** 0.5
+    x = torch.stack([torch.full((K,), top), torch.full((K,), 1.1 * 2.0 ** 64 / K ** 0.5)])
+    out = mt.rms_norm(x.cuda(), torch.ones(K, device="cuda"))
+    assert R.worst(host(out.rstd[:1]) - 1 / x[0, 0].double(), 1 / x[0, :1].double()) <= norm_bound(K)
+    assert float(out.rstd[1]) == 0 and torch.equal(host(out.y[1]), torch.zeros(K))
