@@ -202,7 +202,8 @@ enum { MT_Q8_INT8 = 0, MT_Q8_E4M3 = 1 };
 
 /* A rows x cols tensor in 8 bits. Blocks of 32 columns of a row (the last one shorter) share
  * a scale byte b; a code c (int8, or an e4m3 float) stands for c * 2^(b - 127), and b = 255
- * for NaN. Codes and scales have unit column stride. */
+ * for NaN. (Codes of the caller's own may stand for more than a float holds: that is an infinity,
+ * and NaN in a product.) Codes and scales have unit column stride. */
 typedef struct mt_q8 {
     void* codes;          /* code (r, c) at codes + r * code_pitch + c */
     uint8_t* scales;      /* scale of block j of row r at scales + r * scale_pitch + j */
@@ -255,7 +256,8 @@ MT_API int mt_dequantize_q8(const mt_q8* q, void* out, int type, uint64_t pitch,
 
 /* Linear's weight and bias gradient with its input X [M, in] held in 8 bits: dW [in, out] =
  * X^T dY and db [out] or [1, out] = the column sums of dY (NULL: not wanted), to the accuracy
- * of a float product (there is no TF32 form). */
+ * of a float product (there is no TF32 form). In dW, entries of dY below 2^-110 in magnitude count
+ * to a multiple of 2^-133. */
 MT_API int mt_linear_wgrad_q8(const mt_q8* x, const mt_tensor* dY, const mt_tensor* dW, const mt_tensor* db,
                               void* stream);
 
@@ -264,7 +266,9 @@ MT_API int mt_quantize_q4(const mt_tensor* W, const mt_q4* q, void* stream);
 MT_API int mt_dequantize_q4(const mt_q4* q, const mt_tensor* W, void* stream);
 
 /* Y [M, out] = X [M, in] * W + bias (+ReLU) as mt_linear_fwd_gpu, W in 4 bits; to the accuracy
- * of a float product. */
+ * of a float product: each entry of X counts in full, whatever the entries beside it are. Only
+ * from 5 rows on (fewer, where in is above 10,000) entries below 2^-110 in magnitude count to a
+ * multiple of 2^-133. */
 MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor* bias, const mt_tensor* Y, int relu,
                             void* stream);
 

@@ -10,8 +10,9 @@ counterpart there. Three operators around ``Linear<float>`` (include/Module.hpp:
 * ``quantize_q4`` / ``linear_forward_q4``: Linear with 4-bit weights and group scales, from
   one decoded token to whole prompts.
 
-Activations, gradients and results are float32, computed to the accuracy of a float product;
-there is no TF32 form. Like the rest of the package the functions check their arguments
+Activations, gradients and results are float32, computed to the accuracy of a float product
+(entries below 2^-110 to a multiple of 2^-133, include/mtgemm.h has where); there is no TF32 form.
+Like the rest of the package the functions check their arguments
 (``ValueError``), launch on ``stream`` (default: torch's current stream of the operands'
 device) without synchronising, and raise ``RuntimeError`` on CUDA failures. All operands
 are on one device, which need not be the current one. With ``stream`` given, results are

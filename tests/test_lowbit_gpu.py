@@ -903,3 +903,26 @@ def test_rms_norm_range_of_its_statistics(mt, K):
     out = mt.rms_norm(x.cuda(), torch.ones(K, device="cuda"))
     assert R.worst(host(out.rstd[:1]) - 1 / x[0, 0].double(), 1 / x[0, :1].double()) <= norm_bound(K)
     assert float(out.rstd[1]) == 0 and torch.equal(host(out.y[1]), torch.zeros(K))
+
+
+@pytest.mark.parametrize("e", [-105, -112, -118, -125])
+def test_products_of_tiny_entries(mt, e):
+    """One term per sum, entries around 2^e: what their third part cannot hold is below 2^-133 each, and an
+    accumulator of y / 2048 rounds to a multiple of 2^-138 where y is that small."""
+    g, K, N, group = gen(-e), 300, 200, 64
+    _, codes, s = q4_case(g, 1, K, N, group)
+    W = R.q4_weight(codes, s, group)
+    w = mt.Q4Weight(pack_fast(codes, K).cuda(), s.cuda(), K, group)
+    for M in (5, 40, 200):
+        x, at = torch.zeros(M, K), (torch.arange(M) * 37 + 5) % K
+        x[torch.arange(M), at] = torch.ldexp(torch.rand(M, generator=g) + 1, torch.tensor(e))
+        want = x.double() @ W
+        err = (host(mt.linear_forward_q4(x.cuda(), w)).double() - want).abs()
+        assert R.worst((err - 2.0 ** -133 * W[at].abs() - 4 * 2.0 ** -138).clamp_min(0), want) <= 7
+    q, dy = mt.quantize_q8(rand(g, 200, 300).cuda()), torch.zeros(200, 130)
+    at = (torch.arange(130) * 37 + 5) % 200
+    dy[at, torch.arange(130)] = torch.ldexp(torch.rand(130, generator=g) + 1, torch.tensor(e))
+    xv = host(mt.dequantize_q8(q)).double()[at].t()
+    want = xv * dy.sum(0).double()
+    err = (host(mt.linear_weight_grad_q8(q, dy.cuda())[0]).double() - want).abs()
+    assert R.worst((err - 2.0 ** -133 * xv.abs() - 4 * 2.0 ** -149).clamp_min(0), want) <= 3
