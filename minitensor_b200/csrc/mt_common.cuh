@@ -81,14 +81,13 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // Bounded wait on phase `parity`. Returns false (after recording `code`) when the
 // wait ran past kWaitLimitNs or another role of this CTA already gave up (*abort).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-    uint64_t t0 = 0;   // the clock is read from the 256th try on: it takes longer than a short wait
+    if (mbar_try_wait(bar, parity)) return true;
+    uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 1;; ++it) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((it & 255u) == 0) {
             if (*abort_flag) return false;
-            const uint64_t now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            if (now - t0 > kWaitLimitNs) {
+            if (globaltimer_ns() - t0 > kWaitLimitNs) {
                 atomicCAS(&g_dev_status, 0, code);
                 *abort_flag = 1;
                 return false;
@@ -359,14 +358,13 @@ __device__ __forceinline__ bool mbar_try_wait_cl(uint32_t bar, uint32_t parity) 
 }
 // mbar_wait for barriers that the peer CTA (or its TMA / MMA traffic) completes.
 __device__ __forceinline__ bool mbar_wait_cl(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-    uint64_t t0 = 0;   // the clock is read from the 256th try on: it takes longer than a short wait
+    if (mbar_try_wait_cl(bar, parity)) return true;
+    uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 1;; ++it) {
         if (mbar_try_wait_cl(bar, parity)) return true;
         if ((it & 255u) == 0) {
             if (*abort_flag) return false;
-            const uint64_t now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            if (now - t0 > kWaitLimitNs) {
+            if (globaltimer_ns() - t0 > kWaitLimitNs) {
                 atomicCAS(&g_dev_status, 0, code);
                 *abort_flag = 1;
                 return false;
