@@ -267,7 +267,7 @@ MT_API int mt_dequantize_q4(const mt_q4* q, const mt_tensor* W, void* stream);
 
 /* Y [M, out] = X [M, in] * W + bias (+ReLU) as mt_linear_fwd_gpu, W in 4 bits; to the accuracy
  * of a float product: each entry of X counts in full, whatever the entries beside it are. Only
- * from 5 rows on (fewer, where in is above 10,000) entries below 2^-110 in magnitude count to a
+ * from 5 rows on (fewer, where in is above 9,000) entries below 2^-110 in magnitude count to a
  * multiple of 2^-133. */
 MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor* bias, const mt_tensor* Y, int relu,
                             void* stream);

@@ -43,7 +43,9 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+// The error is reported here, and not once more by the check of the next launch.
 int cuda_fail(cudaError_t e, const char* what) {
+    cudaGetLastError();
     return fail(MT_ECUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
@@ -2263,7 +2265,7 @@ int fail(int code, const char* fmt, ...) {
     }
     return code;
 }
-int cuda_fail(cudaError_t e, const char* what) { return fail(MT_ECUDA, "%s: %s", what, cudaGetErrorString(e)); }
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
 int launched(const char* what) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess && e != cudaErrorStreamCaptureUnsupported) return cuda_fail(e, what);

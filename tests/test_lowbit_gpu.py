@@ -926,3 +926,17 @@ def test_products_of_tiny_entries(mt, e):
     want = xv * dy.sum(0).double()
     err = (host(mt.linear_weight_grad_q8(q, dy.cuda())[0]).double() - want).abs()
     assert R.worst((err - 2.0 ** -133 * xv.abs() - 4 * 2.0 ** -149).clamp_min(0), want) <= 3
+
+
+def test_calls_behind_one_that_found_no_memory(mt):
+    """Scratch of 400 GB is refused by an error of that call; the calls behind it, torch's among them, do
+    not meet it again."""
+    q = mt.quantize_q8(torch.ones(2 ** 20, 1, device="cuda"))
+    dY = torch.ones(1, 1, device="cuda").expand(2 ** 20, 2 ** 16)
+    for again in (lambda: mt.quantize_q8(torch.ones(4, 64, device="cuda")).codes, lambda: torch.ones(4, device="cuda") + 1,
+                  lambda: mt.matmul(torch.ones(64, 64, device="cuda"), torch.ones(64, 64, device="cuda")),
+                  lambda: mt.linear_weight_grad_q8(q, dY[:, :8])[0]):
+        with pytest.raises(RuntimeError, match="memory"):
+            mt.linear_weight_grad_q8(q, dY)
+        again()
+    torch.cuda.synchronize()
