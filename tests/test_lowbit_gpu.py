@@ -940,3 +940,22 @@ def test_calls_behind_one_that_found_no_memory(mt):
             mt.linear_weight_grad_q8(q, dY)
         again()
     torch.cuda.synchronize()
+
+
+def test_linear_forward_q4_passes_follow_the_values_at_replay(mt):
+    """How often few rows go through the weights is decided by x on the GPU: a captured call follows x,
+    and equal calls give equal bits."""
+    g, K, N = gen(41), 1000, 77
+    for M in (1, 3):
+        spread, codes, s = ladder(g, M, K, N, 64, -80, 120)
+        w = mt.Q4Weight(pack_fast(codes, K).cuda(), s.cuda(), K, 64)
+        inputs = [spread.cuda(), rand(g, M, K).cuda(), torch.zeros(M, K, device="cuda"), spread.cuda() * 0.5]
+        want = [mt.linear_forward_q4(x, w) for x in inputs]
+        x = inputs[1].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = mt.linear_forward_q4(x, w)
+        for v, expected in zip(inputs * 2, want * 2):
+            x.copy_(v)
+            graph.replay()
+            assert torch.equal(y, expected)
