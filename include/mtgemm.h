@@ -266,9 +266,9 @@ MT_API int mt_quantize_q4(const mt_tensor* W, const mt_q4* q, void* stream);
 MT_API int mt_dequantize_q4(const mt_q4* q, const mt_tensor* W, void* stream);
 
 /* Y [M, out] = X [M, in] * W + bias (+ReLU) as mt_linear_fwd_gpu, W in 4 bits; to the accuracy
- * of a float product: each entry of X counts in full, whatever the entries beside it are. Only
- * from 5 rows on (fewer, where in is above 9,000) entries below 2^-110 in magnitude count to a
- * multiple of 2^-133. */
+ * of a float product: each entry of X counts, whatever the entries beside it are. Entries below
+ * 2^-110 in magnitude count to a multiple of 2^-133, but in full for up to 4 rows of up to 9,000
+ * inputs. */
 MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor* bias, const mt_tensor* Y, int relu,
                             void* stream);
 

@@ -904,9 +904,12 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Few rows in integers, batches with the weights in tensor memory, prompts as a product of
     // unpacked operands. Microseconds, either side: 192 rows on weights of 4096 x 16384 (group 64) 96
-    // and 109, 256 rows 138 and 109; 4 rows there 27 and 31, 5 rows 35 and 31. In two launches: 1 row on
-    // 20000 x 16384 63 and 86, 2 rows on 16384 x 4096 36 and 31, but 56 and 101 on 12000 x 16384 in
-    // groups of 32, which cost a batch twice the drains. In three: 1 row on 30000 x 4096 58 and 45.
+    // and 109, 256 rows 138 and 109; 4 rows there 27 and 31, 5 rows 35 and 31. 5 to 8 rows take the
+    // weights twice, which on small ones costs less than a batch's further launches: 8 rows in a row of
+    // calls on 4096 x 4096 16.5 and 18.4, on 4096 x 6000 17.0 and 18.2, on 4096 x 11008 24.7 and 21.2.
+    // In two launches: 1 row on 20000 x 16384 63 and 86, 2 rows on 16384 x 4096 36 and 31, but 56 and
+    // 101 on 12000 x 16384 in groups of 32, which cost a batch twice the drains. In three: 1 row on
+    // 30000 x 4096 58 and 45.
     if (M > 192 && w.K > 0) {
         switch (w.group) {   // k16-steps per group
             case 32: return linear_q4_planes<2>(vx, w, vb.m.p, vy.m, M, relu, st, who);
@@ -914,8 +917,9 @@ MT_API int mt_linear_fwd_q4(const mt_tensor* X, const mt_q4* W, const mt_tensor*
             default: return linear_q4_planes<8>(vx, w, vb.m.p, vy.m, M, relu, st, who);
         }
     }
+    const int64_t few = w.K * w.N <= 24 << 20 ? 2 * mt::q4::kGemvMaxRows : mt::q4::kGemvMaxRows;
     const int64_t spans = (w.K + mt::q4::kSpan - 1) / mt::q4::kSpan;
-    if (w.K > 0 && (M > mt::q4::kGemvMaxRows || plan_gemv(M, spans).launches > (M == 1 || w.group == 32 ? 2 : 1)))
+    if (w.K > 0 && (M > few || plan_gemv(M, spans).launches > (M == 1 || w.group == 32 ? 2 : 1)))
         return linear_q4_batch(vx, w, vb.m.p, vy.m, M, relu, st, who);
     return linear_q4_gemv(vx, w, vb.m.p, vy.m, M, relu, st, who);
 }
