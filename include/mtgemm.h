@@ -30,8 +30,9 @@
  *       . the conv weight gradient, stated below (mt_conv2d_wgrad can take a caller
  *         workspace, mt_conv2d_wgrad_noalloc a fixed library array);
  *       . mt_matmul_host without a workspace: the device copies of A, B and C;
- *       . mt_rms_norm_backward (partial sums of dgamma), mt_linear_wgrad_q8 and, from 9 rows of
- *         X on, mt_linear_fwd_q4 (bfloat16 forms of the operands, partial tiles).
+ *       . mt_rms_norm_backward (partial sums of dgamma), mt_linear_wgrad_q8 and, from 5 rows of
+ *         X on (9 on up to 25 million weights, fewer where `in` is above 9,000),
+ *         mt_linear_fwd_q4 (bfloat16 forms of the operands, partial tiles).
  *     Strict-fp32 calls and every other path allocate nothing.
  *   - Every function returns an mt_status and never throws; mt_last_error() gives the
  *     thread-local message of the last failure.

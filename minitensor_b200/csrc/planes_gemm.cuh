@@ -31,7 +31,8 @@
 // seems to cost the L1 with the scales in it at every chunk: groups of 32, 2048 x 4096 x 8192 379
 // against 337 us, 2048 x 5376 x 1536 168 against 128 us.
 // Bound: tensor pipe, 3 * 2 R C K operations: 8192^3 in 1956 us, 1686 TFLOP/s of bfloat16 work,
-// 1.01 of the measured cuBLAS rate (one launch; 2.25 ms in a row, under the power cap).
+// 1.01 of the measured cuBLAS rate (one launch at full clock; a few after one another 2075 us, in a
+// row 2.25 to 2.4 ms, under the power cap).
 // Three 64-deep stages, because 64 KB a stage leave room for no fourth; 256 x 256 tiles, because
 // a CTA alone on 128 x 256 would move 112 KB through shared memory in the time that bandwidth
 // has for 190 KB of reads and writes, of which the MMAs' reads alone are 144 KB.
