@@ -187,9 +187,11 @@ __device__ __forceinline__ int gemv_stage_x(const Gemv& p, uint8_t* xs, float* f
                     *reinterpret_cast<uint32_t*>(o + 3 * (size_t)col_bytes) = __byte_perm(h0, h1, 0x7632);
                     o += 4 * (size_t)col_bytes;
                 }
-                // 2^14 times the span's unit: sums in the unit itself would fall below a float's normal
-                // numbers where y does not, and with 2^16 the low digits' could overflow first.
-                if (lane == 0) fs[r * (spans + 1) + s] = __uint_as_float((uint32_t)max(e - 19 - 62 * max(pass - 1, 0), 1) << 23);
+                // 2^30 times the span's unit. 2^16 of it come off the scales, whose products with the sums
+                // of digits would overflow from 2^98 on (2^-16 of the least bfloat16 is a float still). With
+                // the rest, sums do not fall below a float's normal numbers where y does not; with 2^16
+                // for 2^14 the low digits' could overflow first.
+                if (lane == 0) fs[r * (spans + 1) + s] = __uint_as_float((uint32_t)max(e - 3 - 62 * max(pass - 1, 0), 1) << 23);
             }
         }
     }
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
                 const uint8_t* xl = xs + (size_t)g * col_bytes + t * 32;
                 const uint4* w = ring;
                 // A lane's digits: 2^16 for the high ones, 2^-31 for the second number, 2^-62 for later passes;
-                // and 2^-14 for what the spans' powers of two have too much.
+                // and 2^-14 for what the spans' powers of two still have too much.
                 const float weight = (t & 1 ? 4.f : 0x1p-14f) * (t & 2 ? 0x1p-31f : 1.f) * (pass ? 0x1p-62f : 1.f);
 #pragma unroll 1
                 for (int i = lo; i < hi; ++i) {
@@ -337,8 +339,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) gemv_kernel(const Gemv p) {
                         float fa[SEG], fb[SEG];
 #pragma unroll
                         for (int k = 0; k < SEG; ++k) {
-                            fa[k] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)ca[k], (lane & 28) + j) << 16);
-                            fb[k] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)cb[k], (lane & 28) + j) << 16);
+                            fa[k] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)ca[k], (lane & 28) + j) << 16) * 0x1p-16f;
+                            fb[k] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)cb[k], (lane & 28) + j) << 16) * 0x1p-16f;
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {

@@ -959,3 +959,17 @@ def test_linear_forward_q4_passes_follow_the_values_at_replay(mt):
             x.copy_(v)
             graph.replay()
             assert torch.equal(y, expected)
+
+
+@pytest.mark.parametrize("scale,e", [(-133, 120), (-126, 30), (60, -40), (97, -60), (105, -90), (112, -20)])
+@pytest.mark.parametrize("M", [1, 4, 9, 200])
+def test_linear_forward_q4_scales_of_any_size(mt, M, scale, e):
+    """Scales from the least bfloat16 to 2^113, whose products with x are ordinary floats."""
+    g, K, N, group = gen(scale + 200), 300, 40, 128
+    codes = torch.randint(0, 16, (N, K), generator=g)
+    s = torch.ldexp(1 + torch.rand(N, 3, generator=g), torch.tensor(scale)).to(torch.bfloat16)
+    x = torch.ldexp(rand(g, M, K), torch.tensor(e))
+    w = mt.Q4Weight(R.q4_pack(codes, K).cuda(), s.cuda(), K, group)
+    W = R.q4_weight(codes, s, group)
+    err = host(mt.linear_forward_q4(x.cuda(), w)).double() - x.double() @ W
+    assert R.worst(err, x.double().abs() @ W.abs()) <= R.q4_bound(M, K, group)
