@@ -973,3 +973,22 @@ def test_linear_forward_q4_scales_of_any_size(mt, M, scale, e):
     W = R.q4_weight(codes, s, group)
     err = host(mt.linear_forward_q4(x.cuda(), w)).double() - x.double() @ W
     assert R.worst(err, x.double().abs() @ W.abs()) <= R.q4_bound(M, K, group)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N,path", [(1, 45000, 130, "batch"), (2, 22000, 300, "batch"), (3, 23000, 17, "batch"), (4, 20000, 70, "batch"),
+                                        (8, 20000, 130, "batch"), (5, 5000, 6000, "batch"), (1, 11000, 40, "gemv rows=1 x 1"),
+                                        (3, 9000, 33, "gemv rows=2 x 2"), (4, 5000, 33, "gemv rows=2 x 2"), (7, 5000, 33, "gemv rows=3 x 3"),
+                                        (4, 4500, 33, "gemv rows=4 x 1"), (7, 4500, 33, "gemv rows=4 x 2"), (8, 9000, 33, "gemv rows=2 x 4")])
+def test_linear_forward_q4_few_long_rows(mt, M, K, N, path, group):
+    """Either side of the rows and lengths at which few rows become a batch, and rows that share a CTA by
+    four, three or two (four rows of 5000 inputs take 242,944 bytes of shared memory, 232,448 are there)."""
+    g = gen(M + K)
+    x, codes, s = ladder(g, M, K, N, group, -30, 20)
+    bias = rand(g, N) * 2.0 ** 10
+    w = mt.Q4Weight(pack_fast(codes, K).cuda(), s.cuda(), K, group)
+    y = host(mt.linear_forward_q4(x.cuda(), w, bias=bias.cuda())).double()
+    assert path in mt.engine.last_path()
+    W = R.q4_weight(codes, s, group)
+    err, mag = y - x.double() @ W - bias.double(), x.double().abs() @ W.abs() + bias.double().abs()
+    assert R.worst(err, mag) <= R.q4_bound(M, K, group)
